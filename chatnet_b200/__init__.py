@@ -21,7 +21,7 @@ from ._native import (CudaError, NotSupportedError, TYPE_F16, TYPE_F32, TYPE_Q4_
                       DIST_NORM_W, check, byte_size)
 
 __all__ = [
-    "Context", "Tensor", "CudaError", "NotSupportedError", "check", "byte_size", "synth_fill",
+    "Context", "Tensor", "KvQ4Cache", "CudaError", "NotSupportedError", "check", "byte_size", "synth_fill",
     "synth_seed", "device_count", "TYPE_F32", "TYPE_F16", "TYPE_Q4_0", "TYPE_Q4_K", "TYPE_Q6_K",
     "TYPE_Q4_1", "TYPE_Q5_0", "TYPE_Q5_1", "TYPE_Q8_0", "TYPE_Q2_K", "TYPE_Q3_K", "TYPE_Q5_K", "TYPE_Q8_K",
     "TYPE_IQ4_NL", "TYPE_IQ4_XS", "TYPE_IQ2_XXS", "TYPE_IQ2_XS", "TYPE_IQ3_XXS", "TYPE_IQ1_S", "TYPE_IQ3_S",
@@ -90,6 +90,18 @@ class Tensor:
             self.free()
         except Exception:
             pass
+
+
+class KvQ4Cache:
+    """One layer's 4-bit KV cache in the caller's device memory (cn_kvq4): the device addresses of its
+    quants [n_seqs][n_kv_heads][ctx_len][head_dim/2] bytes and scales [n_seqs][n_kv_heads][ctx_len][head_dim/32] fp16."""
+
+    def __init__(self, k_quants: int, k_scales: int, v_quants: int, v_scales: int, n_seqs: int, n_kv_heads: int,
+                 head_dim: int, ctx_len: int, seq_rows: int = 0):
+        self.n_kv_heads, self.head_dim, self.ctx_len = n_kv_heads, head_dim, ctx_len
+        self.kv_dim = n_kv_heads * head_dim
+        self._c = N.KvQ4C(k_quants, k_scales, v_quants, v_scales, n_seqs, n_kv_heads, head_dim, ctx_len, seq_rows)
+        self._ref = C.byref(self._c)
 
 
 class Context:
@@ -183,6 +195,46 @@ class Context:
         check(N.lib().cn_sample_dev(self.handle, C.c_void_p(d_logits), vocab, batch, float(temperature),
                                     int(top_k), float(top_p), rr.ctypes.data, out.ctypes.data), "cn_sample_dev")
         return out
+
+    # Device addresses (int) throughout; stream = a cudaStream_t (0: the legacy default stream).
+
+    def kvq4_append_dev(self, cache: KvQ4Cache, k: int, v: int, pos: int, batch: int, n_new: int = 1, *,
+                        count: int = 0, kv_stride: int = 0, rope: int = 0, rope_neox: bool = False,
+                        stream: int = 0) -> None:
+        """Stores the new tokens' k and v rows in the 4-bit cache (cn_kvq4_append_dev)."""
+        rc = N.lib().cn_kvq4_append_dev(self.handle, cache._ref, k, v, kv_stride or cache.kv_dim, pos, count, batch,
+                                        n_new, rope, int(rope_neox), stream)
+        if rc:
+            check(rc, "cn_kvq4_append_dev")
+
+    def kvq4_attend_dev(self, cache: KvQ4Cache, q: int, out: int, pos: int, batch: int, n_heads: int, *,
+                        n_new: int = 1, count: int = 0, q_stride: int = 0, out_stride: int = 0,
+                        scale: float | None = None, rope: int = 0, rope_neox: bool = False, stream: int = 0) -> None:
+        """Causal attention of the new tokens over the 4-bit cache (cn_kvq4_attend_dev); scale: 1/sqrt(head_dim)."""
+        width = n_heads * cache.head_dim
+        rc = N.lib().cn_kvq4_attend_dev(self.handle, cache._ref, q, q_stride or width, out, out_stride or width, pos,
+                                        count, batch, n_new, n_heads,
+                                        cache.head_dim ** -0.5 if scale is None else scale, rope, int(rope_neox),
+                                        stream)
+        if rc:
+            check(rc, "cn_kvq4_attend_dev")
+
+    def kvq4_read_dev(self, cache: KvQ4Cache, k: int, v: int, pos: int, batch: int, n_new: int = 1, *,
+                      count: int = 0, kv_stride: int = 0, stream: int = 0) -> None:
+        """Reads cache rows back as fp32 values (cn_kvq4_read_dev); k or v may be 0."""
+        rc = N.lib().cn_kvq4_read_dev(self.handle, cache._ref, k, v, kv_stride or cache.kv_dim, pos, count, batch,
+                                      n_new, stream)
+        if rc:
+            check(rc, "cn_kvq4_read_dev")
+
+    def logprobs_dev(self, logits: int, rows: int, vocab: int, tokens: int = 0, logprob: int = 0, entropy: int = 0,
+                     top_n: int = 0, top_ids: int = 0, top_logprobs: int = 0, *, row_stride: int = 0,
+                     type_: int = TYPE_F32, stream: int = 0) -> None:
+        """Log probabilities of tokens, entropies and the top_n alternatives of rows of logits (cn_logprobs_dev)."""
+        rc = N.lib().cn_logprobs_dev(self.handle, type_, logits, row_stride or vocab, rows, vocab, tokens, top_n,
+                                     logprob, entropy, top_ids, top_logprobs, stream)
+        if rc:
+            check(rc, "cn_logprobs_dev")
 
     def close(self) -> None:
         if self.handle:

@@ -140,6 +140,10 @@ SIGNATURES: dict[str, tuple] = {
     "cn_tp_destroy": (_i, [_vp]),
     "cn_llama_create_tp": (_i, [_vp, _vp, C.POINTER(_vp), _i, _vp, C.POINTER(_vp)]),
     "cn_llama_prepare": (_i, [_vp, _i]),
+    "cn_kvq4_append_dev": (_i, [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _i, _i, _vp, _i, _vp]),
+    "cn_kvq4_attend_dev": (_i, [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i, _i, _i, _f, _vp, _i, _vp]),
+    "cn_kvq4_read_dev": (_i, [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _i, _i, _vp]),
+    "cn_logprobs_dev": (_i, [_vp, _i, _vp, _i64, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp]),
 }
 
 TP_HANDLE_BYTES = 64
@@ -154,6 +158,13 @@ class LlamaConfigC(C.Structure):
                 ("n_kv_heads", _i), ("head_dim", _i), ("vocab", _i), ("ctx_len", _i),
                 ("rope_base", _f), ("rms_eps", _f), ("kv_dtype", _i), ("max_batch", _i),
                 ("rope_neox", _i), ("act_gelu", _i), ("norm_offset", _i)]
+
+
+class KvQ4C(C.Structure):
+    """cn_kvq4 (include/chatnet_cuda.h)."""
+    _fields_ = [("k_quants", _vp), ("k_scales", _vp), ("v_quants", _vp), ("v_scales", _vp), ("n_seqs", _i),
+                ("n_kv_heads", _i), ("head_dim", _i), ("ctx_len", _i), ("seq_rows", _i64)]
+
 
 _lib = None
 

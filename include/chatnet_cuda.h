@@ -237,6 +237,81 @@ int cn_matvec_noalloc_dev(int type, const void* d_w, int out_dim, int in_dim, co
  * the allocation-free GEMV) */
 int cn_matvec_noalloc_status(void* stream);
 
+/* ---- 4-bit KV cache ------------------------------------------------------
+ * The keys and values of one layer in 4 bits with an fp16 scale per 32 values
+ * (4.5 bits a value: 0.28 of an fp16 cache, 0.14 of an fp32 one).  A row is
+ * the head_dim values of one (sequence, kv head, position); rows lie
+ * [sequence][kv head][position], each in two arrays, quants [row][head_dim/2]
+ * bytes and scales [row][head_dim/32] fp16.  With nb = head_dim / 32, value
+ * 32 b + 8 i + g of a row (block b, i < 4, g < 8) is the nibble i & 1 (low
+ * first) of byte g * 2 nb + 2 b + (i >> 1) and stands for scale[b] *
+ * (nibble - 8): the values of a GGUF Q4_0 block (DequantQ4_0.cs:42-53), laid
+ * out for the attention's tensor-core fragments.  (no reference counterpart:
+ * LlamaModel keeps its cache in fp32, LlamaModel.cs:60-61)
+ *
+ * Calls work on sequences 0..batch-1 (their slots in the cache), n_new tokens
+ * each: token i of sequence b stands at position d_pos[b] + i.  d_count
+ * (device int[batch], may be NULL) gives how many of its n_new tokens each
+ * sequence has.  A sequence with a negative position or no tokens, and tokens
+ * past the cache's end, are left out: their cache rows and output rows stay
+ * as they were.  Tensors are [batch][n_new] rows of the given stride
+ * (in values).  d_rope (may be NULL) is a [ctx_len][head_dim/2] table of
+ * (cos, sin) as ApplyRoPE uses it (TensorMath.cs:418-470), rope_neox = 1 pairs
+ * (i, i + head_dim/2) (TensorMath.cs:475).  The calls run on ctx's device,
+ * enqueue on `stream` only, allocate nothing and keep nothing between calls,
+ * so they may be captured, replayed and issued from several streams; all
+ * pointers are device pointers. */
+typedef struct {
+    void* k_quants; /* [n_seqs][n_kv_heads][ctx_len][head_dim/2] bytes, 16-byte aligned */
+    void* k_scales; /* [n_seqs][n_kv_heads][ctx_len][head_dim/32] fp16, 16-byte aligned */
+    void* v_quants;
+    void* v_scales;
+    int n_seqs, n_kv_heads;
+    int head_dim;     /* 32, 64, 96, 128 or 256 */
+    int ctx_len;      /* positions per sequence, a multiple of 8 */
+    int64_t seq_rows; /* rows between two sequences (a multiple of 8); 0: n_kv_heads * ctx_len */
+} cn_kvq4;
+
+/* Stores the new tokens' k and v rows (fp32, n_kv_heads * head_dim values at
+ * stride kv_stride), k rotated first when d_rope is given.  Per block: values
+ * limited to +-524032 (NaN as 0), scale = fp16(-m / 8) with m the value of
+ * largest magnitude (the negative one of a tie), then the nearest level,
+ * halves up. */
+int cn_kvq4_append_dev(cn_ctx* ctx, const cn_kvq4* cache, const float* d_k, const float* d_v, int64_t kv_stride,
+                       const int* d_pos, const int* d_count, int batch, int n_new, const float* d_rope, int rope_neox,
+                       void* stream);
+/* Causal attention of the new tokens over the cache (their own rows included:
+ * append first): out[b][i][h] = softmax(scale * q . k_p over p <= d_pos[b] + i)
+ * . v_p, query head h on kv head h / (n_heads / n_kv_heads) (ComputeAttention +
+ * Softmax, LlamaModel.cs:241-346).  q (rotated first when d_rope is given) and
+ * out: n_heads * head_dim fp32 values per token, 16-byte aligned, strides
+ * multiples of 4, not overlapping.  fp32 results (products of q and of the
+ * softmax weights carry 22 bits, sums 24). */
+int cn_kvq4_attend_dev(cn_ctx* ctx, const cn_kvq4* cache, const float* d_q, int64_t q_stride, float* d_out,
+                       int64_t out_stride, const int* d_pos, const int* d_count, int batch, int n_new, int n_heads,
+                       float scale, const float* d_rope, int rope_neox, void* stream);
+/* Reads rows back as fp32 values (d_k or d_v may be NULL). */
+int cn_kvq4_read_dev(cn_ctx* ctx, const cn_kvq4* cache, float* d_k, float* d_v, int64_t kv_stride, const int* d_pos,
+                     const int* d_count, int batch, int n_new, void* stream);
+
+/* ---- log probabilities -----------------------------------------------------
+ * For each of `rows` rows of logits (type CN_TYPE_F32 or CN_TYPE_F16, vocab
+ * values at stride row_stride): the log probability (natural, of the softmax
+ * at temperature 1) of token d_tokens[row] -> d_logprob[row]; the
+ * distribution's entropy in nats -> d_entropy[row]; the top_n (0..64) most
+ * likely tokens, ties to the lower id, -> d_top_ids [rows][top_n] and their
+ * log probabilities -> d_top_logprobs [rows][top_n].  Tokens and d_logprob go
+ * together; each output but d_top_ids (with top_n > 0) may be NULL.  A token
+ * outside [0, vocab) gets NaN.  -inf logits (banned tokens) have probability
+ * 0; a row that holds a NaN or +inf, or nothing but -inf, has no distribution:
+ * its results are NaN (its alternatives still in order, NaN last).  Enqueues
+ * on `stream` only, allocates nothing, keeps nothing between calls.  (no
+ * reference counterpart: TemperatureSampler discards its probabilities,
+ * Samplers/TemperatureSampler.cs:33-113) */
+int cn_logprobs_dev(cn_ctx* ctx, int type, const void* d_logits, int64_t row_stride, int rows, int vocab,
+                    const int* d_tokens, int top_n, float* d_logprob, float* d_entropy, int* d_top_ids,
+                    float* d_top_logprobs, void* stream);
+
 /* ---- model level: one Llama decoder resident on the device ------------- */
 
 typedef struct cn_llama cn_llama;
