@@ -3,95 +3,515 @@
 //   o = sum_p w_p v_p / sum_p w_p,  w_p = exp(scale (q . k_p) - max)
 // over positions p = 0 .. pos[b] + i of token i, with one pass over the cache
 // (running maximum and sum, fp32).
+//
+// Rows: the queries that read one kv head of one sequence, row r = token
+// r / mul, query head kvh * mul + r % mul (mul = n_heads / n_kv).
+#include <math.h>
+
 #include "kvq4.cuh"
 
 namespace cn {
 
-// One warp per (token, query head): lane (g = lane >> 2, t = lane & 3) holds
-// values 32 b + 8 t + g of every block, i.e. nibble t of the pieces of chunk g.
-template <int NB>
-__global__ void __launch_bounds__(128)
-    kvq4_attend_plain_kernel(const float* __restrict__ q, int64_t q_stride, float* __restrict__ out, int64_t out_stride,
-                             const int* __restrict__ pos, const int* __restrict__ count, int n_new, int n_heads,
-                             int n_kv, int64_t n_rows, float scale, const float2* __restrict__ rope, int neox,
-                             const uint8_t* __restrict__ kq, const __half* __restrict__ kd,
-                             const uint8_t* __restrict__ vq, const __half* __restrict__ vd, int64_t seq_rows,
-                             int ctx_len) {
-    constexpr int HD = 32 * NB;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= n_rows) return;
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int h = (int)(row % n_heads);
-    const int64_t tok = row / n_heads;
-    const int b = (int)(tok / n_new), i = (int)(tok % n_new);
-    int p0;
-    if (i >= kvq4_active(pos, count, b, n_new, ctx_len, p0)) return;
-    const int len = p0 + i + 1;
-    float x[NB], o[NB];
-    const float* qr = q + tok * q_stride + (int64_t)h * HD;
-    const float2* tab = rope + (int64_t)(p0 + i) * (HD / 2);
+struct AttendArgs {
+    const float* q;
+    float* out;
+    int64_t q_stride, out_stride;
+    const int* pos;
+    const int* count;
+    const float2* rope;
+    const uint8_t *kq, *vq;
+    const __half *kd, *vd;
+    int64_t seq_rows;
+    int n_new, n_heads, n_kv, ctx_len, neox, groups;
+    float scale;
+    uint32_t* err;
+};
+
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kTile = 32;        // positions a warp takes at a time
+constexpr float kLazy = 8.f;     // a row's reference moves only when the maximum outgrows it by 2^8
+constexpr int kMaxCluster = 16;
+
+__host__ __device__ constexpr int stage_bytes(int nb) { return kTile * 36 * nb; }
+__host__ __device__ constexpr int stages(int nb) { return nb <= 4 ? 4 : 2; }
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+        "l"(src), "r"(bytes), "r"(smem_u32(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr, uint32_t rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(map_rank(addr, rank))
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_rank(addr, rank)) : "memory");
+    return v;
+}
+
+// The halves of hi + lo = x: hi keeps 11 bits (x truncated, so the
+// conversion is exact in fp16's normal range), lo the next 11.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const float ah = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u);
+    const float bh = __uint_as_float(__float_as_uint(b) & 0xFFFFE000u);
+    hi = pack_half2(ah, bh);
+    lo = pack_half2(a - ah, b - bh);
+}
+
+// Rotated query values e, e + 1 (e even) of one row.
+template <int HD>
+__device__ __forceinline__ float2 query_pair(const float* __restrict__ x, const float2* __restrict__ tab, int neox,
+                                             int e) {
+    const float2 a = *reinterpret_cast<const float2*>(x + e);
+    if (!tab) return a;
+    if (!neox) {
+        const float2 cs = tab[e / 2];
+        return make_float2(__fsub_rn(__fmul_rn(a.x, cs.x), __fmul_rn(a.y, cs.y)),
+                           __fadd_rn(__fmul_rn(a.x, cs.y), __fmul_rn(a.y, cs.x)));
+    }
+    constexpr int H = HD / 2;
+    const bool first = e < H;
+    const float2 b = *reinterpret_cast<const float2*>(x + (first ? e + H : e - H));
+    const float4 cs = *reinterpret_cast<const float4*>(tab + (first ? e : e - H));
+    if (first)
+        return make_float2(__fsub_rn(__fmul_rn(a.x, cs.x), __fmul_rn(b.x, cs.y)),
+                           __fsub_rn(__fmul_rn(a.y, cs.z), __fmul_rn(b.y, cs.w)));
+    return make_float2(__fadd_rn(__fmul_rn(b.x, cs.y), __fmul_rn(a.x, cs.x)),
+                       __fadd_rn(__fmul_rn(b.y, cs.w), __fmul_rn(a.y, cs.z)));
+}
+
+// N 32-bit (or 16-bit) words from shared memory with the widest loads the
+// row layout allows.
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t* w, const uint8_t* p) {
+    if constexpr (N % 4 == 0) {
 #pragma unroll
-    for (int j = 0; j < NB; j++) {
-        const int e = 32 * j + 8 * t + g;
-        o[j] = 0.f;
-        if (!rope) {
-            x[j] = qr[e];
-        } else if (neox) {
-            const float2 cs = tab[e % (HD / 2)];
-            x[j] = e < HD / 2 ? __fsub_rn(__fmul_rn(qr[e], cs.x), __fmul_rn(qr[e + HD / 2], cs.y))
-                              : __fadd_rn(__fmul_rn(qr[e - HD / 2], cs.y), __fmul_rn(qr[e], cs.x));
-        } else {
-            const float2 cs = tab[e / 2];
-            x[j] = (e & 1) ? __fadd_rn(__fmul_rn(qr[e - 1], cs.y), __fmul_rn(qr[e], cs.x))
-                           : __fsub_rn(__fmul_rn(qr[e], cs.x), __fmul_rn(qr[e + 1], cs.y));
+        for (int i = 0; i < N / 4; i++) {
+            const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+        }
+    } else if constexpr (N == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w[0] = v.x, w[1] = v.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    }
+}
+// NB 16-bit values: two per word
+template <int NB>
+__device__ __forceinline__ void lds_halves(uint32_t* w, const uint8_t* p) {
+    if constexpr (NB % 2 == 0) {
+        lds_words<NB / 2>(w, p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NB; i += 2)
+            w[i / 2] = (uint32_t) reinterpret_cast<const uint16_t*>(p)[i] |
+                       (i + 1 < NB ? (uint32_t) reinterpret_cast<const uint16_t*>(p)[i + 1] << 16 : 0u);
+    }
+}
+__device__ __forceinline__ float half_at(const uint32_t* w, int b) {
+    const __half2 h = *reinterpret_cast<const __half2*>(&w[b >> 1]);
+    return (b & 1) ? __high2float(h) : __low2float(h);
+}
+// {16-bit piece i of a, piece j of b}
+__device__ __forceinline__ uint32_t pair16(const uint32_t* a, int i, const uint32_t* b, int j) {
+    return __byte_perm(a[i >> 1], b[j >> 1], ((i & 1) ? 0x32u : 0x10u) | ((j & 1) ? 0x7600u : 0x5400u));
+}
+
+}  // namespace
+
+// Few rows against a long cache (decode).  An item is eight rows of one
+// (sequence, kv head); its CTAs form a cluster, and every warp of it takes
+// tiles of 32 positions in turn, each through its own ring of bulk copies, with
+// its own running reference, sum and output.  The partials meet in shared
+// memory, first the CTA's, then the cluster's: no workspace, no atomics, one
+// launch.
+//
+// Scores: S = Q K^T on mma.m16n8k16, the eight rows' high halves in the
+// tile's rows 0-7 and their low halves in rows 8-15 (q scaled to [2^14, 2^15)
+// by a power of two: 22 bits).  K's levels go in as fp16 subnormals, level *
+// 2^-24 straight from the nibble (every second nibble as 16 * level, with q
+// divided by 16 there), so a fragment costs one AND per two values; the
+// -8 of a value is the accumulator's start, -8 sum(q), and the block's scale
+// multiplies the block's sums in fp32.
+// Output: O = W V with w_p d_p,b (weight times the block's scale) split into
+// halves the same way and V's signed levels exact in fp16.
+// A row's reference R (log2 units) is its running maximum plus the exponent of
+// the largest V scale seen, less 6: w d stays below 2^14 and keeps 22 bits down
+// to 2^-18 of it, whatever the cache's range.
+template <int NB>
+__global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows_kernel(const AttendArgs a) {
+    constexpr int HD = 32 * NB, RB = 16 * NB, SB = 2 * NB;  // bytes of a row's quants and scales
+    constexpr int ST = stages(NB), STB = stage_bytes(NB);
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint64_t bars[kWarps][ST];
+    __shared__ float sR[kWarps + 1][8], sL[kWarps + 1][8];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t cs = cluster_size(), rank = cluster_rank();
+    const int item = (int)(blockIdx.x / cs);
+    const int grp = item % a.groups, bh = item / a.groups, kvh = bh % a.n_kv, b = bh / a.n_kv;
+    const int mul = a.n_heads / a.n_kv;
+    int p0;
+    const int n = kvq4_active(a.pos, a.count, b, a.n_new, a.ctx_len, p0);
+    const int rows = n * mul - 8 * grp;  // of this item (more than 8: 8)
+    if (rows <= 0) return;               // (the whole cluster)
+    const int r0 = 8 * grp;
+    const int len = p0 + min(n - 1, (r0 + 7) / mul) + 1;  // positions any of the rows sees
+    const int tiles = (len + kTile - 1) / kTile, step = (int)cs * kWarps;
+    const int64_t base = (int64_t)b * a.seq_rows + (int64_t)kvh * a.ctx_len;
+    uint8_t* ring = smem + (size_t)warp * ST * STB;
+
+    auto issue = [&](int tile, int s) {  // lane 0
+        const int64_t row = base + (int64_t)tile * kTile;
+        const int np = min(kTile, (len - tile * kTile + 7) & ~7);  // (ctx_len is a multiple of 8)
+        uint8_t* d = ring + s * STB;
+        mbar_expect_tx(&bars[warp][s], (uint32_t)(np * 36 * NB));
+        bulk_load(d, a.kq + row * RB, np * RB, &bars[warp][s]);
+        bulk_load(d + kTile * RB, a.vq + row * RB, np * RB, &bars[warp][s]);
+        bulk_load(d + 2 * kTile * RB, a.kd + row * NB, np * SB, &bars[warp][s]);
+        bulk_load(d + 2 * kTile * RB + kTile * SB, a.vd + row * NB, np * SB, &bars[warp][s]);
+    };
+    if (lane == 0) {
+        for (int s = 0; s < ST; s++) mbar_init(&bars[warp][s], 1);
+        fence_mbar_init();
+        fence_proxy_async();
+        for (int s = 0; s < ST; s++) {
+            const int tile = (int)rank * kWarps + warp + s * step;
+            if (tile < tiles) issue(tile, s);
         }
     }
-    const int64_t base = (int64_t)b * seq_rows + (int64_t)(h / (n_heads / n_kv)) * ctx_len;
-    float m = -INFINITY, l = 0.f;
-    for (int p = 0; p < len; p++) {
-        const int64_t r = base + p;
-        const uint16_t* kr = reinterpret_cast<const uint16_t*>(kq + r * (HD / 2) + g * (2 * NB));
-        const uint16_t* vr = reinterpret_cast<const uint16_t*>(vq + r * (HD / 2) + g * (2 * NB));
-        float s = 0.f;
+
+    // the rows' queries as A fragments; limit = last position the row sees
+    uint32_t qa[NB][8];
+    float bias[NB], factor;
+    int limit;
+    {
+        const int r = r0 + min(g, rows - 1);
+        const int tok = r / mul;
+        limit = p0 + tok;
+        const float* x = a.q + ((int64_t)b * a.n_new + tok) * a.q_stride + (int64_t)(kvh * mul + r % mul) * HD;
+        const float2* tab = a.rope ? a.rope + (int64_t)limit * (HD / 2) : nullptr;
+        float2 v[NB][4];
+        float amax = 0.f;
 #pragma unroll
         for (int j = 0; j < NB; j++)
-            s = fmaf(x[j], __half2float(kd[r * NB + j]) * (float)((int)((kr[j] >> (4 * t)) & 15) - 8), s);
 #pragma unroll
-        for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
-        s *= scale;
-        const float mn = fmaxf(m, s), a = expf(m - mn), w = expf(s - mn);
-        l = fmaf(l, a, w);
+            for (int i = 0; i < 4; i++) {
+                v[j][i] = query_pair<HD>(x, tab, a.neox, 32 * j + 8 * i + 2 * t);
+                amax = fmaxf(amax, fmaxf(fabsf(v[j][i].x), fabsf(v[j][i].y)));
+            }
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        float sc, inv;
+        row_pow2_scale(amax, sc, inv);
+        factor = a.scale * 1.44269504088896341f * 16777216.f * inv;
 #pragma unroll
-        for (int j = 0; j < NB; j++)
-            o[j] = fmaf(o[j], a, w * (__half2float(vd[r * NB + j]) * (float)((int)((vr[j] >> (4 * t)) & 15) - 8)));
-        m = mn;
+        for (int j = 0; j < NB; j++) {
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float m = (i & 1) ? sc * 0.0625f : sc;
+                const float x0 = v[j][i].x * m, x1 = v[j][i].y * m;
+                sum += (v[j][i].x + v[j][i].y) * sc;
+                // a0 / a1: high and low halves of k 2t, 2t+1; a2 / a3: of k 2t+8, 2t+9
+                split2(x0, x1, qa[j][4 * (i >> 1) + 2 * (i & 1)], qa[j][4 * (i >> 1) + 2 * (i & 1) + 1]);
+            }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            bias[j] = sum * (-8.f / 16777216.f);
+        }
     }
-    float* dst = out + tok * out_stride + (int64_t)h * HD;
+
+    float o[4 * NB][4];
 #pragma unroll
-    for (int j = 0; j < NB; j++) dst[32 * j + 8 * t + g] = o[j] / l;
+    for (int j = 0; j < 4 * NB; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    float R = -1e30f, l = 0.f;
+    uint32_t dtop = 0;            // largest |V scale| seen, fp16 bits rounded up to a power of two's top
+    float voff = -14.f - 6.f;     // log2 of a bound of it, less 6
+    bool ok = true;
+    // column c of a score tile is position c ^ ((c >> 1) & 1) of its eight: rows
+    // of both parities for the four t of a V load, and for K's
+    const int kcol = g ^ ((g >> 1) & 1);
+    const int c0 = (2 * t) ^ (t & 1), c1 = (2 * t + 1) ^ (t & 1);
+
+    int s = 0;
+    uint32_t parity = 0;
+    for (int tile = (int)rank * kWarps + warp; tile < tiles; tile += step) {
+        if (ok && !mbar_wait(&bars[warp][s], parity)) {
+            ok = false;
+            if (lane == 0) atomicOr(a.err, kErrTimeout);
+        }
+        const uint8_t* sk = ring + s * STB;
+        const uint8_t* sv = sk + kTile * RB;
+        uint8_t* skd = ring + s * STB + 2 * kTile * RB;
+        uint8_t* svd = skd + kTile * SB;
+        const int first = tile * kTile;
+        if (first + kTile > len && first + lane >= len) {
+            // rows past the end (the warp's last tile): no scale
+            for (int j = 0; j < NB; j++) {
+                reinterpret_cast<uint16_t*>(skd + lane * SB)[j] = 0;
+                reinterpret_cast<uint16_t*>(svd + lane * SB)[j] = 0;
+            }
+        }
+        __syncwarp();
+
+        // ---- scores ----
+        float p[4][2];
+        float top = -INFINITY;
+#pragma unroll
+        for (int nt = 0; nt < 4; nt++) {
+            uint32_t w[NB], d0[(NB + 1) / 2], d1[(NB + 1) / 2];
+            lds_words<NB>(w, sk + (8 * nt + kcol) * RB + t * 4 * NB);
+            lds_halves<NB>(d0, skd + (8 * nt + c0) * SB);
+            lds_halves<NB>(d1, skd + (8 * nt + c1) * SB);
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int j = 0; j < NB; j++) {
+                const uint32_t x = pair16(w, j, w, NB + j), y = x >> 8;
+                const uint32_t ba[2] = {x & 0x000F000Fu, x & 0x00F000F0u};
+                const uint32_t bb[2] = {y & 0x000F000Fu, y & 0x00F000F0u};
+                float c[4] = {bias[j], bias[j], 0.f, 0.f};
+                mma_16816(c, &qa[j][0], ba, c);
+                mma_16816(c, &qa[j][4], bb, c);
+                const float e0 = half_at(d0, j), e1 = half_at(d1, j);
+                s0 = fmaf(e0, c[0] + c[2], s0);
+                s1 = fmaf(e1, c[1] + c[3], s1);
+            }
+            p[nt][0] = first + 8 * nt + c0 <= limit ? s0 * factor : -INFINITY;
+            p[nt][1] = first + 8 * nt + c1 <= limit ? s1 * factor : -INFINITY;
+            top = fmaxf(top, fmaxf(p[nt][0], p[nt][1]));
+        }
+
+        // ---- reference ----
+        {
+            uint32_t h[(NB + 1) / 2], mx = 0;
+            lds_halves<NB>(h, svd + lane * SB);
+#pragma unroll
+            for (int j = 0; j < (NB + 1) / 2; j++) mx = __vmaxu2(mx, h[j] & 0x7FFF7FFFu);
+            mx = max(mx & 0xFFFFu, mx >> 16);
+            float up = 0.f;
+            if (__any_sync(0xffffffffu, mx > dtop)) {
+                dtop = __reduce_max_sync(0xffffffffu, mx) | 0x3FFu;
+                const float v = (float)(int)(dtop >> 10) - 14.f - 6.f;
+                up = v - voff;
+                voff = v;
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) + voff;
+            const bool move = top > R + kLazy || up > 0.f;
+            if (__any_sync(0xffffffffu, move)) {
+                const float Rn = move ? fmaxf(R + up, top) : R;
+                const float al = ex2(R - Rn);
+                R = Rn;
+                l *= al;
+#pragma unroll
+                for (int j = 0; j < 4 * NB; j++) {
+                    o[j][0] *= al;
+                    o[j][1] *= al;
+                    o[j][2] *= al;
+                    o[j][3] *= al;
+                }
+            }
+        }
+#pragma unroll
+        for (int nt = 0; nt < 4; nt++) {
+            p[nt][0] = ex2(p[nt][0] - R);
+            p[nt][1] = ex2(p[nt][1] - R);
+            l += p[nt][0] + p[nt][1];
+        }
+
+        // ---- output ----
+#pragma unroll
+        for (int G = 0; G < 2; G++) {
+            uint32_t w[4][(NB + 1) / 2], d[4][(NB + 1) / 2];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int r = 16 * G + 8 * (k >> 1) + ((k & 1) ? c1 : c0);
+                lds_halves<NB>(w[k], sv + r * RB + g * 2 * NB);
+                lds_halves<NB>(d[k], svd + r * SB);
+            }
+#pragma unroll
+            for (int j = 0; j < NB; j++) {
+                uint32_t af[4];
+                split2(p[2 * G][0] * half_at(d[0], j), p[2 * G][1] * half_at(d[1], j), af[0], af[1]);
+                split2(p[2 * G + 1][0] * half_at(d[2], j), p[2 * G + 1][1] * half_at(d[3], j), af[2], af[3]);
+                uint32_t x0 = pair16(w[0], j, w[1], j), x1 = pair16(w[2], j, w[3], j);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    uint32_t bf[2];
+                    if (i & 1) {  // 1024 + 16 level -> level - 8
+                        bf[0] = h2_fma(lop3_and_or(x0, 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u);
+                        bf[1] = h2_fma(lop3_and_or(x1, 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u);
+                    } else {  // 1024 + level -> level - 8
+                        bf[0] = h2_sub(lop3_and_or(x0, 0x000F000Fu, 0x64006400u), 0x64086408u);
+                        bf[1] = h2_sub(lop3_and_or(x1, 0x000F000Fu, 0x64006400u), 0x64086408u);
+                    }
+                    mma_16816(o[4 * j + i], af, bf, o[4 * j + i]);
+                    if (i == 1) {
+                        x0 >>= 8;
+                        x1 >>= 8;
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        if (lane == 0 && ok && tile + ST * step < tiles) issue(tile + ST * step, s);
+        if (++s == ST) {
+            s = 0;
+            parity ^= 1;
+        }
+    }
+
+    // ---- the CTA's partials, then the cluster's ----
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    __syncthreads();  // every warp is done with its ring
+    float* so = reinterpret_cast<float*>(smem);  // [kWarps + 1][8][HD]: the warps', then the CTA's
+    if (t == 0) {
+        sR[warp][g] = R;
+        sL[warp][g] = l;
+    }
+#pragma unroll
+    for (int j = 0; j < NB; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            *reinterpret_cast<float2*>(so + (warp * 8 + g) * HD + 32 * j + 8 * i + 2 * t) =
+                make_float2(o[4 * j + i][0] + o[4 * j + i][2], o[4 * j + i][1] + o[4 * j + i][3]);
+    __syncthreads();
+    float* sc = so + kWarps * 8 * HD;
+    for (int e = threadIdx.x; e < 8 * HD / 4; e += 32 * kWarps) {
+        const int r = e / (HD / 4);
+        float M = sR[0][r];
+#pragma unroll
+        for (int w = 1; w < kWarps; w++) M = fmaxf(M, sR[w][r]);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        float ls = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            const float f = ex2(sR[w][r] - M);
+            const float4 x = reinterpret_cast<const float4*>(so + w * 8 * HD)[e];
+            v.x = fmaf(f, x.x, v.x);
+            v.y = fmaf(f, x.y, v.y);
+            v.z = fmaf(f, x.z, v.z);
+            v.w = fmaf(f, x.w, v.w);
+            ls = fmaf(f, sL[w][r], ls);
+        }
+        reinterpret_cast<float4*>(sc)[e] = v;
+        if (e % (HD / 4) == 0) {
+            sR[kWarps][r] = M;
+            sL[kWarps][r] = ls;
+        }
+    }
+    __syncthreads();
+    if (cs > 1) {
+        cluster_arrive();
+        cluster_wait();
+    }
+    const uint32_t aR = smem_u32(&sR[kWarps][0]), aL = smem_u32(&sL[kWarps][0]), aO = smem_u32(sc);
+    for (int e = (int)rank * 32 * kWarps + threadIdx.x; e < min(rows, 8) * (HD / 4); e += (int)cs * 32 * kWarps) {
+        const int r = e / (HD / 4);
+        float M = -1e30f;
+        for (uint32_t c = 0; c < cs; c++) M = fmaxf(M, ld_cluster(aR + 4 * r, c));
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        float ls = 0.f;
+        for (uint32_t c = 0; c < cs; c++) {
+            const float f = ex2(ld_cluster(aR + 4 * r, c) - M);
+            const float4 x = ld_cluster4(aO + 16 * e, c);
+            v.x = fmaf(f, x.x, v.x);
+            v.y = fmaf(f, x.y, v.y);
+            v.z = fmaf(f, x.z, v.z);
+            v.w = fmaf(f, x.w, v.w);
+            ls = fmaf(f, ld_cluster(aL + 4 * r, c), ls);
+        }
+        const int rr = r0 + r;
+        float* dst = a.out + ((int64_t)b * a.n_new + rr / mul) * a.out_stride + (int64_t)(kvh * mul + rr % mul) * HD +
+                     4 * (e % (HD / 4));
+        *reinterpret_cast<float4*>(dst) = make_float4(v.x / ls, v.y / ls, v.z / ls, v.w / ls);
+    }
+    if (cs > 1) {  // no CTA's shared memory goes while another reads it
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+    }
 }
+
+namespace {
+
+using RowsFn = void (*)(AttendArgs);
+RowsFn rows_fn(int hd) {
+    switch (hd) {
+        case 32: return kvq4_attend_rows_kernel<1>;
+        case 64: return kvq4_attend_rows_kernel<2>;
+        case 96: return kvq4_attend_rows_kernel<3>;
+        case 128: return kvq4_attend_rows_kernel<4>;
+        default: return kvq4_attend_rows_kernel<8>;
+    }
+}
+
+size_t rows_smem(int nb) {
+    const size_t ring = (size_t)kWarps * stages(nb) * stage_bytes(nb), merge = (size_t)(kWarps + 1) * 8 * 32 * nb * 4;
+    return ring > merge ? ring : merge;
+}
+
+}  // namespace
 
 int kvq4_attend(cn_ctx* ctx, const cn_kvq4& c, const float* q, int64_t q_stride, float* out, int64_t out_stride,
                 const int* pos, const int* count, int batch, int n_new, int n_heads, float scale, const float2* rope,
                 int neox, cudaStream_t st) {
-    const int64_t rows = (int64_t)batch * n_new * n_heads, ctas = (rows + 3) / 4;
-    CN_CHECK(ctas < (1ll << 31), CN_ERR_INVALID_ARG, "too many rows (%lld)", (long long)rows);
-#define CALL(NB)                                                                                                   \
-    kvq4_attend_plain_kernel<NB><<<(unsigned)ctas, 128, 0, st>>>(                                                  \
-        q, q_stride, out, out_stride, pos, count, n_new, n_heads, c.n_kv_heads, rows, scale, rope, neox,           \
-        static_cast<const uint8_t*>(c.k_quants), static_cast<const __half*>(c.k_scales),                           \
-        static_cast<const uint8_t*>(c.v_quants), static_cast<const __half*>(c.v_scales), kvq4_seq_rows(c),         \
-        c.ctx_len);                                                                                                \
-    break
-    switch (c.head_dim) {
-        case 32: CALL(1);
-        case 64: CALL(2);
-        case 96: CALL(3);
-        case 128: CALL(4);
-        default: CALL(8);
-    }
-#undef CALL
-    CN_CUDA(cudaGetLastError());
+    AttendArgs a;
+    a.q = q;
+    a.out = out;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.pos = pos;
+    a.count = count;
+    a.rope = rope;
+    a.kq = static_cast<const uint8_t*>(c.k_quants);
+    a.vq = static_cast<const uint8_t*>(c.v_quants);
+    a.kd = static_cast<const __half*>(c.k_scales);
+    a.vd = static_cast<const __half*>(c.v_scales);
+    a.seq_rows = kvq4_seq_rows(c);
+    a.n_new = n_new;
+    a.n_heads = n_heads;
+    a.n_kv = c.n_kv_heads;
+    a.ctx_len = c.ctx_len;
+    a.neox = neox;
+    a.scale = scale;
+    a.err = ctx->dev_err;
+    const int64_t rows = (int64_t)n_new * (n_heads / c.n_kv_heads);
+    const int64_t groups = (rows + 7) / 8, items = groups * c.n_kv_heads * batch;
+    CN_CHECK(items < (1ll << 31) / kMaxCluster, CN_ERR_INVALID_ARG, "too many rows (%lld items)", (long long)items);
+    a.groups = (int)groups;
+    // CTAs per item: as many as the SMs hold at once (three each), and no more
+    // than give every warp a tile of the longest sequence
+    const int nb = c.head_dim / 32, per_sm = nb <= 4 ? 3 : 2;
+    const int64_t room = (int64_t)ctx->sms * per_sm, most = (c.ctx_len + kTile * kWarps - 1) / (kTile * kWarps);
+    int cluster = 1;
+    const char* env = getenv("KVQ4_CS");
+    if (env) cluster = atoi(env);
+    else
+        while (cluster < kMaxCluster && 2 * cluster <= most && 2 * cluster * items <= room) cluster *= 2;
+    RowsFn fn = rows_fn(c.head_dim);
+    const size_t smem = rows_smem(nb);
+    CN_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    CN_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    CN_CUDA(launch_cluster_k(false, cluster, fn, dim3((unsigned)(items * cluster)), dim3(32 * kWarps), smem, st, a));
     return CN_OK;
 }
 
@@ -111,8 +531,8 @@ extern "C" int cn_kvq4_attend_dev(cn_ctx* ctx, const cn_kvq4* cache, const float
     CN_CHECK(q_stride >= qd && out_stride >= qd && q_stride % 4 == 0 && out_stride % 4 == 0, CN_ERR_INVALID_ARG,
              "q_stride %lld / out_stride %lld: at least %lld values and a multiple of 4", (long long)q_stride,
              (long long)out_stride, (long long)qd);
-    CN_CHECK(((uintptr_t)d_q | (uintptr_t)d_out) % 16 == 0 && (uintptr_t)d_rope % 8 == 0, CN_ERR_INVALID_ARG,
-             "q and out must be 16-byte aligned, the rope table 8-byte");
+    CN_CHECK(((uintptr_t)d_q | (uintptr_t)d_out | (uintptr_t)d_rope) % 16 == 0, CN_ERR_INVALID_ARG,
+             "q, out and the rope table must be 16-byte aligned");
     CN_CHECK(isfinite(scale) && scale > 0.f, CN_ERR_INVALID_ARG, "scale must be finite and positive");
     CN_CHECK(rope_neox == 0 || rope_neox == 1, CN_ERR_INVALID_ARG, "rope_neox is 0 or 1");
     DeviceScope ds(ctx->device);

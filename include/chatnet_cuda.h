@@ -284,8 +284,8 @@ int cn_kvq4_append_dev(cn_ctx* ctx, const cn_kvq4* cache, const float* d_k, cons
  * append first): out[b][i][h] = softmax(scale * q . k_p over p <= d_pos[b] + i)
  * . v_p, query head h on kv head h / (n_heads / n_kv_heads) (ComputeAttention +
  * Softmax, LlamaModel.cs:241-346).  q (rotated first when d_rope is given) and
- * out: n_heads * head_dim fp32 values per token, 16-byte aligned, strides
- * multiples of 4, not overlapping.  fp32 results (products of q and of the
+ * out: n_heads * head_dim fp32 values per token, strides multiples of 4, not
+ * overlapping; q, out and d_rope 16-byte aligned.  fp32 results (products of q and of the
  * softmax weights carry 22 bits, sums 24). */
 int cn_kvq4_attend_dev(cn_ctx* ctx, const cn_kvq4* cache, const float* d_q, int64_t q_stride, float* d_out,
                        int64_t out_stride, const int* d_pos, const int* d_count, int batch, int n_new, int n_heads,
