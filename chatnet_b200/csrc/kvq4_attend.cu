@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows
 
     // the rows' queries as A fragments; limit = last position the row sees
     uint32_t qa[NB][8];
-    float bias[NB], factor;
+    float bias_hi[NB], bias_lo[NB], factor;
     int limit;
     {
         const int r = r0 + min(g, rows - 1);
@@ -223,24 +223,33 @@ __global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows
         factor = a.scale * 1.44269504088896341f * 16777216.f * inv;
 #pragma unroll
         for (int j = 0; j < NB; j++) {
-            float sum = 0.f;
+            float sum_hi = 0.f, sum_lo = 0.f;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float m = (i & 1) ? sc * 0.0625f : sc;
-                const float x0 = v[j][i].x * m, x1 = v[j][i].y * m;
-                sum += (v[j][i].x + v[j][i].y) * sc;
+                const float m = (i & 1) ? 0.0625f : 1.f;
+                const float x0 = v[j][i].x * sc, x1 = v[j][i].y * sc;
+                const float h0 = rintf(x0 * 0.0625f) * 16.f, h1 = rintf(x1 * 0.0625f) * 16.f;
+                const uint32_t hi = pack_half2(h0 * m, h1 * m), lo = pack_half2((x0 - h0) * m, (x1 - h1) * m);
+                const float2 lf = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+                sum_hi += h0 + h1;
+                sum_lo += (lf.x + lf.y) * ((i & 1) ? 16.f : 1.f);
                 // a0 / a1: high and low halves of k 2t, 2t+1; a2 / a3: of k 2t+8, 2t+9
-                split2(x0, x1, qa[j][4 * (i >> 1) + 2 * (i & 1)], qa[j][4 * (i >> 1) + 2 * (i & 1) + 1]);
+                qa[j][4 * (i >> 1) + 2 * (i & 1)] = hi;
+                qa[j][4 * (i >> 1) + 2 * (i & 1) + 1] = lo;
             }
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            bias[j] = sum * (-8.f / 16777216.f);
+#pragma unroll
+            for (int k = 1; k <= 2; k <<= 1) {
+                sum_hi += __shfl_xor_sync(0xffffffffu, sum_hi, k);
+                sum_lo += __shfl_xor_sync(0xffffffffu, sum_lo, k);
+            }
+            bias_hi[j] = sum_hi * (-8.f / 16777216.f);
+            bias_lo[j] = sum_lo * (-8.f / 16777216.f);
         }
     }
 
-    float o[4 * NB][4];
+    float o[4 * NB][2];
 #pragma unroll
-    for (int j = 0; j < 4 * NB; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    for (int j = 0; j < 4 * NB; j++) o[j][0] = o[j][1] = 0.f;
     float R = -1e30f, l = 0.f;
     uint32_t dtop = 0;            // largest |V scale| seen, fp16 bits rounded up to a power of two's top
     float voff = -14.f - 6.f;     // log2 of a bound of it, less 6
@@ -286,7 +295,7 @@ __global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows
                 const uint32_t x = pair16(w, j, w, NB + j), y = x >> 8;
                 const uint32_t ba[2] = {x & 0x000F000Fu, x & 0x00F000F0u};
                 const uint32_t bb[2] = {y & 0x000F000Fu, y & 0x00F000F0u};
-                float c[4] = {bias[j], bias[j], 0.f, 0.f};
+                float c[4] = {bias_hi[j], bias_hi[j], bias_lo[j], bias_lo[j]};
                 mma_16816(c, &qa[j][0], ba, c);
                 mma_16816(c, &qa[j][4], bb, c);
                 const float e0 = half_at(d0, j), e1 = half_at(d1, j);
@@ -324,8 +333,6 @@ __global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows
                 for (int j = 0; j < 4 * NB; j++) {
                     o[j][0] *= al;
                     o[j][1] *= al;
-                    o[j][2] *= al;
-                    o[j][3] *= al;
                 }
             }
         }
@@ -337,37 +344,40 @@ __global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows
         }
 
         // ---- output ----
+        uint32_t w[8][(NB + 1) / 2], d[8][(NB + 1) / 2];
 #pragma unroll
-        for (int G = 0; G < 2; G++) {
-            uint32_t w[4][(NB + 1) / 2], d[4][(NB + 1) / 2];
+        for (int k = 0; k < 8; k++) {
+            const int r = 8 * (k >> 1) + ((k & 1) ? c1 : c0);
+            lds_halves<NB>(w[k], sv + r * RB + g * 2 * NB);
+            lds_halves<NB>(d[k], svd + r * SB);
+        }
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int r = 16 * G + 8 * (k >> 1) + ((k & 1) ? c1 : c0);
-                lds_halves<NB>(w[k], sv + r * RB + g * 2 * NB);
-                lds_halves<NB>(d[k], svd + r * SB);
+        for (int j = 0; j < NB; j++) {
+            uint32_t af[2][4], x[4];
+#pragma unroll
+            for (int G = 0; G < 2; G++) {
+                split2(p[2 * G][0] * half_at(d[4 * G], j), p[2 * G][1] * half_at(d[4 * G + 1], j), af[G][0], af[G][1]);
+                split2(p[2 * G + 1][0] * half_at(d[4 * G + 2], j), p[2 * G + 1][1] * half_at(d[4 * G + 3], j),
+                       af[G][2], af[G][3]);
+                x[2 * G] = pair16(w[4 * G], j, w[4 * G + 1], j);
+                x[2 * G + 1] = pair16(w[4 * G + 2], j, w[4 * G + 3], j);
             }
 #pragma unroll
-            for (int j = 0; j < NB; j++) {
-                uint32_t af[4];
-                split2(p[2 * G][0] * half_at(d[0], j), p[2 * G][1] * half_at(d[1], j), af[0], af[1]);
-                split2(p[2 * G + 1][0] * half_at(d[2], j), p[2 * G + 1][1] * half_at(d[3], j), af[2], af[3]);
-                uint32_t x0 = pair16(w[0], j, w[1], j), x1 = pair16(w[2], j, w[3], j);
+            for (int i = 0; i < 4; i++) {
+                uint32_t bf[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    uint32_t bf[2];
-                    if (i & 1) {  // 1024 + 16 level -> level - 8
-                        bf[0] = h2_fma(lop3_and_or(x0, 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u);
-                        bf[1] = h2_fma(lop3_and_or(x1, 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u);
-                    } else {  // 1024 + level -> level - 8
-                        bf[0] = h2_sub(lop3_and_or(x0, 0x000F000Fu, 0x64006400u), 0x64086408u);
-                        bf[1] = h2_sub(lop3_and_or(x1, 0x000F000Fu, 0x64006400u), 0x64086408u);
-                    }
-                    mma_16816(o[4 * j + i], af, bf, o[4 * j + i]);
-                    if (i == 1) {
-                        x0 >>= 8;
-                        x1 >>= 8;
-                    }
+                for (int k = 0; k < 4; k++) {
+                    if (i & 1)  // 1024 + 16 level -> level - 8
+                        bf[k] = h2_fma(lop3_and_or(x[k], 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u);
+                    else  // 1024 + level -> level - 8
+                        bf[k] = h2_sub(lop3_and_or(x[k], 0x000F000Fu, 0x64006400u), 0x64086408u);
+                    if (i == 1) x[k] >>= 8;
                 }
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+                mma_16816(c, af[0], bf, c);
+                mma_16816(c, af[1], bf + 2, c);
+                o[4 * j + i][0] += c[0] + c[2];
+                o[4 * j + i][1] += c[1] + c[3];
             }
         }
         __syncwarp();
@@ -392,7 +402,7 @@ __global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows
 #pragma unroll
         for (int i = 0; i < 4; i++)
             *reinterpret_cast<float2*>(so + (warp * 8 + g) * HD + 32 * j + 8 * i + 2 * t) =
-                make_float2(o[4 * j + i][0] + o[4 * j + i][2], o[4 * j + i][1] + o[4 * j + i][3]);
+                make_float2(o[4 * j + i][0], o[4 * j + i][1]);
     __syncthreads();
     float* sc = so + kWarps * 8 * HD;
     for (int e = threadIdx.x; e < 8 * HD / 4; e += 32 * kWarps) {
