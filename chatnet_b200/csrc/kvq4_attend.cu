@@ -31,7 +31,8 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kTile = 32;        // positions a warp takes at a time
-constexpr float kLazy = 8.f;     // a row's reference moves only when the maximum outgrows it by 2^8
+constexpr float kPeak = 9.f;     // a weight is 2^9 at the row's reference
+constexpr float kLazy = 4.f;     // a row's reference moves only when the maximum outgrows it by 2^4
 constexpr int kMaxCluster = 16;
 
 __host__ __device__ constexpr int stage_bytes(int nb) { return kTile * 36 * nb; }
@@ -46,7 +47,40 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 
 __device__ __forceinline__ float ex2(float x) {
     float r;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// two fp32 operations in one instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(r)
+        : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+    return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(r)
+        : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)),
+          "l"(*reinterpret_cast<uint64_t*>(&c)));
+    return *reinterpret_cast<float2*>(&r);
+}
+// D = A B + C on m16n8k16, free to be scheduled
+__device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, const float* c) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+// a b - c
+__device__ __forceinline__ uint32_t h2_fms(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("{\n\t.reg .b32 n;\n\tneg.f16x2 n, %3;\n\tfma.rn.f16x2 %0, %1, %2, n;\n\t}" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
 
@@ -148,13 +182,18 @@ __device__ __forceinline__ uint32_t pair16(const uint32_t* a, int i, const uint3
 // by a power of two: 22 bits).  K's levels go in as fp16 subnormals, level *
 // 2^-24 straight from the nibble (every second nibble as 16 * level, with q
 // divided by 16 there), so a fragment costs one AND per two values; the
-// -8 of a value is the accumulator's start, -8 sum(q), and the block's scale
-// multiplies the block's sums in fp32.
-// Output: O = W V with w_p d_p,b (weight times the block's scale) split into
-// halves the same way and V's signed levels exact in fp16.
-// A row's reference R (log2 units) is its running maximum plus the exponent of
-// the largest V scale seen, less 6: w d stays below 2^14 and keeps 22 bits down
-// to 2^-18 of it, whatever the cache's range.
+// -8 of a value is added as -8 sum(q) and the block's scale multiplies the
+// block's sum in fp32.  The high halves are whole multiples of 16, so that their
+// products with a block's levels add up exactly.
+// Output: O = W V with V's signed levels exact in fp16 and w_p d_p,b (weight
+// times the block's scale) as two halves: w's halves hi, lo times the fp16 d
+// give h = hi d rounded, then its exact rounding error and lo d in the second
+// half, all in packed fp16 (three instructions for two positions).  A row's
+// weights are 2^9 at its reference (log2 units), a running maximum that moves when
+// outgrown by 2^4, and V's scales count 2^e times where the largest seen
+// lies outside [2^-7, 4), so w d stays below 2^15 and keeps 22 bits down to 2^-25
+// of that, whatever the cache's range.  Each tile's products are summed from
+// zero and joined in fp32 (the tensor cores truncate where fp32 rounds).
 template <int NB>
 __global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows_kernel(const AttendArgs a) {
     constexpr int HD = 32 * NB, RB = 16 * NB, SB = 2 * NB;  // bytes of a row's quants and scales
@@ -199,7 +238,8 @@ __global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows
 
     // the rows' queries as A fragments; limit = last position the row sees
     uint32_t qa[NB][8];
-    float bias_hi[NB], bias_lo[NB], factor;
+    float2 bias[NB];
+    float factor;
     int limit;
     {
         const int r = r0 + min(g, rows - 1);
@@ -242,18 +282,18 @@ __global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows
                 sum_hi += __shfl_xor_sync(0xffffffffu, sum_hi, k);
                 sum_lo += __shfl_xor_sync(0xffffffffu, sum_lo, k);
             }
-            bias_hi[j] = sum_hi * (-8.f / 16777216.f);
-            bias_lo[j] = sum_lo * (-8.f / 16777216.f);
+            bias[j].x = bias[j].y = (sum_hi + sum_lo) * (-8.f / 16777216.f);
         }
     }
 
-    float o[4 * NB][2];
+    float2 o[4 * NB];
 #pragma unroll
-    for (int j = 0; j < 4 * NB; j++) o[j][0] = o[j][1] = 0.f;
+    for (int j = 0; j < 4 * NB; j++) o[j] = make_float2(0.f, 0.f);
     float R = -1e30f, l = 0.f;
-    uint32_t dtop = 0;            // largest |V scale| seen, fp16 bits rounded up to a power of two's top
-    float voff = -14.f - 6.f;     // log2 of a bound of it, less 6
-    bool ok = true;
+    uint32_t dtop = 0;  // bound of the |V scale| seen, fp16 bits
+    int e2 = 0;         // V's scales count 2^e2 times
+    bool ok = true, fresh = true;
+    const int seen_by_all = p0 + r0 / mul + 1;  // positions every row sees
     // column c of a score tile is position c ^ ((c >> 1) & 1) of its eight: rows
     // of both parities for the four t of a V load, and for K's
     const int kcol = g ^ ((g >> 1) & 1);
@@ -281,7 +321,7 @@ __global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows
         __syncwarp();
 
         // ---- scores ----
-        float p[4][2];
+        float2 p[4];
         float top = -INFINITY;
 #pragma unroll
         for (int nt = 0; nt < 4; nt++) {
@@ -289,62 +329,81 @@ __global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows
             lds_words<NB>(w, sk + (8 * nt + kcol) * RB + t * 4 * NB);
             lds_halves<NB>(d0, skd + (8 * nt + c0) * SB);
             lds_halves<NB>(d1, skd + (8 * nt + c1) * SB);
-            float s0 = 0.f, s1 = 0.f;
+            p[nt] = make_float2(0.f, 0.f);
 #pragma unroll
             for (int j = 0; j < NB; j++) {
                 const uint32_t x = pair16(w, j, w, NB + j), y = x >> 8;
-                const uint32_t ba[2] = {x & 0x000F000Fu, x & 0x00F000F0u};
-                const uint32_t bb[2] = {y & 0x000F000Fu, y & 0x00F000F0u};
-                float c[4] = {bias_hi[j], bias_hi[j], bias_lo[j], bias_lo[j]};
-                mma_16816(c, &qa[j][0], ba, c);
-                mma_16816(c, &qa[j][4], bb, c);
-                const float e0 = half_at(d0, j), e1 = half_at(d1, j);
-                s0 = fmaf(e0, c[0] + c[2], s0);
-                s1 = fmaf(e1, c[1] + c[3], s1);
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+                mma(c, &qa[j][0], x & 0x000F000Fu, x & 0x00F000F0u, c);
+                mma(c, &qa[j][4], y & 0x000F000Fu, y & 0x00F000F0u, c);
+                p[nt] = fma2(make_float2(half_at(d0, j), half_at(d1, j)),
+                             add2(make_float2(c[0], c[1]), add2(make_float2(c[2], c[3]), bias[j])), p[nt]);
             }
-            p[nt][0] = first + 8 * nt + c0 <= limit ? s0 * factor : -INFINITY;
-            p[nt][1] = first + 8 * nt + c1 <= limit ? s1 * factor : -INFINITY;
-            top = fmaxf(top, fmaxf(p[nt][0], p[nt][1]));
         }
+        if (first + kTile > seen_by_all) {  // positions some row does not see
+#pragma unroll
+            for (int nt = 0; nt < 4; nt++) {
+                if (first + 8 * nt + c0 > limit) p[nt].x = -INFINITY;
+                if (first + 8 * nt + c1 > limit) p[nt].y = -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int nt = 0; nt < 4; nt++) top = fmaxf(top, fmaxf(p[nt].x, p[nt].y));
+        top *= factor;
 
-        // ---- reference ----
+        // ---- reference and scale (a lane looks at one position's V scales) ----
         {
             uint32_t h[(NB + 1) / 2], mx = 0;
             lds_halves<NB>(h, svd + lane * SB);
 #pragma unroll
             for (int j = 0; j < (NB + 1) / 2; j++) mx = __vmaxu2(mx, h[j] & 0x7FFF7FFFu);
             mx = max(mx & 0xFFFFu, mx >> 16);
-            float up = 0.f;
-            if (__any_sync(0xffffffffu, mx > dtop)) {
-                dtop = __reduce_max_sync(0xffffffffu, mx) | 0x3FFu;
-                const float v = (float)(int)(dtop >> 10) - 14.f - 6.f;
-                up = v - voff;
-                voff = v;
-            }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) + voff;
-            const bool move = top > R + kLazy || up > 0.f;
-            if (__any_sync(0xffffffffu, move)) {
-                const float Rn = move ? fmaxf(R + up, top) : R;
-                const float al = ex2(R - Rn);
-                R = Rn;
+            if (__any_sync(0xffffffffu, top > R + (kPeak + kLazy) || mx > dtop)) {
+                float grow = 1.f;
+                mx = __reduce_max_sync(0xffffffffu, mx);
+                if (mx > dtop) {
+                    // the scales lie below 2^(E - 14), E the exponent field
+                    dtop = mx | 0x3FFu;
+                    const int E = (int)(dtop >> 10) - 14, ne = E >= -6 && E <= 2 ? 0 : min(2 - E, 15);
+                    grow = fresh ? 1.f : exp2f((float)(ne - e2));
+                    e2 = ne;
+                    fresh = false;
+                }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                float al = 1.f;
+                if (top > R + (kPeak + kLazy)) {  // R: the score at which a weight is 1
+                    al = ex2(R - (top - kPeak));
+                    R = top - kPeak;
+                }
                 l *= al;
+                al *= grow;
 #pragma unroll
                 for (int j = 0; j < 4 * NB; j++) {
-                    o[j][0] *= al;
-                    o[j][1] *= al;
+                    o[j].x *= al;
+                    o[j].y *= al;
                 }
+            }
+            if (e2 != 0) {
+                const uint32_t f = (uint32_t)(15 + e2) << 10;  // e2 is in -14..15
+#pragma unroll
+                for (int j = 0; j < NB; j++) {
+                    uint16_t* q = reinterpret_cast<uint16_t*>(svd + lane * SB) + j;
+                    *q = (uint16_t)h2_mul(*q, f);
+                }
+                fence_proxy_async();  // (the ring's next copy into this place comes after)
+                __syncwarp();
             }
         }
 #pragma unroll
         for (int nt = 0; nt < 4; nt++) {
-            p[nt][0] = ex2(p[nt][0] - R);
-            p[nt][1] = ex2(p[nt][1] - R);
-            l += p[nt][0] + p[nt][1];
+            p[nt].x = ex2(fmaf(p[nt].x, factor, -R));
+            p[nt].y = ex2(fmaf(p[nt].y, factor, -R));
+            l += p[nt].x + p[nt].y;
         }
 
         // ---- output ----
-        uint32_t w[8][(NB + 1) / 2], d[8][(NB + 1) / 2];
+        uint32_t w[8][(NB + 1) / 2], d[8][(NB + 1) / 2], hi[4], lo[4];
 #pragma unroll
         for (int k = 0; k < 8; k++) {
             const int r = 8 * (k >> 1) + ((k & 1) ? c1 : c0);
@@ -352,15 +411,17 @@ __global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows
             lds_halves<NB>(d[k], svd + r * SB);
         }
 #pragma unroll
+        for (int nt = 0; nt < 4; nt++) split2(p[nt].x, p[nt].y, hi[nt], lo[nt]);
+#pragma unroll
         for (int j = 0; j < NB; j++) {
             uint32_t af[2][4], x[4];
 #pragma unroll
-            for (int G = 0; G < 2; G++) {
-                split2(p[2 * G][0] * half_at(d[4 * G], j), p[2 * G][1] * half_at(d[4 * G + 1], j), af[G][0], af[G][1]);
-                split2(p[2 * G + 1][0] * half_at(d[4 * G + 2], j), p[2 * G + 1][1] * half_at(d[4 * G + 3], j),
-                       af[G][2], af[G][3]);
-                x[2 * G] = pair16(w[4 * G], j, w[4 * G + 1], j);
-                x[2 * G + 1] = pair16(w[4 * G + 2], j, w[4 * G + 3], j);
+            for (int nt = 0; nt < 4; nt++) {
+                const uint32_t dd = pair16(d[2 * nt], j, d[2 * nt + 1], j);
+                const uint32_t h = h2_mul(hi[nt], dd);
+                af[nt >> 1][2 * (nt & 1)] = h;
+                af[nt >> 1][2 * (nt & 1) + 1] = h2_fma(lo[nt], dd, h2_fms(hi[nt], dd, h));
+                x[nt] = pair16(w[2 * nt], j, w[2 * nt + 1], j);
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -374,10 +435,9 @@ __global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows
                     if (i == 1) x[k] >>= 8;
                 }
                 float c[4] = {0.f, 0.f, 0.f, 0.f};
-                mma_16816(c, af[0], bf, c);
-                mma_16816(c, af[1], bf + 2, c);
-                o[4 * j + i][0] += c[0] + c[2];
-                o[4 * j + i][1] += c[1] + c[3];
+                mma(c, af[0], bf[0], bf[1], c);
+                mma(c, af[1], bf[2], bf[3], c);
+                o[4 * j + i] = add2(o[4 * j + i], add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])));
             }
         }
         __syncwarp();
@@ -393,6 +453,7 @@ __global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     __syncthreads();  // every warp is done with its ring
     float* so = reinterpret_cast<float*>(smem);  // [kWarps + 1][8][HD]: the warps', then the CTA's
+    const float un = exp2f((float)-e2);
     if (t == 0) {
         sR[warp][g] = R;
         sL[warp][g] = l;
@@ -402,7 +463,7 @@ __global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows
 #pragma unroll
         for (int i = 0; i < 4; i++)
             *reinterpret_cast<float2*>(so + (warp * 8 + g) * HD + 32 * j + 8 * i + 2 * t) =
-                make_float2(o[4 * j + i][0], o[4 * j + i][1]);
+                make_float2(o[4 * j + i].x * un, o[4 * j + i].y * un);
     __syncthreads();
     float* sc = so + kWarps * 8 * HD;
     for (int e = threadIdx.x; e < 8 * HD / 4; e += 32 * kWarps) {
