@@ -31,12 +31,14 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kTile = 32;        // positions a warp takes at a time
+constexpr int kStage = kTile * kWarps;  // positions of a ring stage
 constexpr float kPeak = 9.f;     // a weight is 2^9 at the row's reference
 constexpr float kLazy = 4.f;     // a row's reference moves only when the maximum outgrows it by 2^4
 constexpr int kMaxCluster = 16;
 
-__host__ __device__ constexpr int stage_bytes(int nb) { return kTile * 36 * nb; }
-__host__ __device__ constexpr int stages(int nb) { return nb <= 4 ? 4 : 2; }
+__host__ __device__ constexpr int stage_bytes(int nb) { return kStage * 36 * nb; }
+__host__ __device__ constexpr int stages(int nb) { return nb <= 4 ? 3 : 2; }
+__host__ __device__ constexpr int ctas_per_sm(int nb) { return nb <= 4 ? 4 : 2; }
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile(
@@ -66,6 +68,16 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
           "l"(*reinterpret_cast<uint64_t*>(&c)));
     return *reinterpret_cast<float2*>(&r);
 }
+// The halves of hi + lo = x: hi keeps 11 bits (x truncated, so the
+// conversion is exact in fp16's normal range), lo the next 11.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const float2 h = make_float2(__uint_as_float(__float_as_uint(a) & 0xFFFFE000u),
+                                 __uint_as_float(__float_as_uint(b) & 0xFFFFE000u));
+    const float2 l = fma2(h, make_float2(-1.f, -1.f), make_float2(a, b));
+    hi = pack_half2(h.x, h.y);
+    lo = pack_half2(l.x, l.y);
+}
+
 // D = A B + C on m16n8k16, free to be scheduled
 __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, const float* c) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
@@ -96,15 +108,6 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
     float v;
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_rank(addr, rank)) : "memory");
     return v;
-}
-
-// The halves of hi + lo = x: hi keeps 11 bits (x truncated, so the
-// conversion is exact in fp16's normal range), lo the next 11.
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-    const float ah = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u);
-    const float bh = __uint_as_float(__float_as_uint(b) & 0xFFFFE000u);
-    hi = pack_half2(ah, bh);
-    lo = pack_half2(a - ah, b - bh);
 }
 
 // Rotated query values e, e + 1 (e even) of one row.
@@ -172,7 +175,7 @@ __device__ __forceinline__ uint32_t pair16(const uint32_t* a, int i, const uint3
 
 // Few rows against a long cache (decode).  An item is eight rows of one
 // (sequence, kv head); its CTAs form a cluster, and every warp of it takes
-// tiles of 32 positions in turn, each through its own ring of bulk copies, with
+// 32 of every 128 positions its CTA takes in turn (a ring of bulk copies), with
 // its own running reference, sum and output.  The partials meet in shared
 // memory, first the CTA's, then the cluster's: no workspace, no atomics, one
 // launch.
@@ -195,11 +198,11 @@ __device__ __forceinline__ uint32_t pair16(const uint32_t* a, int i, const uint3
 // of that, whatever the cache's range.  Each tile's products are summed from
 // zero and joined in fp32 (the tensor cores truncate where fp32 rounds).
 template <int NB>
-__global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows_kernel(const AttendArgs a) {
     constexpr int HD = 32 * NB, RB = 16 * NB, SB = 2 * NB;  // bytes of a row's quants and scales
     constexpr int ST = stages(NB), STB = stage_bytes(NB);
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ uint64_t bars[kWarps][ST];
+    __shared__ uint64_t full[ST], freed[ST];
     __shared__ float sR[kWarps + 1][8], sL[kWarps + 1][8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t cs = cluster_size(), rank = cluster_rank();
@@ -212,28 +215,28 @@ __global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows
     if (rows <= 0) return;               // (the whole cluster)
     const int r0 = 8 * grp;
     const int len = p0 + min(n - 1, (r0 + 7) / mul) + 1;  // positions any of the rows sees
-    const int tiles = (len + kTile - 1) / kTile, step = (int)cs * kWarps;
+    const int tiles = (len + kStage - 1) / kStage;  // stages in all; this CTA's: rank, rank + cs, ...
     const int64_t base = (int64_t)b * a.seq_rows + (int64_t)kvh * a.ctx_len;
-    uint8_t* ring = smem + (size_t)warp * ST * STB;
 
-    auto issue = [&](int tile, int s) {  // lane 0
-        const int64_t row = base + (int64_t)tile * kTile;
-        const int np = min(kTile, (len - tile * kTile + 7) & ~7);  // (ctx_len is a multiple of 8)
-        uint8_t* d = ring + s * STB;
-        mbar_expect_tx(&bars[warp][s], (uint32_t)(np * 36 * NB));
-        bulk_load(d, a.kq + row * RB, np * RB, &bars[warp][s]);
-        bulk_load(d + kTile * RB, a.vq + row * RB, np * RB, &bars[warp][s]);
-        bulk_load(d + 2 * kTile * RB, a.kd + row * NB, np * SB, &bars[warp][s]);
-        bulk_load(d + 2 * kTile * RB + kTile * SB, a.vd + row * NB, np * SB, &bars[warp][s]);
+    auto issue = [&](int tile, int s) {  // one thread
+        const int64_t row = base + (int64_t)tile * kStage;
+        const int np = min(kStage, (len - tile * kStage + 7) & ~7);  // (ctx_len is a multiple of 8)
+        uint8_t* d = smem + s * STB;
+        mbar_expect_tx(&full[s], (uint32_t)(np * 36 * NB));
+        bulk_load(d, a.kq + row * RB, np * RB, &full[s]);
+        bulk_load(d + kStage * RB, a.vq + row * RB, np * RB, &full[s]);
+        bulk_load(d + 2 * kStage * RB, a.kd + row * NB, np * SB, &full[s]);
+        bulk_load(d + 2 * kStage * RB + kStage * SB, a.vd + row * NB, np * SB, &full[s]);
     };
-    if (lane == 0) {
-        for (int s = 0; s < ST; s++) mbar_init(&bars[warp][s], 1);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < ST; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&freed[s], kWarps);
+        }
         fence_mbar_init();
         fence_proxy_async();
-        for (int s = 0; s < ST; s++) {
-            const int tile = (int)rank * kWarps + warp + s * step;
-            if (tile < tiles) issue(tile, s);
-        }
+        for (int s = 0; s < ST; s++)
+            if ((int)(rank + s * cs) < tiles) issue((int)(rank + s * cs), s);
     }
 
     // the rows' queries as A fragments; limit = last position the row sees
@@ -289,7 +292,8 @@ __global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows
     float2 o[4 * NB];
 #pragma unroll
     for (int j = 0; j < 4 * NB; j++) o[j] = make_float2(0.f, 0.f);
-    float R = -1e30f, l = 0.f;
+    float R = -1e30f;
+    float2 l2 = make_float2(0.f, 0.f);
     uint32_t dtop = 0;  // bound of the |V scale| seen, fp16 bits
     int e2 = 0;         // V's scales count 2^e2 times
     bool ok = true, fresh = true;
@@ -299,20 +303,29 @@ __global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows
     const int kcol = g ^ ((g >> 1) & 1);
     const int c0 = (2 * t) ^ (t & 1), c1 = (2 * t + 1) ^ (t & 1);
 
-    int s = 0;
+    __syncthreads();  // the barriers are set up
+    int s = 0, it = 0;
     uint32_t parity = 0;
-    for (int tile = (int)rank * kWarps + warp; tile < tiles; tile += step) {
-        if (ok && !mbar_wait(&bars[warp][s], parity)) {
+    for (int tile = (int)rank; tile < tiles; tile += (int)cs, it++) {
+        // the stage of the step before is filled again once every warp is done
+        // with it; the warps take turns
+        if (it > 0 && warp == (it & (kWarps - 1)) && lane == 0 && ok && tile + (ST - 1) * (int)cs < tiles) {
+            const int ps = s ? s - 1 : ST - 1;
+            ok = mbar_wait(&freed[ps], s ? parity : parity ^ 1);
+            if (ok) issue(tile + (ST - 1) * (int)cs, ps);
+            else atomicOr(a.err, kErrTimeout);
+        }
+        if (ok && !mbar_wait(&full[s], parity)) {
             ok = false;
             if (lane == 0) atomicOr(a.err, kErrTimeout);
         }
-        const uint8_t* sk = ring + s * STB;
-        const uint8_t* sv = sk + kTile * RB;
-        uint8_t* skd = ring + s * STB + 2 * kTile * RB;
-        uint8_t* svd = skd + kTile * SB;
-        const int first = tile * kTile;
+        const uint8_t* sk = smem + s * STB + warp * kTile * RB;
+        const uint8_t* sv = sk + kStage * RB;
+        uint8_t* skd = smem + s * STB + 2 * kStage * RB + warp * kTile * SB;
+        uint8_t* svd = skd + kStage * SB;
+        const int first = tile * kStage + warp * kTile;
         if (first + kTile > len && first + lane >= len) {
-            // rows past the end (the warp's last tile): no scale
+            // rows past the end (the last stage): no scale
             for (int j = 0; j < NB; j++) {
                 reinterpret_cast<uint16_t*>(skd + lane * SB)[j] = 0;
                 reinterpret_cast<uint16_t*>(svd + lane * SB)[j] = 0;
@@ -376,7 +389,8 @@ __global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows
                     al = ex2(R - (top - kPeak));
                     R = top - kPeak;
                 }
-                l *= al;
+                l2.x *= al;
+                l2.y *= al;
                 al *= grow;
 #pragma unroll
                 for (int j = 0; j < 4 * NB; j++) {
@@ -399,49 +413,62 @@ __global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows
         for (int nt = 0; nt < 4; nt++) {
             p[nt].x = ex2(fmaf(p[nt].x, factor, -R));
             p[nt].y = ex2(fmaf(p[nt].y, factor, -R));
-            l += p[nt].x + p[nt].y;
+            l2 = add2(l2, p[nt]);
         }
 
         // ---- output ----
-        uint32_t w[8][(NB + 1) / 2], d[8][(NB + 1) / 2], hi[4], lo[4];
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const int r = 8 * (k >> 1) + ((k & 1) ? c1 : c0);
-            lds_halves<NB>(w[k], sv + r * RB + g * 2 * NB);
-            lds_halves<NB>(d[k], svd + r * SB);
-        }
+        uint32_t hi[4], lo[4];
 #pragma unroll
         for (int nt = 0; nt < 4; nt++) split2(p[nt].x, p[nt].y, hi[nt], lo[nt]);
 #pragma unroll
-        for (int j = 0; j < NB; j++) {
-            uint32_t af[2][4], x[4];
+        for (int jp = 0; jp < NB; jp += 2) {  // two blocks: one word of a chunk, one of the scales
+            uint32_t w[8], d[8];
 #pragma unroll
-            for (int nt = 0; nt < 4; nt++) {
-                const uint32_t dd = pair16(d[2 * nt], j, d[2 * nt + 1], j);
-                const uint32_t h = h2_mul(hi[nt], dd);
-                af[nt >> 1][2 * (nt & 1)] = h;
-                af[nt >> 1][2 * (nt & 1) + 1] = h2_fma(lo[nt], dd, h2_fms(hi[nt], dd, h));
-                x[nt] = pair16(w[2 * nt], j, w[2 * nt + 1], j);
+            for (int k = 0; k < 8; k++) {
+                const int r = 8 * (k >> 1) + ((k & 1) ? c1 : c0);
+                if constexpr (NB % 2 == 0) {
+                    w[k] = *reinterpret_cast<const uint32_t*>(sv + r * RB + g * 2 * NB + 2 * jp);
+                    d[k] = *reinterpret_cast<const uint32_t*>(svd + r * SB + 2 * jp);
+                } else {
+                    const uint16_t* wp = reinterpret_cast<const uint16_t*>(sv + r * RB + g * 2 * NB) + jp;
+                    const uint16_t* dp = reinterpret_cast<const uint16_t*>(svd + r * SB) + jp;
+                    w[k] = (uint32_t)wp[0] | (jp + 1 < NB ? (uint32_t)wp[1] << 16 : 0u);
+                    d[k] = (uint32_t)dp[0] | (jp + 1 < NB ? (uint32_t)dp[1] << 16 : 0u);
+                }
             }
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                uint32_t bf[4];
+            for (int jj = 0; jj < 2; jj++) {
+                if (jp + jj >= NB) break;
+                const int j = jp + jj;
+                uint32_t af[2][4], x[4];
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    if (i & 1)  // 1024 + 16 level -> level - 8
-                        bf[k] = h2_fma(lop3_and_or(x[k], 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u);
-                    else  // 1024 + level -> level - 8
-                        bf[k] = h2_sub(lop3_and_or(x[k], 0x000F000Fu, 0x64006400u), 0x64086408u);
-                    if (i == 1) x[k] >>= 8;
+                for (int nt = 0; nt < 4; nt++) {
+                    const uint32_t dd = pair16(&d[2 * nt], jj, &d[2 * nt + 1], jj);
+                    const uint32_t h = h2_mul(hi[nt], dd);
+                    af[nt >> 1][2 * (nt & 1)] = h;
+                    af[nt >> 1][2 * (nt & 1) + 1] = h2_fma(lo[nt], dd, h2_fms(hi[nt], dd, h));
+                    x[nt] = pair16(&w[2 * nt], jj, &w[2 * nt + 1], jj);
                 }
-                float c[4] = {0.f, 0.f, 0.f, 0.f};
-                mma(c, af[0], bf[0], bf[1], c);
-                mma(c, af[1], bf[2], bf[3], c);
-                o[4 * j + i] = add2(o[4 * j + i], add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])));
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    uint32_t bf[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        if (i & 1)  // 1024 + 16 level -> level - 8
+                            bf[k] = h2_fma(lop3_and_or(x[k], 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u);
+                        else  // 1024 + level -> level - 8
+                            bf[k] = h2_sub(lop3_and_or(x[k], 0x000F000Fu, 0x64006400u), 0x64086408u);
+                        if (i == 1) x[k] >>= 8;
+                    }
+                    float c[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma(c, af[0], bf[0], bf[1], c);
+                    mma(c, af[1], bf[2], bf[3], c);
+                    o[4 * j + i] = add2(o[4 * j + i], add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])));
+                }
             }
         }
         __syncwarp();
-        if (lane == 0 && ok && tile + ST * step < tiles) issue(tile + ST * step, s);
+        if (lane == 0) mbar_arrive(&freed[s]);
         if (++s == ST) {
             s = 0;
             parity ^= 1;
@@ -449,6 +476,7 @@ __global__ void __launch_bounds__(32 * kWarps, NB <= 4 ? 3 : 2) kvq4_attend_rows
     }
 
     // ---- the CTA's partials, then the cluster's ----
+    float l = l2.x + l2.y;
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     __syncthreads();  // every warp is done with its ring
@@ -536,7 +564,7 @@ RowsFn rows_fn(int hd) {
 }
 
 size_t rows_smem(int nb) {
-    const size_t ring = (size_t)kWarps * stages(nb) * stage_bytes(nb), merge = (size_t)(kWarps + 1) * 8 * 32 * nb * 4;
+    const size_t ring = (size_t)stages(nb) * stage_bytes(nb), merge = (size_t)(kWarps + 1) * 8 * 32 * nb * 4;
     return ring > merge ? ring : merge;
 }
 
@@ -569,10 +597,10 @@ int kvq4_attend(cn_ctx* ctx, const cn_kvq4& c, const float* q, int64_t q_stride,
     const int64_t groups = (rows + 7) / 8, items = groups * c.n_kv_heads * batch;
     CN_CHECK(items < (1ll << 31) / kMaxCluster, CN_ERR_INVALID_ARG, "too many rows (%lld items)", (long long)items);
     a.groups = (int)groups;
-    // CTAs per item: as many as the SMs hold at once (three each), and no more
+    // CTAs per item: as many as the SMs hold at once , and no more
     // than give every warp a tile of the longest sequence
-    const int nb = c.head_dim / 32, per_sm = nb <= 4 ? 3 : 2;
-    const int64_t room = (int64_t)ctx->sms * per_sm, most = (c.ctx_len + kTile * kWarps - 1) / (kTile * kWarps);
+    const int nb = c.head_dim / 32, per_sm = ctas_per_sm(nb);
+    const int64_t room = (int64_t)ctx->sms * per_sm, most = (c.ctx_len + kStage - 1) / kStage;
     int cluster = 1;
     const char* env = getenv("KVQ4_CS");
     if (env) cluster = atoi(env);
