@@ -30,15 +30,18 @@ struct AttendArgs {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kTile = 32;        // positions a warp takes at a time
-constexpr int kStage = kTile * kWarps;  // positions of a ring stage
 constexpr float kPeak = 9.f;     // a weight is 2^9 at the row's reference
 constexpr float kLazy = 4.f;     // a row's reference moves only when the maximum outgrows it by 2^4
 constexpr int kMaxCluster = 16;
 
-__host__ __device__ constexpr int stage_bytes(int nb) { return kStage * 36 * nb; }
-__host__ __device__ constexpr int stages(int nb) { return nb <= 4 ? 3 : 2; }
-__host__ __device__ constexpr int ctas_per_sm(int nb) { return nb <= 4 ? 4 : 2; }
+// positions a warp takes at a time, and a ring stage of its CTA's
+__host__ __device__ constexpr int tile_pos(int nb) { return nb <= 4 ? 64 : 32; }
+__host__ __device__ constexpr int stage_pos(int nb) { return tile_pos(nb) * kWarps; }
+__host__ __device__ constexpr int stage_bytes(int nb) { return stage_pos(nb) * 36 * nb; }
+constexpr int kStages = 2;
+// K's scales of 32 positions as fp32, per warp
+__host__ __device__ constexpr int kscale_bytes(int nb) { return 32 * 4 * nb; }
+__host__ __device__ constexpr int ctas_per_sm(int nb) { return nb <= 4 ? 3 : 2; }
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile(
@@ -175,7 +178,7 @@ __device__ __forceinline__ uint32_t pair16(const uint32_t* a, int i, const uint3
 
 // Few rows against a long cache (decode).  An item is eight rows of one
 // (sequence, kv head); its CTAs form a cluster, and every warp of it takes
-// 32 of every 128 positions its CTA takes in turn (a ring of bulk copies), with
+// a quarter of every stage its CTA takes in turn (a ring of bulk copies), with
 // its own running reference, sum and output.  The partials meet in shared
 // memory, first the CTA's, then the cluster's: no workspace, no atomics, one
 // launch.
@@ -200,7 +203,7 @@ __device__ __forceinline__ uint32_t pair16(const uint32_t* a, int i, const uint3
 template <int NB>
 __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows_kernel(const AttendArgs a) {
     constexpr int HD = 32 * NB, RB = 16 * NB, SB = 2 * NB;  // bytes of a row's quants and scales
-    constexpr int ST = stages(NB), STB = stage_bytes(NB);
+    constexpr int ST = kStages, STB = stage_bytes(NB), TP = tile_pos(NB), SP = stage_pos(NB), NT = TP / 8;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t full[ST], freed[ST];
     __shared__ float sR[kWarps + 1][8], sL[kWarps + 1][8];
@@ -215,18 +218,18 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
     if (rows <= 0) return;               // (the whole cluster)
     const int r0 = 8 * grp;
     const int len = p0 + min(n - 1, (r0 + 7) / mul) + 1;  // positions any of the rows sees
-    const int tiles = (len + kStage - 1) / kStage;  // stages in all; this CTA's: rank, rank + cs, ...
+    const int tiles = (len + SP - 1) / SP;  // stages in all; this CTA's: rank, rank + cs, ...
     const int64_t base = (int64_t)b * a.seq_rows + (int64_t)kvh * a.ctx_len;
 
     auto issue = [&](int tile, int s) {  // one thread
-        const int64_t row = base + (int64_t)tile * kStage;
-        const int np = min(kStage, (len - tile * kStage + 7) & ~7);  // (ctx_len is a multiple of 8)
+        const int64_t row = base + (int64_t)tile * SP;
+        const int np = min(SP, (len - tile * SP + 7) & ~7);  // (ctx_len is a multiple of 8)
         uint8_t* d = smem + s * STB;
         mbar_expect_tx(&full[s], (uint32_t)(np * 36 * NB));
         bulk_load(d, a.kq + row * RB, np * RB, &full[s]);
-        bulk_load(d + kStage * RB, a.vq + row * RB, np * RB, &full[s]);
-        bulk_load(d + 2 * kStage * RB, a.kd + row * NB, np * SB, &full[s]);
-        bulk_load(d + 2 * kStage * RB + kStage * SB, a.vd + row * NB, np * SB, &full[s]);
+        bulk_load(d + SP * RB, a.vq + row * RB, np * RB, &full[s]);
+        bulk_load(d + 2 * SP * RB, a.kd + row * NB, np * SB, &full[s]);
+        bulk_load(d + 2 * SP * RB + SP * SB, a.vd + row * NB, np * SB, &full[s]);
     };
     if (threadIdx.x == 0) {
         for (int s = 0; s < ST; s++) {
@@ -301,6 +304,10 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
     // column c of a score tile is position c ^ ((c >> 1) & 1) of its eight: rows
     // of both parities for the four t of a V load, and for K's
     const int kcol = g ^ ((g >> 1) & 1);
+    // this lane's position of 32 in pairs of columns: 2 * (4 * tile + t) + column & 1
+    const int mypair = (lane & 24) | (lane & 7) ^ ((lane >> 1) & 1);
+    float* kfw = reinterpret_cast<float*>(smem + ST * STB + warp * kscale_bytes(NB));
+    float* kf = kfw + (mypair >> 1) * 2 * NB + (mypair & 1);
     const int c0 = (2 * t) ^ (t & 1), c1 = (2 * t + 1) ^ (t & 1);
 
     __syncthreads();  // the barriers are set up
@@ -319,63 +326,71 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
             ok = false;
             if (lane == 0) atomicOr(a.err, kErrTimeout);
         }
-        const uint8_t* sk = smem + s * STB + warp * kTile * RB;
-        const uint8_t* sv = sk + kStage * RB;
-        uint8_t* skd = smem + s * STB + 2 * kStage * RB + warp * kTile * SB;
-        uint8_t* svd = skd + kStage * SB;
-        const int first = tile * kStage + warp * kTile;
-        if (first + kTile > len && first + lane >= len) {
-            // rows past the end (the last stage): no scale
-            for (int j = 0; j < NB; j++) {
-                reinterpret_cast<uint16_t*>(skd + lane * SB)[j] = 0;
-                reinterpret_cast<uint16_t*>(svd + lane * SB)[j] = 0;
-            }
-        }
-        __syncwarp();
+        const uint8_t* sk = smem + s * STB + warp * TP * RB;
+        const uint8_t* sv = sk + SP * RB;
+        const uint8_t* skd = smem + s * STB + 2 * SP * RB + warp * TP * SB;
+        uint8_t* svd = smem + s * STB + 2 * SP * RB + SP * SB + warp * TP * SB;
+        const int first = tile * SP + warp * TP;
 
         // ---- scores ----
-        float2 p[4];
+        float2 p[NT];
         float top = -INFINITY;
 #pragma unroll
-        for (int nt = 0; nt < 4; nt++) {
-            uint32_t w[NB], d0[(NB + 1) / 2], d1[(NB + 1) / 2];
-            lds_words<NB>(w, sk + (8 * nt + kcol) * RB + t * 4 * NB);
-            lds_halves<NB>(d0, skd + (8 * nt + c0) * SB);
-            lds_halves<NB>(d1, skd + (8 * nt + c1) * SB);
-            p[nt] = make_float2(0.f, 0.f);
+        for (int half = 0; half < TP / 32; half++) {
+            {  // the scales as fp32, the two columns of a thread side by side
+                uint32_t h[(NB + 1) / 2];
+                lds_halves<NB>(h, skd + (32 * half + lane) * SB);
+                if (half) __syncwarp();
 #pragma unroll
-            for (int j = 0; j < NB; j++) {
-                const uint32_t x = pair16(w, j, w, NB + j), y = x >> 8;
-                float c[4] = {0.f, 0.f, 0.f, 0.f};
-                mma(c, &qa[j][0], x & 0x000F000Fu, x & 0x00F000F0u, c);
-                mma(c, &qa[j][4], y & 0x000F000Fu, y & 0x00F000F0u, c);
-                p[nt] = fma2(make_float2(half_at(d0, j), half_at(d1, j)),
-                             add2(make_float2(c[0], c[1]), add2(make_float2(c[2], c[3]), bias[j])), p[nt]);
+                for (int j = 0; j < NB; j++) kf[2 * j] = half_at(h, j);
+                __syncwarp();
+            }
+#pragma unroll
+            for (int n4 = 0; n4 < 4; n4++) {
+                const int nt = 4 * half + n4;
+                uint32_t w[NB];
+                lds_words<NB>(w, sk + (8 * nt + kcol) * RB + t * 4 * NB);
+                const float2* d = reinterpret_cast<const float2*>(kfw + (4 * n4 + t) * 2 * NB);
+                p[nt] = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int j = 0; j < NB; j++) {
+                    const uint32_t x = pair16(w, j, w, NB + j), y = x >> 8;
+                    float c[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma(c, &qa[j][0], x & 0x000F000Fu, x & 0x00F000F0u, c);
+                    mma(c, &qa[j][4], y & 0x000F000Fu, y & 0x00F000F0u, c);
+                    p[nt] = fma2(d[j], add2(make_float2(c[0], c[1]), add2(make_float2(c[2], c[3]), bias[j])), p[nt]);
+                }
             }
         }
-        if (first + kTile > seen_by_all) {  // positions some row does not see
+        if (first + TP > seen_by_all) {  // positions some row does not see
 #pragma unroll
-            for (int nt = 0; nt < 4; nt++) {
+            for (int nt = 0; nt < NT; nt++) {
                 if (first + 8 * nt + c0 > limit) p[nt].x = -INFINITY;
                 if (first + 8 * nt + c1 > limit) p[nt].y = -INFINITY;
             }
         }
 #pragma unroll
-        for (int nt = 0; nt < 4; nt++) top = fmaxf(top, fmaxf(p[nt].x, p[nt].y));
+        for (int nt = 0; nt < NT; nt++) top = fmaxf(top, fmaxf(p[nt].x, p[nt].y));
         top *= factor;
 
-        // ---- reference and scale (a lane looks at one position's V scales) ----
+        // ---- reference, and V's scales: a lane takes the positions lane, lane + 32 ----
         {
-            uint32_t h[(NB + 1) / 2], mx = 0;
-            lds_halves<NB>(h, svd + lane * SB);
+            uint32_t h[TP / 32][(NB + 1) / 2], mx = 0;
 #pragma unroll
-            for (int j = 0; j < (NB + 1) / 2; j++) mx = __vmaxu2(mx, h[j] & 0x7FFF7FFFu);
+            for (int k = 0; k < TP / 32; k++) {
+                lds_halves<NB>(h[k], svd + (32 * k + lane) * SB);
+#pragma unroll
+                for (int j = 0; j < (NB + 1) / 2; j++) {
+                    if (first + 32 * k + lane >= len) h[k][j] = 0;  // (rows past the end hold anything)
+                    mx = __vmaxu2(mx, h[k][j] & 0x7FFF7FFFu);
+                }
+            }
             mx = max(mx & 0xFFFFu, mx >> 16);
             if (__any_sync(0xffffffffu, top > R + (kPeak + kLazy) || mx > dtop)) {
                 float grow = 1.f;
                 mx = __reduce_max_sync(0xffffffffu, mx);
                 if (mx > dtop) {
-                    // the scales lie below 2^(E - 14), E the exponent field
+                    // the scales lie below 2^E
                     dtop = mx | 0x3FFu;
                     const int E = (int)(dtop >> 10) - 14, ne = E >= -6 && E <= 2 ? 0 : min(2 - E, 15);
                     grow = fresh ? 1.f : exp2f((float)(ne - e2));
@@ -398,71 +413,85 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
                     o[j].y *= al;
                 }
             }
-            if (e2 != 0) {
-                const uint32_t f = (uint32_t)(15 + e2) << 10;  // e2 is in -14..15
+            const uint32_t f = (uint32_t)(15 + e2) * 0x04000400u;  // 2^e2 (-14..15), twice
+            __syncwarp();
 #pragma unroll
-                for (int j = 0; j < NB; j++) {
-                    uint16_t* q = reinterpret_cast<uint16_t*>(svd + lane * SB) + j;
-                    *q = (uint16_t)h2_mul(*q, f);
+            for (int k = 0; k < TP / 32; k++)
+#pragma unroll
+                for (int j = 0; j < NB; j += 2) {
+                    const uint32_t v = h2_mul(h[k][j / 2], f);
+                    uint16_t* q = reinterpret_cast<uint16_t*>(svd) + (32 * k * NB / 2 + mypair / 2 * NB + j) * 2 + (mypair & 1);
+                    q[0] = (uint16_t)v;
+                    if (j + 1 < NB) q[2] = (uint16_t)(v >> 16);
                 }
-                fence_proxy_async();  // (the ring's next copy into this place comes after)
-                __syncwarp();
-            }
-        }
-#pragma unroll
-        for (int nt = 0; nt < 4; nt++) {
-            p[nt].x = ex2(fmaf(p[nt].x, factor, -R));
-            p[nt].y = ex2(fmaf(p[nt].y, factor, -R));
-            l2 = add2(l2, p[nt]);
+            fence_proxy_async();  // (the next copy into this stage comes after)
+            __syncwarp();
         }
 
         // ---- output ----
-        uint32_t hi[4], lo[4];
+        uint32_t hi[NT], lo[NT];
 #pragma unroll
-        for (int nt = 0; nt < 4; nt++) split2(p[nt].x, p[nt].y, hi[nt], lo[nt]);
+        for (int nt = 0; nt < NT; nt++) {
+            p[nt].x = ex2(fmaf(p[nt].x, factor, -R));
+            p[nt].y = ex2(fmaf(p[nt].y, factor, -R));
+            l2 = add2(l2, p[nt]);
+            split2(p[nt].x, p[nt].y, hi[nt], lo[nt]);
+        }
 #pragma unroll
-        for (int jp = 0; jp < NB; jp += 2) {  // two blocks: one word of a chunk, one of the scales
-            uint32_t w[8], d[8];
+        for (int jp = 0; jp < NB; jp += 2) {  // two blocks: one word of a chunk
+            uint32_t w[2 * NT], d[2][NT];
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const int r = 8 * (k >> 1) + ((k & 1) ? c1 : c0);
+            for (int nt = 0; nt < NT; nt++) {
+                const uint32_t* dp = reinterpret_cast<const uint32_t*>(svd) + (4 * nt + t) * NB + jp;
                 if constexpr (NB % 2 == 0) {
-                    w[k] = *reinterpret_cast<const uint32_t*>(sv + r * RB + g * 2 * NB + 2 * jp);
-                    d[k] = *reinterpret_cast<const uint32_t*>(svd + r * SB + 2 * jp);
+                    const uint2 v = *reinterpret_cast<const uint2*>(dp);
+                    d[0][nt] = v.x;
+                    d[1][nt] = v.y;
                 } else {
-                    const uint16_t* wp = reinterpret_cast<const uint16_t*>(sv + r * RB + g * 2 * NB) + jp;
-                    const uint16_t* dp = reinterpret_cast<const uint16_t*>(svd + r * SB) + jp;
-                    w[k] = (uint32_t)wp[0] | (jp + 1 < NB ? (uint32_t)wp[1] << 16 : 0u);
-                    d[k] = (uint32_t)dp[0] | (jp + 1 < NB ? (uint32_t)dp[1] << 16 : 0u);
+                    d[0][nt] = dp[0];
+                    d[1][nt] = jp + 1 < NB ? dp[1] : 0u;
+                }
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const uint8_t* wp = sv + (8 * nt + (u ? c1 : c0)) * RB + g * 2 * NB + 2 * jp;
+                    if constexpr (NB % 2 == 0)
+                        w[2 * nt + u] = *reinterpret_cast<const uint32_t*>(wp);
+                    else
+                        w[2 * nt + u] = (uint32_t) * reinterpret_cast<const uint16_t*>(wp) |
+                                        (jp + 1 < NB ? (uint32_t) reinterpret_cast<const uint16_t*>(wp)[1] << 16 : 0u);
                 }
             }
 #pragma unroll
             for (int jj = 0; jj < 2; jj++) {
                 if (jp + jj >= NB) break;
                 const int j = jp + jj;
-                uint32_t af[2][4], x[4];
+                uint32_t af[NT / 2][4], x[NT];
 #pragma unroll
-                for (int nt = 0; nt < 4; nt++) {
-                    const uint32_t dd = pair16(&d[2 * nt], jj, &d[2 * nt + 1], jj);
-                    const uint32_t h = h2_mul(hi[nt], dd);
+                for (int nt = 0; nt < NT; nt++) {
+                    const uint32_t dd = d[jj][nt], h = h2_mul(hi[nt], dd);
                     af[nt >> 1][2 * (nt & 1)] = h;
                     af[nt >> 1][2 * (nt & 1) + 1] = h2_fma(lo[nt], dd, h2_fms(hi[nt], dd, h));
                     x[nt] = pair16(&w[2 * nt], jj, &w[2 * nt + 1], jj);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    uint32_t bf[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        if (i & 1)  // 1024 + 16 level -> level - 8
-                            bf[k] = h2_fma(lop3_and_or(x[k], 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u);
-                        else  // 1024 + level -> level - 8
-                            bf[k] = h2_sub(lop3_and_or(x[k], 0x000F000Fu, 0x64006400u), 0x64086408u);
-                        if (i == 1) x[k] >>= 8;
-                    }
                     float c[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma(c, af[0], bf[0], bf[1], c);
-                    mma(c, af[1], bf[2], bf[3], c);
+#pragma unroll
+                    for (int k = 0; k < NT / 2; k++) {
+                        uint32_t b0, b1;
+                        if (i & 1) {  // 1024 + 16 level -> level - 8
+                            b0 = h2_fma(lop3_and_or(x[2 * k], 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u);
+                            b1 = h2_fma(lop3_and_or(x[2 * k + 1], 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u);
+                        } else {  // 1024 + level -> level - 8
+                            b0 = h2_sub(lop3_and_or(x[2 * k], 0x000F000Fu, 0x64006400u), 0x64086408u);
+                            b1 = h2_sub(lop3_and_or(x[2 * k + 1], 0x000F000Fu, 0x64006400u), 0x64086408u);
+                        }
+                        mma(c, af[k], b0, b1, c);
+                        if (i == 1) {
+                            x[2 * k] >>= 8;
+                            x[2 * k + 1] >>= 8;
+                        }
+                    }
                     o[4 * j + i] = add2(o[4 * j + i], add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])));
                 }
             }
@@ -564,7 +593,7 @@ RowsFn rows_fn(int hd) {
 }
 
 size_t rows_smem(int nb) {
-    const size_t ring = (size_t)stages(nb) * stage_bytes(nb), merge = (size_t)(kWarps + 1) * 8 * 32 * nb * 4;
+    const size_t ring = (size_t)kStages * stage_bytes(nb) + kWarps * kscale_bytes(nb), merge = (size_t)(kWarps + 1) * 8 * 32 * nb * 4;
     return ring > merge ? ring : merge;
 }
 
@@ -600,7 +629,7 @@ int kvq4_attend(cn_ctx* ctx, const cn_kvq4& c, const float* q, int64_t q_stride,
     // CTAs per item: as many as the SMs hold at once , and no more
     // than give every warp a tile of the longest sequence
     const int nb = c.head_dim / 32, per_sm = ctas_per_sm(nb);
-    const int64_t room = (int64_t)ctx->sms * per_sm, most = (c.ctx_len + kStage - 1) / kStage;
+    const int64_t room = (int64_t)ctx->sms * per_sm, most = (c.ctx_len + stage_pos(nb) - 1) / stage_pos(nb);
     int cluster = 1;
     const char* env = getenv("KVQ4_CS");
     if (env) cluster = atoi(env);
