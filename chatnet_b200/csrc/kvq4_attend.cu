@@ -34,13 +34,14 @@ constexpr float kPeak = 9.f;     // a weight is 2^9 at the row's reference
 constexpr float kLazy = 4.f;     // a row's reference moves only when the maximum outgrows it by 2^4
 constexpr int kMaxCluster = 16;
 
-// positions a warp takes at a time, and a ring stage of its CTA's
-__host__ __device__ constexpr int tile_pos(int nb) { return nb <= 4 ? 64 : 32; }
-__host__ __device__ constexpr int stage_pos(int nb) { return tile_pos(nb) * kWarps; }
-__host__ __device__ constexpr int stage_bytes(int nb) { return stage_pos(nb) * 36 * nb; }
-constexpr int kStages = 2;
-// K's scales of 32 positions as fp32, per warp
-__host__ __device__ constexpr int kscale_bytes(int nb) { return 32 * 4 * nb; }
+// positions of a warp's tile, bytes of a tile in the ring (quants and scales of K and V)
+__host__ __device__ constexpr int tile_pos(int nb) { return nb <= 4 ? 48 : 32; }
+__host__ __device__ constexpr int tile_bytes(int nb) { return tile_pos(nb) * 36 * nb; }
+constexpr int kRing = 2;  // tiles in a warp's ring
+// a tile's scales laid out for the fragments (K's as fp32, then V's as fp16), per warp
+__host__ __device__ constexpr int scale_bytes(int nb) { return tile_pos(nb) * 4 * nb; }
+// the rows' query fragments
+__host__ __device__ constexpr int query_bytes(int nb) { return 32 * 32 * nb; }
 __host__ __device__ constexpr int ctas_per_sm(int nb) { return nb <= 4 ? 3 : 2; }
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -178,8 +179,8 @@ __device__ __forceinline__ uint32_t pair16(const uint32_t* a, int i, const uint3
 
 // Few rows against a long cache (decode).  An item is eight rows of one
 // (sequence, kv head); its CTAs form a cluster, and every warp of it takes
-// a quarter of every stage its CTA takes in turn (a ring of bulk copies), with
-// its own running reference, sum and output.  The partials meet in shared
+// every so-manieth tile of 48 positions through a ring of bulk copies of its own,
+// with its own running reference, sum and output.  The partials meet in shared
 // memory, first the CTA's, then the cluster's: no workspace, no atomics, one
 // launch.
 //
@@ -203,9 +204,9 @@ __device__ __forceinline__ uint32_t pair16(const uint32_t* a, int i, const uint3
 template <int NB>
 __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows_kernel(const AttendArgs a) {
     constexpr int HD = 32 * NB, RB = 16 * NB, SB = 2 * NB;  // bytes of a row's quants and scales
-    constexpr int ST = kStages, STB = stage_bytes(NB), TP = tile_pos(NB), SP = stage_pos(NB), NT = TP / 8;
+    constexpr int TP = tile_pos(NB), TB = tile_bytes(NB), NT = TP / 8;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ uint64_t full[ST], freed[ST];
+    __shared__ uint64_t full[kWarps][kRing];
     __shared__ float sR[kWarps + 1][8], sL[kWarps + 1][8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t cs = cluster_size(), rank = cluster_rank();
@@ -218,32 +219,35 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
     if (rows <= 0) return;               // (the whole cluster)
     const int r0 = 8 * grp;
     const int len = p0 + min(n - 1, (r0 + 7) / mul) + 1;  // positions any of the rows sees
-    const int tiles = (len + SP - 1) / SP;  // stages in all; this CTA's: rank, rank + cs, ...
+    const int tiles = (len + TP - 1) / TP, step = (int)cs * kWarps;  // this warp's: tile0, tile0 + step, ...
+    const int tile0 = (int)rank * kWarps + warp;
     const int64_t base = (int64_t)b * a.seq_rows + (int64_t)kvh * a.ctx_len;
+    uint8_t* ring = smem + warp * kRing * TB;
+    float* fs = reinterpret_cast<float*>(smem + kWarps * kRing * TB + warp * scale_bytes(NB));
+    uint4* qs = reinterpret_cast<uint4*>(smem + kWarps * (kRing * TB + scale_bytes(NB)));  // [2 NB][32]
 
-    auto issue = [&](int tile, int s) {  // one thread
-        const int64_t row = base + (int64_t)tile * SP;
-        const int np = min(SP, (len - tile * SP + 7) & ~7);  // (ctx_len is a multiple of 8)
-        uint8_t* d = smem + s * STB;
-        mbar_expect_tx(&full[s], (uint32_t)(np * 36 * NB));
-        bulk_load(d, a.kq + row * RB, np * RB, &full[s]);
-        bulk_load(d + SP * RB, a.vq + row * RB, np * RB, &full[s]);
-        bulk_load(d + 2 * SP * RB, a.kd + row * NB, np * SB, &full[s]);
-        bulk_load(d + 2 * SP * RB + SP * SB, a.vd + row * NB, np * SB, &full[s]);
+    auto issue = [&](int tile, int s) {  // one lane
+        const int64_t row = base + (int64_t)tile * TP;
+        const int np = min(TP, (len - tile * TP + 7) & ~7);  // (ctx_len is a multiple of 8)
+        uint8_t* d = ring + s * TB;
+        uint64_t* bar = &full[warp][s];
+        mbar_expect_tx(bar, (uint32_t)(np * 36 * NB));
+        bulk_load(d, a.kq + row * RB, np * RB, bar);
+        bulk_load(d + TP * RB, a.vq + row * RB, np * RB, bar);
+        bulk_load(d + 2 * TP * RB, a.kd + row * NB, np * SB, bar);
+        bulk_load(d + 2 * TP * RB + TP * SB, a.vd + row * NB, np * SB, bar);
     };
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < ST; s++) {
-            mbar_init(&full[s], 1);
-            mbar_init(&freed[s], kWarps);
-        }
+    if (lane == 0) {
+        for (int s = 0; s < kRing; s++) mbar_init(&full[warp][s], 1);
         fence_mbar_init();
         fence_proxy_async();
-        for (int s = 0; s < ST; s++)
-            if ((int)(rank + s * cs) < tiles) issue((int)(rank + s * cs), s);
+        for (int s = 0; s < kRing; s++)
+            if (tile0 + s * step < tiles) issue(tile0 + s * step, s);
     }
 
-    // the rows' queries as A fragments; limit = last position the row sees
-    uint32_t qa[NB][8];
+    // the rows' queries as A fragments in shared memory (every warp needs a
+    // row's maximum, block j is left by warp j % kWarps); limit = last position
+    // the row sees
     float2 bias[NB];
     float factor;
     int limit;
@@ -270,6 +274,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
 #pragma unroll
         for (int j = 0; j < NB; j++) {
             float sum_hi = 0.f, sum_lo = 0.f;
+            uint32_t qa[8];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const float m = (i & 1) ? 0.0625f : 1.f;
@@ -280,8 +285,12 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
                 sum_hi += h0 + h1;
                 sum_lo += (lf.x + lf.y) * ((i & 1) ? 16.f : 1.f);
                 // a0 / a1: high and low halves of k 2t, 2t+1; a2 / a3: of k 2t+8, 2t+9
-                qa[j][4 * (i >> 1) + 2 * (i & 1)] = hi;
-                qa[j][4 * (i >> 1) + 2 * (i & 1) + 1] = lo;
+                qa[4 * (i >> 1) + 2 * (i & 1)] = hi;
+                qa[4 * (i >> 1) + 2 * (i & 1) + 1] = lo;
+            }
+            if (j % kWarps == warp) {
+                qs[64 * j + lane] = make_uint4(qa[0], qa[1], qa[2], qa[3]);
+                qs[64 * j + 32 + lane] = make_uint4(qa[4], qa[5], qa[6], qa[7]);
             }
 #pragma unroll
             for (int k = 1; k <= 2; k <<= 1) {
@@ -304,64 +313,58 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
     // column c of a score tile is position c ^ ((c >> 1) & 1) of its eight: rows
     // of both parities for the four t of a V load, and for K's
     const int kcol = g ^ ((g >> 1) & 1);
-    // this lane's position of 32 in pairs of columns: 2 * (4 * tile + t) + column & 1
-    const int mypair = (lane & 24) | (lane & 7) ^ ((lane >> 1) & 1);
-    float* kfw = reinterpret_cast<float*>(smem + ST * STB + warp * kscale_bytes(NB));
-    float* kf = kfw + (mypair >> 1) * 2 * NB + (mypair & 1);
     const int c0 = (2 * t) ^ (t & 1), c1 = (2 * t + 1) ^ (t & 1);
-
-    __syncthreads();  // the barriers are set up
-    int s = 0, it = 0;
+    // where position `lane` of 32 goes among the pairs of columns: 2 * (4 * (tile of 8) + t) + (column & 1)
+    const int mypair = (lane & 24) | ((lane & 7) ^ ((lane >> 1) & 1));
+    __syncthreads();  // the queries
+    int s = 0;
     uint32_t parity = 0;
-    for (int tile = (int)rank; tile < tiles; tile += (int)cs, it++) {
-        // the stage of the step before is filled again once every warp is done
-        // with it; the warps take turns
-        if (it > 0 && warp == (it & (kWarps - 1)) && lane == 0 && ok && tile + (ST - 1) * (int)cs < tiles) {
-            const int ps = s ? s - 1 : ST - 1;
-            ok = mbar_wait(&freed[ps], s ? parity : parity ^ 1);
-            if (ok) issue(tile + (ST - 1) * (int)cs, ps);
-            else atomicOr(a.err, kErrTimeout);
-        }
-        if (ok && !mbar_wait(&full[s], parity)) {
+    for (int tile = tile0; tile < tiles; tile += step) {
+        if (ok && !mbar_wait(&full[warp][s], parity)) {
             ok = false;
             if (lane == 0) atomicOr(a.err, kErrTimeout);
         }
-        const uint8_t* sk = smem + s * STB + warp * TP * RB;
-        const uint8_t* sv = sk + SP * RB;
-        const uint8_t* skd = smem + s * STB + 2 * SP * RB + warp * TP * SB;
-        uint8_t* svd = smem + s * STB + 2 * SP * RB + SP * SB + warp * TP * SB;
-        const int first = tile * SP + warp * TP;
+        const uint8_t* sk = ring + s * TB;
+        const uint8_t* sv = sk + TP * RB;
+        const uint8_t* skd = sv + TP * RB;
+        const uint8_t* svd = skd + TP * SB;
+        const int first = tile * TP;
 
         // ---- scores ----
+        // K's scales as fp32, the two columns of a thread side by side
+#pragma unroll
+        for (int k = 0; k < TP; k += 32) {
+            if (k + 32 > TP && lane >= TP - k) break;
+            uint32_t h[(NB + 1) / 2];
+            lds_halves<NB>(h, skd + (k + lane) * SB);
+#pragma unroll
+            for (int j = 0; j < NB; j++) fs[(k / 2 + (mypair >> 1)) * 2 * NB + 2 * j + (mypair & 1)] = half_at(h, j);
+        }
+        __syncwarp();
         float2 p[NT];
-        float top = -INFINITY;
+        {
+            uint32_t w[NT][NB];
 #pragma unroll
-        for (int half = 0; half < TP / 32; half++) {
-            {  // the scales as fp32, the two columns of a thread side by side
-                uint32_t h[(NB + 1) / 2];
-                lds_halves<NB>(h, skd + (32 * half + lane) * SB);
-                if (half) __syncwarp();
-#pragma unroll
-                for (int j = 0; j < NB; j++) kf[2 * j] = half_at(h, j);
-                __syncwarp();
+            for (int nt = 0; nt < NT; nt++) {
+                lds_words<NB>(w[nt], sk + (8 * nt + kcol) * RB + t * 4 * NB);
+                p[nt] = make_float2(0.f, 0.f);
             }
 #pragma unroll
-            for (int n4 = 0; n4 < 4; n4++) {
-                const int nt = 4 * half + n4;
-                uint32_t w[NB];
-                lds_words<NB>(w, sk + (8 * nt + kcol) * RB + t * 4 * NB);
-                const float2* d = reinterpret_cast<const float2*>(kfw + (4 * n4 + t) * 2 * NB);
-                p[nt] = make_float2(0.f, 0.f);
+            for (int j = 0; j < NB; j++) {
+                const uint4 qa = qs[64 * j + lane], qb = qs[64 * j + 32 + lane];
+                const uint32_t a0[4] = {qa.x, qa.y, qa.z, qa.w}, a1[4] = {qb.x, qb.y, qb.z, qb.w};
 #pragma unroll
-                for (int j = 0; j < NB; j++) {
-                    const uint32_t x = pair16(w, j, w, NB + j), y = x >> 8;
+                for (int nt = 0; nt < NT; nt++) {
+                    const uint32_t x = pair16(w[nt], j, w[nt], NB + j), y = x >> 8;
                     float c[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma(c, &qa[j][0], x & 0x000F000Fu, x & 0x00F000F0u, c);
-                    mma(c, &qa[j][4], y & 0x000F000Fu, y & 0x00F000F0u, c);
-                    p[nt] = fma2(d[j], add2(make_float2(c[0], c[1]), add2(make_float2(c[2], c[3]), bias[j])), p[nt]);
+                    mma(c, a0, x & 0x000F000Fu, x & 0x00F000F0u, c);
+                    mma(c, a1, y & 0x000F000Fu, y & 0x00F000F0u, c);
+                    const float2 d = reinterpret_cast<const float2*>(fs)[(4 * nt + t) * NB + j];
+                    p[nt] = fma2(d, add2(make_float2(c[0], c[1]), add2(make_float2(c[2], c[3]), bias[j])), p[nt]);
                 }
             }
         }
+        float top = -INFINITY;
         if (first + TP > seen_by_all) {  // positions some row does not see
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
@@ -373,15 +376,18 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
         for (int nt = 0; nt < NT; nt++) top = fmaxf(top, fmaxf(p[nt].x, p[nt].y));
         top *= factor;
 
-        // ---- reference, and V's scales: a lane takes the positions lane, lane + 32 ----
+        // ---- reference, and V's scales ----
         {
-            uint32_t h[TP / 32][(NB + 1) / 2], mx = 0;
+            constexpr int K = (TP + 31) / 32;
+            uint32_t h[K][(NB + 1) / 2], mx = 0;
 #pragma unroll
-            for (int k = 0; k < TP / 32; k++) {
-                lds_halves<NB>(h[k], svd + (32 * k + lane) * SB);
+            for (int k = 0; k < K; k++) {
+                const int q = 32 * k + lane;
+                const bool in = (32 * k + 32 <= TP || q < TP) && first + q < len;  // (rows past the end hold anything)
+                lds_halves<NB>(h[k], svd + (in ? q : 0) * SB);
 #pragma unroll
                 for (int j = 0; j < (NB + 1) / 2; j++) {
-                    if (first + 32 * k + lane >= len) h[k][j] = 0;  // (rows past the end hold anything)
+                    if (!in) h[k][j] = 0;
                     mx = __vmaxu2(mx, h[k][j] & 0x7FFF7FFFu);
                 }
             }
@@ -414,17 +420,18 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
                 }
             }
             const uint32_t f = (uint32_t)(15 + e2) * 0x04000400u;  // 2^e2 (-14..15), twice
-            __syncwarp();
+            __syncwarp();  // (K's are read)
 #pragma unroll
-            for (int k = 0; k < TP / 32; k++)
+            for (int k = 0; k < K; k++) {
+                if (32 * k + 32 > TP && lane >= TP - 32 * k) break;
 #pragma unroll
                 for (int j = 0; j < NB; j += 2) {
                     const uint32_t v = h2_mul(h[k][j / 2], f);
-                    uint16_t* q = reinterpret_cast<uint16_t*>(svd) + (32 * k * NB / 2 + mypair / 2 * NB + j) * 2 + (mypair & 1);
+                    uint16_t* q = reinterpret_cast<uint16_t*>(fs) + ((16 * k + (mypair >> 1)) * NB + j) * 2 + (mypair & 1);
                     q[0] = (uint16_t)v;
                     if (j + 1 < NB) q[2] = (uint16_t)(v >> 16);
                 }
-            fence_proxy_async();  // (the next copy into this stage comes after)
+            }
             __syncwarp();
         }
 
@@ -442,7 +449,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
             uint32_t w[2 * NT], d[2][NT];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                const uint32_t* dp = reinterpret_cast<const uint32_t*>(svd) + (4 * nt + t) * NB + jp;
+                const uint32_t* dp = reinterpret_cast<const uint32_t*>(fs) + (4 * nt + t) * NB + jp;
                 if constexpr (NB % 2 == 0) {
                     const uint2 v = *reinterpret_cast<const uint2*>(dp);
                     d[0][nt] = v.x;
@@ -497,8 +504,8 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
             }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&freed[s]);
-        if (++s == ST) {
+        if (lane == 0 && ok && tile + kRing * step < tiles) issue(tile + kRing * step, s);
+        if (++s == kRing) {
             s = 0;
             parity ^= 1;
         }
@@ -593,7 +600,7 @@ RowsFn rows_fn(int hd) {
 }
 
 size_t rows_smem(int nb) {
-    const size_t ring = (size_t)kStages * stage_bytes(nb) + kWarps * kscale_bytes(nb), merge = (size_t)(kWarps + 1) * 8 * 32 * nb * 4;
+    const size_t ring = (size_t)kWarps * (kRing * tile_bytes(nb) + scale_bytes(nb)) + query_bytes(nb), merge = (size_t)(kWarps + 1) * 8 * 32 * nb * 4;
     return ring > merge ? ring : merge;
 }
 
@@ -629,7 +636,7 @@ int kvq4_attend(cn_ctx* ctx, const cn_kvq4& c, const float* q, int64_t q_stride,
     // CTAs per item: as many as the SMs hold at once , and no more
     // than give every warp a tile of the longest sequence
     const int nb = c.head_dim / 32, per_sm = ctas_per_sm(nb);
-    const int64_t room = (int64_t)ctx->sms * per_sm, most = (c.ctx_len + stage_pos(nb) - 1) / stage_pos(nb);
+    const int64_t room = (int64_t)ctx->sms * per_sm, most = (c.ctx_len + kWarps * tile_pos(nb) - 1) / (kWarps * tile_pos(nb));
     int cluster = 1;
     const char* env = getenv("KVQ4_CS");
     if (env) cluster = atoi(env);
