@@ -22,7 +22,7 @@ struct AttendArgs {
     const uint8_t *kq, *vq;
     const __half *kd, *vd;
     int64_t seq_rows;
-    int n_new, n_heads, n_kv, ctx_len, neox, groups;
+    int batch, n_new, n_heads, n_kv, ctx_len, neox, groups;
     float scale;
     uint32_t* err;
 };
@@ -211,7 +211,18 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t cs = cluster_size(), rank = cluster_rank();
     const int item = (int)(blockIdx.x / cs);
-    const int grp = item % a.groups, bh = item / a.groups, kvh = bh % a.n_kv, b = bh / a.n_kv;
+    const int grp = item % a.groups, bh = item / a.groups, kvh = bh % a.n_kv;
+    int b = bh / a.n_kv;
+    if (a.batch > 1 && a.batch <= 32) {
+        // the longest sequences first: what starts last is short
+        const int mine = lane < a.batch ? a.pos[lane] : -1;
+        int before = 0;
+        for (int k = 0; k < a.batch; k++) {
+            const int other = __shfl_sync(0xffffffffu, mine, k);
+            before += other > mine || (other == mine && k < lane);
+        }
+        b = __ffs(__ballot_sync(0xffffffffu, lane < a.batch && before == b)) - 1;
+    }
     const int mul = a.n_heads / a.n_kv;
     int p0;
     const int n = kvq4_active(a.pos, a.count, b, a.n_new, a.ctx_len, p0);
@@ -353,14 +364,23 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
             for (int j = 0; j < NB; j++) {
                 const uint4 qa = qs[64 * j + lane], qb = qs[64 * j + 32 + lane];
                 const uint32_t a0[4] = {qa.x, qa.y, qa.z, qa.w}, a1[4] = {qb.x, qb.y, qb.z, qb.w};
+                float c[NT][4];
+                uint32_t y[NT];
+                // (the tiles side by side: an MMA's result is long in coming)
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    const uint32_t x = pair16(w[nt], j, w[nt], NB + j), y = x >> 8;
-                    float c[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma(c, a0, x & 0x000F000Fu, x & 0x00F000F0u, c);
-                    mma(c, a1, y & 0x000F000Fu, y & 0x00F000F0u, c);
+                    const uint32_t x = pair16(w[nt], j, w[nt], NB + j);
+                    c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.f;
+                    mma(c[nt], a0, x & 0x000F000Fu, x & 0x00F000F0u, c[nt]);
+                    y[nt] = x >> 8;
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) mma(c[nt], a1, y[nt] & 0x000F000Fu, y[nt] & 0x00F000F0u, c[nt]);
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
                     const float2 d = reinterpret_cast<const float2*>(fs)[(4 * nt + t) * NB + j];
-                    p[nt] = fma2(d, add2(make_float2(c[0], c[1]), add2(make_float2(c[2], c[3]), bias[j])), p[nt]);
+                    p[nt] = fma2(d, add2(make_float2(c[nt][0], c[nt][1]), add2(make_float2(c[nt][2], c[nt][3]), bias[j])),
+                                 p[nt]);
                 }
             }
         }
@@ -446,60 +466,74 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
         }
 #pragma unroll
         for (int jp = 0; jp < NB; jp += 2) {  // two blocks: one word of a chunk
-            uint32_t w[2 * NT], d[2][NT];
+            float c[2][4][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                const uint32_t* dp = reinterpret_cast<const uint32_t*>(fs) + (4 * nt + t) * NB + jp;
-                if constexpr (NB % 2 == 0) {
-                    const uint2 v = *reinterpret_cast<const uint2*>(dp);
-                    d[0][nt] = v.x;
-                    d[1][nt] = v.y;
-                } else {
-                    d[0][nt] = dp[0];
-                    d[1][nt] = jp + 1 < NB ? dp[1] : 0u;
+            for (int i = 0; i < 4; i++)
+                c[0][i][0] = c[0][i][1] = c[0][i][2] = c[0][i][3] = c[1][i][0] = c[1][i][1] = c[1][i][2] = c[1][i][3] = 0.f;
+#pragma unroll
+            for (int k = 0; k < NT / 2; k++) {
+                uint32_t w[4], d[2][2];
+#pragma unroll
+                for (int n2 = 0; n2 < 2; n2++) {
+                    const int nt = 2 * k + n2;
+                    const uint32_t* dp = reinterpret_cast<const uint32_t*>(fs) + (4 * nt + t) * NB + jp;
+                    if constexpr (NB % 2 == 0) {
+                        const uint2 v = *reinterpret_cast<const uint2*>(dp);
+                        d[0][n2] = v.x;
+                        d[1][n2] = v.y;
+                    } else {
+                        d[0][n2] = dp[0];
+                        d[1][n2] = jp + 1 < NB ? dp[1] : 0u;
+                    }
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const uint8_t* wp = sv + (8 * nt + (u ? c1 : c0)) * RB + g * 2 * NB + 2 * jp;
+                        if constexpr (NB % 2 == 0)
+                            w[2 * n2 + u] = *reinterpret_cast<const uint32_t*>(wp);
+                        else
+                            w[2 * n2 + u] =
+                                (uint32_t) * reinterpret_cast<const uint16_t*>(wp) |
+                                (jp + 1 < NB ? (uint32_t) reinterpret_cast<const uint16_t*>(wp)[1] << 16 : 0u);
+                    }
                 }
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const uint8_t* wp = sv + (8 * nt + (u ? c1 : c0)) * RB + g * 2 * NB + 2 * jp;
-                    if constexpr (NB % 2 == 0)
-                        w[2 * nt + u] = *reinterpret_cast<const uint32_t*>(wp);
-                    else
-                        w[2 * nt + u] = (uint32_t) * reinterpret_cast<const uint16_t*>(wp) |
-                                        (jp + 1 < NB ? (uint32_t) reinterpret_cast<const uint16_t*>(wp)[1] << 16 : 0u);
+                for (int jj = 0; jj < 2; jj++) {
+                    if (jp + jj >= NB) break;
+                    uint32_t af[4], x0, x1;
+#pragma unroll
+                    for (int n2 = 0; n2 < 2; n2++) {
+                        const uint32_t dd = d[jj][n2], h = h2_mul(hi[2 * k + n2], dd);
+                        af[2 * n2] = h;
+                        af[2 * n2 + 1] = h2_fma(lo[2 * k + n2], dd, h2_fms(hi[2 * k + n2], dd, h));
+                    }
+                    x0 = pair16(w, jj, w + 1, jj);
+                    x1 = pair16(w + 2, jj, w + 3, jj);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        uint32_t b0, b1;
+                        if (i & 1) {  // 1024 + 16 level -> level - 8
+                            b0 = h2_fma(lop3_and_or(x0, 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u);
+                            b1 = h2_fma(lop3_and_or(x1, 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u);
+                        } else {  // 1024 + level -> level - 8
+                            b0 = h2_sub(lop3_and_or(x0, 0x000F000Fu, 0x64006400u), 0x64086408u);
+                            b1 = h2_sub(lop3_and_or(x1, 0x000F000Fu, 0x64006400u), 0x64086408u);
+                        }
+                        mma(c[jj][i], af, b0, b1, c[jj][i]);
+                        if (i == 1) {
+                            x0 >>= 8;
+                            x1 >>= 8;
+                        }
+                    }
                 }
             }
 #pragma unroll
             for (int jj = 0; jj < 2; jj++) {
                 if (jp + jj >= NB) break;
-                const int j = jp + jj;
-                uint32_t af[NT / 2][4], x[NT];
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    const uint32_t dd = d[jj][nt], h = h2_mul(hi[nt], dd);
-                    af[nt >> 1][2 * (nt & 1)] = h;
-                    af[nt >> 1][2 * (nt & 1) + 1] = h2_fma(lo[nt], dd, h2_fms(hi[nt], dd, h));
-                    x[nt] = pair16(&w[2 * nt], jj, &w[2 * nt + 1], jj);
-                }
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    float c[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int k = 0; k < NT / 2; k++) {
-                        uint32_t b0, b1;
-                        if (i & 1) {  // 1024 + 16 level -> level - 8
-                            b0 = h2_fma(lop3_and_or(x[2 * k], 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u);
-                            b1 = h2_fma(lop3_and_or(x[2 * k + 1], 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u);
-                        } else {  // 1024 + level -> level - 8
-                            b0 = h2_sub(lop3_and_or(x[2 * k], 0x000F000Fu, 0x64006400u), 0x64086408u);
-                            b1 = h2_sub(lop3_and_or(x[2 * k + 1], 0x000F000Fu, 0x64006400u), 0x64086408u);
-                        }
-                        mma(c, af[k], b0, b1, c);
-                        if (i == 1) {
-                            x[2 * k] >>= 8;
-                            x[2 * k + 1] >>= 8;
-                        }
-                    }
-                    o[4 * j + i] = add2(o[4 * j + i], add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])));
+                    const float* f = c[jj][i];
+                    float2& r = o[4 * (jp + jj) + i];
+                    r = add2(r, add2(make_float2(f[0], f[1]), make_float2(f[2], f[3])));
                 }
             }
         }
@@ -622,6 +656,7 @@ int kvq4_attend(cn_ctx* ctx, const cn_kvq4& c, const float* q, int64_t q_stride,
     a.kd = static_cast<const __half*>(c.k_scales);
     a.vd = static_cast<const __half*>(c.v_scales);
     a.seq_rows = kvq4_seq_rows(c);
+    a.batch = batch;
     a.n_new = n_new;
     a.n_heads = n_heads;
     a.n_kv = c.n_kv_heads;
