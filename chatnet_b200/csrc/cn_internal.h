@@ -35,6 +35,9 @@ struct cn_ctx {
     void* samp = nullptr;
     size_t samp_bytes = 0;
 
+    // 4-bit attention kernels (by head_dim / 32) whose launch attributes are set
+    uint32_t kvq4_ready = 0;
+
     // staging for the host-pointer entry points
     void* dstage = nullptr;
     size_t dstage_bytes = 0;

@@ -51,27 +51,6 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
         : "memory");
 }
 
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-// two fp32 operations in one instruction
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;"
-        : "=l"(r)
-        : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
-    return *reinterpret_cast<float2*>(&r);
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;"
-        : "=l"(r)
-        : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)),
-          "l"(*reinterpret_cast<uint64_t*>(&c)));
-    return *reinterpret_cast<float2*>(&r);
-}
 // The halves of hi + lo = x: hi keeps 11 bits (x truncated, so the
 // conversion is exact in fp16's normal range), lo the next 11.
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
@@ -668,19 +647,22 @@ int kvq4_attend(cn_ctx* ctx, const cn_kvq4& c, const float* q, int64_t q_stride,
     const int64_t groups = (rows + 7) / 8, items = groups * c.n_kv_heads * batch;
     CN_CHECK(items < (1ll << 31) / kMaxCluster, CN_ERR_INVALID_ARG, "too many rows (%lld items)", (long long)items);
     a.groups = (int)groups;
-    // CTAs per item: as many as the SMs hold at once , and no more
-    // than give every warp a tile of the longest sequence
-    const int nb = c.head_dim / 32, per_sm = ctas_per_sm(nb);
-    const int64_t room = (int64_t)ctx->sms * per_sm, most = (c.ctx_len + kWarps * tile_pos(nb) - 1) / (kWarps * tile_pos(nb));
+    // CTAs per item: the most that all run at once (8 x 64 heads of 128 at 131
+    // thousand positions, 64 items: 372 us with 4, 301 with 6, 347 with 8), and
+    // no more than give every warp a tile of the longest sequence
+    const int nb = c.head_dim / 32;
+    const int64_t room = (int64_t)ctx->sms * ctas_per_sm(nb);
+    const int64_t most = (c.ctx_len + kWarps * tile_pos(nb) - 1) / (kWarps * tile_pos(nb));
     int cluster = 1;
-    const char* env = getenv("KVQ4_CS");
-    if (env) cluster = atoi(env);
-    else
-        while (cluster < kMaxCluster && 2 * cluster <= most && 2 * cluster * items <= room) cluster *= 2;
+    for (int k : {2, 3, 4, 6, 8, kMaxCluster})
+        if (k <= most && k * items <= room) cluster = k;
     RowsFn fn = rows_fn(c.head_dim);
     const size_t smem = rows_smem(nb);
-    CN_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    CN_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    if (!(__atomic_load_n(&ctx->kvq4_ready, __ATOMIC_RELAXED) & (1u << nb))) {
+        CN_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        CN_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        __atomic_fetch_or(&ctx->kvq4_ready, 1u << nb, __ATOMIC_RELAXED);
+    }
     CN_CUDA(launch_cluster_k(false, cluster, fn, dim3((unsigned)(items * cluster)), dim3(32 * kWarps), smem, st, a));
     return CN_OK;
 }

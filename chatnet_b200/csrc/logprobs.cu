@@ -4,6 +4,20 @@
 //
 //   m = max x, S = sum e^(x - m), T = sum (x - m) e^(x - m)
 //   logprob(t) = x_t - m - log S,   entropy = log S - T / S
+// One pass over the logits: each thread keeps its own m, S and T, which are
+// scaled to a common m at the end.  Bound: the logits' bytes, each read once.
+//
+// The alternatives come out of the same pass.  Order: larger value, then lower
+// id, NaN last, as one 64-bit key.  A CTA keeps a buffer of candidates and a
+// bound t below which nothing can be among its top n.  t starts from the first
+// chunk (each of the W warps finds the k-th largest of its lanes' maxima, k =
+// ceil(n / W); the smallest of the W has at least n values at or above it)
+// and is the n-th best key whenever the buffer is cut back to n; after the first
+// chunks next to nothing passes it.
+//
+// A row is split over a cluster of CTAs when there are few rows; their sums and
+// lists meet in the first CTA's shared memory.  No workspace, no atomics on
+// global memory, one launch.
 #include <float.h>
 
 #include "cn_common.cuh"
@@ -15,111 +29,380 @@ namespace cn {
 namespace {
 
 constexpr int kMaxTop = 64;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kPer = 16;              // values a thread takes at a time
+constexpr int kChunk = kThreads * kPer;
+constexpr int kCut = 512;             // candidates at which the buffer is cut back
+constexpr int kBuf = kCut + kChunk;   // (a chunk can add all its values)
+constexpr int kMaxCluster = 16;
 
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+using Key = unsigned long long;
 
-// An order on (value, lower index first) as one whole number: larger values
-// first, NaN after everything.
-__device__ __forceinline__ uint64_t order_key(float v, int i) {
+struct LpArgs {
+    const void* logits;
+    int64_t stride;
+    int n, top;
+    const int* tokens;
+    float *logprob, *entropy;
+    int* top_ids;
+    float* top_lp;
+};
+
+// A value's place in the order as a whole number (NaN 0).
+__device__ __forceinline__ uint32_t order32(float v) {
     const uint32_t u = __float_as_uint(v + 0.f);  // -0 as +0
-    const uint32_t o = v != v ? 0u : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-    return ((uint64_t)o << 32) | (0xFFFFFFFFu - (uint32_t)i);
+    return v != v ? 0u : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float order_value(uint32_t o) {
+    return o == 0u ? NAN : __uint_as_float((o & 0x80000000u) ? o & 0x7FFFFFFFu : ~o);
+}
+constexpr uint32_t kMinusInf = 0x007FFFFFu;  // order32(-inf)
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 
-__device__ __forceinline__ uint64_t warp_max_u64(uint64_t k) {
+// 16 bytes of logits as floats
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+    static constexpr int N = 4;
+    __device__ static void get(const uint4& u, float* x) {
+        x[0] = __uint_as_float(u.x), x[1] = __uint_as_float(u.y), x[2] = __uint_as_float(u.z),
+        x[3] = __uint_as_float(u.w);
+    }
+    __device__ static uint32_t minus_inf() { return 0xFF800000u; }
+};
+template <>
+struct Vec<__half> {
+    static constexpr int N = 8;
+    __device__ static void get(const uint4& u, float* x) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        }
+    }
+    __device__ static uint32_t minus_inf() { return 0xFC00FC00u; }
+};
+
+// The running sums of one thread.
+struct Sums {
+    float m = -INFINITY;
+    float2 S = {0.f, 0.f}, T = {0.f, 0.f};
+    __device__ void raise(float to) {  // to > m
+        if (m != -INFINITY) {
+            const float d = fmaxf(m - to, -200.f), f = expf(d);  // (0 from there on, and d stays finite)
+            T.x = f * fmaf(d, S.x, T.x), T.y = f * fmaf(d, S.y, T.y);
+            S.x *= f, S.y *= f;
+        }
+        m = to;
+    }
+    template <int N>
+    __device__ void add(const float* x) {
+        const float mu = m == -INFINITY ? 0.f : m;
+        const float2 nm = make_float2(-mu, -mu);
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            float2 d = add2(make_float2(x[i], x[i + 1]), nm);
+            // (below e^-200 nothing is left; keeps -inf * 0 out and NaN in)
+            d.x = max_nan(d.x, -200.f), d.y = max_nan(d.y, -200.f);
+            const float2 e = make_float2(ex2(d.x * 1.44269504088896341f), ex2(d.y * 1.44269504088896341f));
+            S = add2(S, e);
+            T = fma2(d, e, T);
+        }
+    }
+};
+
+// Brings sums over [m, S, T] to their common maximum; every lane gets them.
+__device__ __forceinline__ void join(float& m, float& S, float& T, float m2, float S2, float T2) {
+    const float M = fmaxf(m, m2);
+    auto scale = [&](float& s, float& t, float mi) {
+        if (mi != M && mi != -INFINITY) {
+            const float d = fmaxf(mi - M, -200.f), f = expf(d);
+            t = f * fmaf(d, s, t);
+            s *= f;
+        }
+    };
+    scale(S, T, m);
+    scale(S2, T2, m2);
+    m = M;
+    S += S2;
+    T += T2;
+}
+
+__device__ __forceinline__ Key warp_max(Key k) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        const uint64_t x = __shfl_xor_sync(0xffffffffu, k, o);
+        const Key x = __shfl_xor_sync(0xffffffffu, k, o);
         k = x > k ? x : k;
     }
     return k;
 }
 
+// The `top` largest of buf[0..cnt), largest first, into list (0 where there are
+// fewer).  Whole CTA; buf and list must be visible (a barrier before).
+__device__ void best_keys(const Key* buf, int cnt, int top, Key* list, Key* red) {
+    const int tid = threadIdx.x;
+    if (tid < top) list[tid] = 0;
+    __syncthreads();
+    if (cnt <= kCut) {
+        // a key's place is the number of larger ones
+        for (int i = tid; i < cnt; i += kThreads) {
+            const Key k = buf[i];
+            int r = 0;
+            for (int j = 0; j < cnt; j++) r += buf[j] > k;
+            if (r < top) list[r] = k;
+        }
+    } else {
+        // one after another; a thread looks again only when its own was taken
+        auto mine = [&](Key below) {
+            Key b = 0;
+            for (int i = tid; i < cnt; i += kThreads) {
+                const Key k = buf[i];
+                if (k < below && k > b) b = k;
+            }
+            return b;
+        };
+        Key own = mine(~0ull);
+        for (int r = 0; r < top; r++) {
+            const Key w = warp_max(own);
+            if ((tid & 31) == 0) red[(r & 1) * kWarps + (tid >> 5)] = w;
+            __syncthreads();
+            Key k = 0;
+#pragma unroll
+            for (int i = 0; i < kWarps; i++) {
+                const Key x = red[(r & 1) * kWarps + i];
+                k = x > k ? x : k;
+            }
+            if (tid == 0) list[r] = k;
+            if (k != 0 && own == k) own = mine(k);
+        }
+    }
+    __syncthreads();
+}
+
 }  // namespace
 
-// One CTA per row, three passes, then one pass per alternative.
-template <typename T>
-__global__ void __launch_bounds__(256)
-    logprobs_plain_kernel(const T* __restrict__ logits, int64_t stride, int n, const int* __restrict__ tokens, int top,
-                          float* __restrict__ logprob, float* __restrict__ entropy, int* __restrict__ top_ids,
-                          float* __restrict__ top_lp) {
-    __shared__ float red[3][8];
-    __shared__ uint64_t best[8];
-    const T* x = logits + (int64_t)blockIdx.x * stride;
-    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    float m = -INFINITY;
-    bool nan = false;
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const float v = to_f(x[i]);
-        nan |= v != v;
-        m = fmaxf(m, v);
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const LpArgs a) {
+    constexpr int VN = Vec<T>::N, U = kPer / VN;
+    extern __shared__ __align__(16) uint8_t smem[];
+    Key* buf = reinterpret_cast<Key*>(smem);                // [kBuf] (TOP)
+    Key* meet = buf + kBuf;                                 // [kMaxCluster][kMaxTop] the CTAs' lists (first CTA)
+    __shared__ float red[kWarps][3];
+    __shared__ float sums[kMaxCluster][3];
+    __shared__ Key kred[2 * kWarps], list[kMaxTop];
+    __shared__ uint32_t bound[kWarps];
+    __shared__ int s_count;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t cs = cluster_size(), rank = cluster_rank();
+    const int64_t row = blockIdx.x / cs;
+    if (cs > 1) cluster_arrive_relaxed();
+    if (TOP && tid == 0) s_count = 0;
+    const T* x0 = static_cast<const T*>(a.logits) + row * a.stride;
+    float xt = NAN;
+    if (rank == 0 && tid == 0 && a.logprob) {
+        const int t = a.tokens[row];
+        if (t >= 0 && t < a.n) xt = (float)x0[t];
     }
-    if (nan) m = INFINITY;  // x - inf: every result of the row is NaN or -inf
+    // the row in 16-byte pieces from the boundary at or before its start; this
+    // CTA's share of them
+    const int off = (int)((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T));
+    const uint4* v = reinterpret_cast<const uint4*>(x0 - off);
+    const int pieces = (int)(((int64_t)off + a.n + VN - 1) / VN);
+    const int v0 = (int)((int64_t)pieces * rank / cs), v1 = (int)((int64_t)pieces * (rank + 1) / cs);
+    auto load = [&](int i) -> uint4 {
+        uint4 u = make_uint4(Vec<T>::minus_inf(), Vec<T>::minus_inf(), Vec<T>::minus_inf(), Vec<T>::minus_inf());
+        if (i < v1) {
+            const int64_t e = (int64_t)i * VN - off;
+            if (e >= 0 && e + VN <= a.n) {
+                u = __ldcs(v + i);
+            } else {
+                T* p = reinterpret_cast<T*>(&u);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (!lane) red[0][w] = m;
-    __syncthreads();
-    for (int k = 0; k < 8; k++) m = fmaxf(m, red[0][k]);
-    float S = 0.f, U = 0.f;
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const float d = to_f(x[i]) - m, e = expf(d);
-        S += e;
-        if (!(e == 0.f)) U = fmaf(d, e, U);
-    }
+                for (int k = 0; k < VN; k++)
+                    if (e + k >= 0 && e + k < a.n) p[k] = x0[e + k];
+            }
+        }
+        return u;
+    };
+    uint4 cur[U], nxt[U];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        S += __shfl_xor_sync(0xffffffffu, S, o);
-        U += __shfl_xor_sync(0xffffffffu, U, o);
+    for (int k = 0; k < U; k++) cur[k] = load(v0 + k * kThreads + tid);
+    Sums sm;
+    uint32_t t_ord = 0;   // what may be among the top has order32 >= t_ord (first: > after a cut)
+    bool strict = false;
+    const int chunks = (v1 - v0 + U * kThreads - 1) / (U * kThreads);
+    for (int c = 0; c < chunks; c++) {
+        const int first = v0 + c * U * kThreads + tid;
+#pragma unroll
+        for (int k = 0; k < U; k++) nxt[k] = load(first + (U + k) * kThreads);
+        float cm = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < U; k++) {
+            float x[VN];
+            Vec<T>::get(cur[k], x);
+#pragma unroll
+            for (int i = 0; i < VN; i++) cm = fmaxf(cm, x[i]);
+        }
+        if (cm > sm.m) sm.raise(cm);
+#pragma unroll
+        for (int k = 0; k < U; k++) {
+            float x[VN];
+            Vec<T>::get(cur[k], x);
+            sm.template add<VN>(x);
+        }
+        if constexpr (TOP) {
+            const uint32_t co = order32(cm);
+            if (c == 0) {
+                // (of the warps whose lanes all have values)
+                const int warps = min(v1 - v0, kThreads) / 32;
+                const int rounds = warps ? (a.top + warps - 1) / warps : 33;
+                if (rounds <= 32) {
+                    uint32_t w = co, last = 0;
+                    for (int r = 0; r < rounds; r++) {
+                        last = __reduce_max_sync(0xffffffffu, w);
+                        if (lane == __ffs(__ballot_sync(0xffffffffu, w == last)) - 1) w = 0;
+                    }
+                    if (lane == 0) bound[warp] = warp < warps ? last : 0xFFFFFFFFu;
+                    __syncthreads();
+                    t_ord = bound[0];
+#pragma unroll
+                    for (int i = 1; i < kWarps; i++) t_ord = min(t_ord, bound[i]);
+                } else {
+                    __syncthreads();
+                }
+                // (a maximum of -inf may stand for NaN or nothing)
+                if (t_ord <= kMinusInf) t_ord = 0;
+            }
+            // (where t is -inf or NaN, NaN and -inf count too)
+            if (strict ? co > t_ord || t_ord < kMinusInf : co >= t_ord) {
+#pragma unroll
+                for (int k = 0; k < U; k++) {
+                    float x[VN];
+                    Vec<T>::get(cur[k], x);
+                    const int e = (first + k * kThreads) * VN - off;
+#pragma unroll
+                    for (int i = 0; i < VN; i++) {
+                        const uint32_t o = order32(x[i]);
+                        if ((strict ? o > t_ord : o >= t_ord) && e + i >= 0 && e + i < a.n && first + k * kThreads < v1)
+                            buf[atomicAdd(&s_count, 1)] = ((Key)o << 32) | (0xFFFFFFFFu - (uint32_t)(e + i));
+                    }
+                }
+            }
+            if (__syncthreads_or(*(volatile int*)&s_count > kCut)) {
+                const int cnt = s_count;
+                best_keys(buf, cnt, a.top, list, kred);
+                if (tid < a.top) buf[tid] = list[tid];
+                if (tid == 0) s_count = min(cnt, a.top);
+                if (cnt >= a.top) {
+                    t_ord = (uint32_t)(list[a.top - 1] >> 32);
+                    strict = true;  // (what comes later has higher ids)
+                }
+                __syncthreads();
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < U; k++) cur[k] = nxt[k];
     }
-    if (!lane) {
-        red[1][w] = S;
-        red[2][w] = U;
+    // the CTA's sums
+    float m = sm.m, S = sm.S.x + sm.S.y, Tt = sm.T.x + sm.T.y;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        join(m, S, Tt, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, S, o),
+             __shfl_xor_sync(0xffffffffu, Tt, o));
+    if (lane == 0) {
+        red[warp][0] = m;
+        red[warp][1] = S;
+        red[warp][2] = Tt;
     }
     __syncthreads();
-    S = U = 0.f;
-    for (int k = 0; k < 8; k++) {
-        S += red[1][k];
-        U += red[2][k];
+    if (TOP) best_keys(buf, s_count, a.top, list, kred);
+    if (warp == 0) {
+        const int w = lane < kWarps ? lane : 0;
+        m = lane < kWarps ? red[w][0] : -INFINITY;
+        S = lane < kWarps ? red[w][1] : 0.f;
+        Tt = lane < kWarps ? red[w][2] : 0.f;
+#pragma unroll
+        for (int o = kWarps / 2; o > 0; o >>= 1)
+            join(m, S, Tt, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, S, o),
+                 __shfl_xor_sync(0xffffffffu, Tt, o));
     }
-    const float ls = logf(S);
-    if (threadIdx.x == 0) {
-        if (entropy) entropy[blockIdx.x] = ls - U / S;
-        if (logprob) {
-            const int t = tokens[blockIdx.x];
-            logprob[blockIdx.x] = t >= 0 && t < n ? (to_f(x[t]) - m) - ls : NAN;
+    if (cs > 1) {
+        // to the first CTA
+        __syncwarp();
+        cluster_wait();  // (it has started)
+        if (tid == 0) {
+            const uint32_t d = map_rank(smem_u32(&sums[rank][0]), 0);
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(d), "f"(m) : "memory");
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(d + 4), "f"(S) : "memory");
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(d + 8), "f"(Tt) : "memory");
         }
+        if (TOP && tid < a.top)
+            asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(map_rank(smem_u32(&meet[rank * a.top + tid]), 0)),
+                         "l"(list[tid])
+                         : "memory");
+        __syncwarp();
+        cluster_arrive();
+        if (rank != 0) return;
+        cluster_wait();
+        if (warp == 0) {
+            m = lane < (int)cs ? sums[lane & (kMaxCluster - 1)][0] : -INFINITY;
+            S = lane < (int)cs ? sums[lane & (kMaxCluster - 1)][1] : 0.f;
+            Tt = lane < (int)cs ? sums[lane & (kMaxCluster - 1)][2] : 0.f;
+#pragma unroll
+            for (int o = kMaxCluster / 2; o > 0; o >>= 1)
+                join(m, S, Tt, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, S, o),
+                     __shfl_xor_sync(0xffffffffu, Tt, o));
+        }
+        if (TOP) best_keys(meet, (int)cs * a.top, a.top, list, kred);
     }
-    uint64_t last = ~0ull;
-    for (int k = 0; k < top; k++) {
-        uint64_t bk = 0;
-        for (int i = threadIdx.x; i < n; i += 256) {
-            const uint64_t key = order_key(to_f(x[i]), i);
-            if (key < last && key > bk) bk = key;
-        }
-        bk = warp_max_u64(bk);
+    if (tid == 0) {
+        const float ls = m == -INFINITY ? NAN : logf(S);
+        if (a.entropy) a.entropy[row] = ls - Tt / S;
+        if (a.logprob) a.logprob[row] = (xt - m) - ls;
+        red[0][0] = m;
+        red[0][1] = ls;
+    }
+    if (TOP) {
         __syncthreads();
-        if (!lane) best[w] = bk;
-        __syncthreads();
-        for (int j = 0; j < 8; j++) bk = best[j] > bk ? best[j] : bk;
-        last = bk;
-        if (threadIdx.x == 0) {
-            const int i = (int)(0xFFFFFFFFu - (uint32_t)bk);
-            top_ids[(int64_t)blockIdx.x * top + k] = i;
-            if (top_lp) top_lp[(int64_t)blockIdx.x * top + k] = (to_f(x[i]) - m) - ls;
+        if (tid < a.top) {
+            const Key k = list[tid];
+            a.top_ids[row * a.top + tid] = (int)(0xFFFFFFFFu - (uint32_t)k);
+            if (a.top_lp) a.top_lp[row * a.top + tid] = (order_value((uint32_t)(k >> 32)) - red[0][0]) - red[0][1];
         }
     }
 }
 
 int logprobs_launch(cn_ctx* ctx, int type, const void* logits, int64_t stride, int rows, int vocab, const int* tokens,
                     int top, float* logprob, float* entropy, int* top_ids, float* top_lp, cudaStream_t st) {
-    if (type == CN_TYPE_F16)
-        logprobs_plain_kernel<__half><<<rows, 256, 0, st>>>(static_cast<const __half*>(logits), stride, vocab, tokens,
-                                                            top, logprob, entropy, top_ids, top_lp);
+    LpArgs a{logits, stride, vocab, top, tokens, logprob, entropy, top_ids, top_lp};
+    using Fn = void (*)(LpArgs);
+    const bool half = type == CN_TYPE_F16;
+    const Fn fn = half ? (top ? (Fn)logprobs_kernel<__half, true> : (Fn)logprobs_kernel<__half, false>)
+                       : (top ? (Fn)logprobs_kernel<float, true> : (Fn)logprobs_kernel<float, false>);
+    const size_t smem = top ? (kBuf + kMaxCluster * kMaxTop) * sizeof(Key) : 0;
+    // CTAs per row: as many as the SMs hold at once (four each), and at least a
+    // quarter of a chunk for each
+    const int64_t room = (int64_t)ctx->sms * 4;
+    int cluster = 1;
+    const char* env = getenv("LP_CS");
+    if (env) cluster = atoi(env);
     else
-        logprobs_plain_kernel<float><<<rows, 256, 0, st>>>(static_cast<const float*>(logits), stride, vocab, tokens,
-                                                           top, logprob, entropy, top_ids, top_lp);
-    CN_CUDA(cudaGetLastError());
+    while (cluster < kMaxCluster && 2 * (int64_t)cluster * rows <= room && 2 * cluster * (kChunk / 4) <= vocab) cluster *= 2;
+    CN_CHECK((int64_t)rows * cluster < (1ll << 31), CN_ERR_INVALID_ARG, "too many rows (%d)", rows);
+    const uint32_t bit = 1u << (16 + (half ? 2 : 0) + (top ? 1 : 0));
+    if (!(__atomic_load_n(&ctx->kvq4_ready, __ATOMIC_RELAXED) & bit)) {
+        CN_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        CN_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        __atomic_fetch_or(&ctx->kvq4_ready, bit, __ATOMIC_RELAXED);
+    }
+    CN_CUDA(launch_cluster_k(false, cluster, fn, dim3((unsigned)(rows * cluster)), dim3(kThreads), smem, st, a));
     return CN_OK;
 }
 
@@ -134,7 +417,7 @@ extern "C" int cn_logprobs_dev(cn_ctx* ctx, int type, const void* d_logits, int6
     CN_CHECK(type == CN_TYPE_F32 || type == CN_TYPE_F16, CN_ERR_UNSUPPORTED, "logits of type %d (F32 or F16)", type);
     CN_CHECK(rows >= 1 && vocab >= 1 && row_stride >= vocab, CN_ERR_INVALID_ARG,
              "bad shape (%d rows, vocabulary %d, stride %lld)", rows, vocab, (long long)row_stride);
-    CN_CHECK(row_stride < (1ll << 40), CN_ERR_INVALID_ARG, "row_stride too large");
+    CN_CHECK(row_stride < (1ll << 40) && vocab < (1 << 30), CN_ERR_INVALID_ARG, "row too large");
     CN_CHECK(top_n >= 0 && top_n <= kMaxTop && top_n <= vocab, CN_ERR_INVALID_ARG,
              "top_n %d outside [0, min(%d, vocabulary %d)]", top_n, kMaxTop, vocab);
     CN_CHECK(!d_logprob == !d_tokens, CN_ERR_INVALID_ARG, "tokens and their log probabilities go together");
