@@ -12,7 +12,7 @@
 // bound t below which nothing can be among its top n.  t starts from the first
 // chunk (each of the W warps finds the k-th largest of its lanes' maxima, k =
 // ceil(n / W); the smallest of the W has at least n values at or above it)
-// and is the n-th best key whenever the buffer is cut back to n; after the first
+// and is the n-th best value whenever the buffer is cut back to n; after the first
 // chunks next to nothing passes it.
 //
 // A row is split over a cluster of CTAs when there are few rows; their sums and
@@ -32,7 +32,9 @@ constexpr int kMaxTop = 64;
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kPer = 16;              // values a thread takes at a time
 constexpr int kChunk = kThreads * kPer;
-constexpr int kCut = 512;             // candidates at which the buffer is cut back
+constexpr int kCut = 128;             // candidates at which the careful way cuts the buffer back
+constexpr int kSmall = 256;           // keys that are ranked by counting
+static_assert(kCut >= kMaxTop, "a cut leaves kMaxTop");
 constexpr int kBuf = kCut + kChunk;   // (a chunk can add all its values)
 constexpr int kMaxCluster = 16;
 
@@ -56,7 +58,7 @@ __device__ __forceinline__ uint32_t order32(float v) {
 __device__ __forceinline__ float order_value(uint32_t o) {
     return o == 0u ? NAN : __uint_as_float((o & 0x80000000u) ? o & 0x7FFFFFFFu : ~o);
 }
-constexpr uint32_t kMinusInf = 0x007FFFFFu;  // order32(-inf)
+constexpr uint32_t kMinusInf = 0x007FFFFFu, kZero = 0x80000000u;  // order32 of -inf and 0
 
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
@@ -90,9 +92,9 @@ struct Vec<__half> {
     __device__ static uint32_t minus_inf() { return 0xFC00FC00u; }
 };
 
-// The running sums of one thread.
+// The running sums of one thread, relative to m; `top` is its largest value.
 struct Sums {
-    float m = -INFINITY;
+    float m = -INFINITY, top = -INFINITY;
     float2 S = {0.f, 0.f}, T = {0.f, 0.f};
     __device__ void raise(float to) {  // to > m
         if (m != -INFINITY) {
@@ -101,6 +103,10 @@ struct Sums {
             S.x *= f, S.y *= f;
         }
         m = to;
+    }
+    __device__ void see(float v) {  // m follows when outgrown by e^16 (rarely: the sums stay far inside fp32)
+        top = fmaxf(top, v);
+        if (v > m + 16.f) raise(v);
     }
     template <int N>
     __device__ void add(const float* x) {
@@ -111,7 +117,8 @@ struct Sums {
             float2 d = add2(make_float2(x[i], x[i + 1]), nm);
             // (below e^-200 nothing is left; keeps -inf * 0 out and NaN in)
             d.x = max_nan(d.x, -200.f), d.y = max_nan(d.y, -200.f);
-            const float2 e = make_float2(ex2(d.x * 1.44269504088896341f), ex2(d.y * 1.44269504088896341f));
+            const float2 l = mul2(d, make_float2(1.44269504088896341f, 1.44269504088896341f));
+            const float2 e = make_float2(ex2(l.x), ex2(l.y));
             S = add2(S, e);
             T = fma2(d, e, T);
         }
@@ -144,22 +151,64 @@ __device__ __forceinline__ Key warp_max(Key k) {
     return k;
 }
 
-// The `top` largest of buf[0..cnt), largest first, into list (0 where there are
-// fewer).  Whole CTA; buf and list must be visible (a barrier before).
-__device__ void best_keys(const Key* buf, int cnt, int top, Key* list, Key* red) {
-    const int tid = threadIdx.x;
-    if (tid < top) list[tid] = 0;
-    __syncthreads();
-    if (cnt <= kCut) {
-        // a key's place is the number of larger ones
+// Shared memory of best_keys.
+struct Pick {
+    Key list[kMaxTop];   // the result
+    Key few[kSmall];
+    Key red[2 * kWarps];
+    uint32_t bound[kWarps];
+    int count;
+};
+
+// The `top` largest of buf[0..cnt), largest first, into s.list (0 where there
+// are fewer).  Whole CTA; buf must be visible (a barrier before).  Many keys are
+// first brought down by a bound as in the first chunk, few are ranked by
+// counting the larger ones, and many equal values (the bound lets them all
+// through) go one after another.
+__device__ void best_keys(const Key* buf, int cnt, int top, Pick& s) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid < top) s.list[tid] = 0;
+    if (tid == 0) s.count = 0;
+    const Key* from = buf;
+    bool rank = cnt <= kSmall;
+    if (!rank) {
+        uint32_t w = 0, last = 0;
+        for (int i = tid; i < cnt; i += kThreads) w = max(w, (uint32_t)(buf[i] >> 32));
+        for (int r = 0; r < (top + kWarps - 1) / kWarps; r++) {  // (cnt > kThreads: every lane has a key)
+            last = __reduce_max_sync(0xffffffffu, w);
+            if (lane == __ffs(__ballot_sync(0xffffffffu, w == last)) - 1) w = 0;
+        }
+        if (lane == 0) s.bound[warp] = last;
+        __syncthreads();
+        uint32_t t = s.bound[0];
+#pragma unroll
+        for (int i = 1; i < kWarps; i++) t = min(t, s.bound[i]);
         for (int i = tid; i < cnt; i += kThreads) {
             const Key k = buf[i];
-            int r = 0;
-            for (int j = 0; j < cnt; j++) r += buf[j] > k;
-            if (r < top) list[r] = k;
+            if ((uint32_t)(k >> 32) >= t) {
+                const int at = atomicAdd(&s.count, 1);
+                if (at < kSmall) s.few[at] = k;
+            }
+        }
+        __syncthreads();
+        if (s.count <= kSmall) {
+            rank = true;
+            from = s.few;
+            cnt = s.count;
         }
     } else {
-        // one after another; a thread looks again only when its own was taken
+        __syncthreads();
+    }
+    if (rank) {
+        if (tid < cnt) {
+            const Key k = from[tid];
+            int r = 0;
+#pragma unroll 4
+            for (int j = 0; j < cnt; j++) r += from[j] > k;
+            if (r < top) s.list[r] = k;
+        }
+    } else {
+        // a thread looks again only when its own was taken
         auto mine = [&](Key below) {
             Key b = 0;
             for (int i = tid; i < cnt; i += kThreads) {
@@ -171,15 +220,15 @@ __device__ void best_keys(const Key* buf, int cnt, int top, Key* list, Key* red)
         Key own = mine(~0ull);
         for (int r = 0; r < top; r++) {
             const Key w = warp_max(own);
-            if ((tid & 31) == 0) red[(r & 1) * kWarps + (tid >> 5)] = w;
+            if (lane == 0) s.red[(r & 1) * kWarps + warp] = w;
             __syncthreads();
             Key k = 0;
 #pragma unroll
             for (int i = 0; i < kWarps; i++) {
-                const Key x = red[(r & 1) * kWarps + i];
+                const Key x = s.red[(r & 1) * kWarps + i];
                 k = x > k ? x : k;
             }
-            if (tid == 0) list[r] = k;
+            if (tid == 0) s.list[r] = k;
             if (k != 0 && own == k) own = mine(k);
         }
     }
@@ -191,13 +240,14 @@ __device__ void best_keys(const Key* buf, int cnt, int top, Key* list, Key* red)
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const LpArgs a) {
     constexpr int VN = Vec<T>::N, U = kPer / VN;
-    extern __shared__ __align__(16) uint8_t smem[];
-    Key* buf = reinterpret_cast<Key*>(smem);                // [kBuf] (TOP)
+    extern __shared__ __align__(16) uint8_t smem[];         // (TOP)
+    Key* buf = reinterpret_cast<Key*>(smem);                // [kBuf]
     Key* meet = buf + kBuf;                                 // [kMaxCluster][kMaxTop] the CTAs' lists (first CTA)
+    Pick& pick = *reinterpret_cast<Pick*>(meet + kMaxCluster * kMaxTop);
+    uint32_t* bound = pick.bound;
+    Key* list = pick.list;
     __shared__ float red[kWarps][3];
     __shared__ float sums[kMaxCluster][3];
-    __shared__ Key kred[2 * kWarps], list[kMaxTop];
-    __shared__ uint32_t bound[kWarps];
     __shared__ int s_count;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t cs = cluster_size(), rank = cluster_rank();
@@ -216,32 +266,42 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const LpArgs a) {
     const uint4* v = reinterpret_cast<const uint4*>(x0 - off);
     const int pieces = (int)(((int64_t)off + a.n + VN - 1) / VN);
     const int v0 = (int)((int64_t)pieces * rank / cs), v1 = (int)((int64_t)pieces * (rank + 1) / cs);
-    auto load = [&](int i) -> uint4 {
-        uint4 u = make_uint4(Vec<T>::minus_inf(), Vec<T>::minus_inf(), Vec<T>::minus_inf(), Vec<T>::minus_inf());
-        if (i < v1) {
-            const int64_t e = (int64_t)i * VN - off;
-            if (e >= 0 && e + VN <= a.n) {
-                u = __ldcs(v + i);
-            } else {
-                T* p = reinterpret_cast<T*>(&u);
+    // pieces within the row as a whole
+    const int in0 = max(v0, off ? 1 : 0), in1 = min(v1, (int)(((int64_t)off + a.n) / VN));
+    auto load_chunk = [&](uint4(&to)[U], int q) {
+        const int b = v0 + q * U * kThreads;
+        if (b >= in0 && b + U * kThreads <= in1) {
+            const uint4* p = v + b + tid;
 #pragma unroll
-                for (int k = 0; k < VN; k++)
-                    if (e + k >= 0 && e + k < a.n) p[k] = x0[e + k];
+            for (int k = 0; k < U; k++) to[k] = __ldcs(p + k * kThreads);
+            return;
+        }
+#pragma unroll
+        for (int k = 0; k < U; k++) {
+            const int i = b + k * kThreads + tid;
+            to[k] = make_uint4(Vec<T>::minus_inf(), Vec<T>::minus_inf(), Vec<T>::minus_inf(), Vec<T>::minus_inf());
+            if (i >= in0 && i < in1) {
+                to[k] = __ldcs(v + i);
+            } else if (i < v1) {  // the row's first or last piece
+                T* p = reinterpret_cast<T*>(&to[k]);
+#pragma unroll
+                for (int j = 0; j < VN; j++) {
+                    const int e = i * VN - off + j;
+                    if (e >= 0 && e < a.n) p[j] = x0[e];
+                }
             }
         }
-        return u;
     };
-    uint4 cur[U], nxt[U];
-#pragma unroll
-    for (int k = 0; k < U; k++) cur[k] = load(v0 + k * kThreads + tid);
     Sums sm;
-    uint32_t t_ord = 0;   // what may be among the top has order32 >= t_ord (first: > after a cut)
-    bool strict = false;
-    const int chunks = (v1 - v0 + U * kThreads - 1) / (U * kThreads);
-    for (int c = 0; c < chunks; c++) {
-        const int first = v0 + c * U * kThreads + tid;
-#pragma unroll
-        for (int k = 0; k < U; k++) nxt[k] = load(first + (U + k) * kThreads);
+    // Candidates are the values above the float t (in the order: above t_ord).
+    // They go into buf as they come; the buffer is cut back to the best after
+    // chunks 0, 4, 16, 64 and so on, which leaves it far from full unless the
+    // row rises along its length.  Then, or where no t tells NaN or -inf apart, the
+    // CTA's share is gone through again chunk by chunk.
+    uint32_t t_ord = 0;
+    float t = INFINITY;
+    bool again = false;
+    auto take = [&](const uint4(&cur)[U]) {
         float cm = -INFINITY;
 #pragma unroll
         for (int k = 0; k < U; k++) {
@@ -250,66 +310,118 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const LpArgs a) {
 #pragma unroll
             for (int i = 0; i < VN; i++) cm = fmaxf(cm, x[i]);
         }
-        if (cm > sm.m) sm.raise(cm);
+        sm.see(cm);
 #pragma unroll
         for (int k = 0; k < U; k++) {
             float x[VN];
             Vec<T>::get(cur[k], x);
             sm.template add<VN>(x);
         }
+        return cm;
+    };
+    auto keep = [&](const uint4(&cur)[U], int c) {
+#pragma unroll
+        for (int k = 0; k < U; k++) {
+            float x[VN];
+            Vec<T>::get(cur[k], x);
+            const int e = (v0 + (c * U + k) * kThreads + tid) * VN - off;
+#pragma unroll
+            for (int i = 0; i < VN; i++)
+                if (x[i] > t) {
+                    const int at = atomicAdd(&s_count, 1);
+                    if (at < kBuf) buf[at] = ((Key)order32(x[i]) << 32) | (0xFFFFFFFFu - (uint32_t)(e + i));
+                }
+        }
+    };
+    // (whole CTA, after a barrier)
+    auto cut = [&]() {
+        const int cnt = s_count;
+        if (cnt > a.top && cnt <= kBuf) {
+            best_keys(buf, cnt, a.top, pick);
+            if (tid < a.top) buf[tid] = list[tid];
+            if (tid == 0) s_count = a.top;
+            // (what comes later has higher ids: an equal value is not better)
+            t_ord = (uint32_t)(list[a.top - 1] >> 32);
+            t = order_value(t_ord);
+        }
+        __syncthreads();
+    };
+    const int chunks = (v1 - v0 + U * kThreads - 1) / (U * kThreads);
+    // (a CTA keeps 16 KB of loads in flight: one chunk of fp32, two of fp16)
+    constexpr int AHEAD = VN / 4;
+    uint4 ring[AHEAD + 1][U];
+#pragma unroll
+    for (int q = 0; q <= AHEAD; q++) load_chunk(ring[q], q);
+    {
+        const float cm = take(ring[0]);
         if constexpr (TOP) {
-            const uint32_t co = order32(cm);
-            if (c == 0) {
-                // (of the warps whose lanes all have values)
-                const int warps = min(v1 - v0, kThreads) / 32;
-                const int rounds = warps ? (a.top + warps - 1) / warps : 33;
-                if (rounds <= 32) {
-                    uint32_t w = co, last = 0;
-                    for (int r = 0; r < rounds; r++) {
-                        last = __reduce_max_sync(0xffffffffu, w);
-                        if (lane == __ffs(__ballot_sync(0xffffffffu, w == last)) - 1) w = 0;
-                    }
-                    if (lane == 0) bound[warp] = warp < warps ? last : 0xFFFFFFFFu;
-                    __syncthreads();
-                    t_ord = bound[0];
-#pragma unroll
-                    for (int i = 1; i < kWarps; i++) t_ord = min(t_ord, bound[i]);
-                } else {
-                    __syncthreads();
+            // (of the warps whose lanes all have values)
+            const int warps = min(v1 - v0, kThreads) / 32;
+            const int rounds = warps ? (a.top + warps - 1) / warps : 33;
+            if (rounds <= 32) {
+                uint32_t w = order32(cm), last = 0;
+                for (int r = 0; r < rounds; r++) {
+                    last = __reduce_max_sync(0xffffffffu, w);
+                    if (lane == __ffs(__ballot_sync(0xffffffffu, w == last)) - 1) w = 0;
                 }
-                // (a maximum of -inf may stand for NaN or nothing)
-                if (t_ord <= kMinusInf) t_ord = 0;
+                if (lane == 0) bound[warp] = warp < warps ? last : 0xFFFFFFFFu;
             }
-            // (where t is -inf or NaN, NaN and -inf count too)
-            if (strict ? co > t_ord || t_ord < kMinusInf : co >= t_ord) {
+            __syncthreads();
+            if (rounds <= 32) {
+                t_ord = bound[0];
 #pragma unroll
-                for (int k = 0; k < U; k++) {
-                    float x[VN];
-                    Vec<T>::get(cur[k], x);
-                    const int e = (first + k * kThreads) * VN - off;
-#pragma unroll
-                    for (int i = 0; i < VN; i++) {
-                        const uint32_t o = order32(x[i]);
-                        if ((strict ? o > t_ord : o >= t_ord) && e + i >= 0 && e + i < a.n && first + k * kThreads < v1)
-                            buf[atomicAdd(&s_count, 1)] = ((Key)o << 32) | (0xFFFFFFFFu - (uint32_t)(e + i));
-                    }
-                }
+                for (int i = 1; i < kWarps; i++) t_ord = min(t_ord, bound[i]);
             }
-            if (__syncthreads_or(*(volatile int*)&s_count > kCut)) {
-                const int cnt = s_count;
-                best_keys(buf, cnt, a.top, list, kred);
-                if (tid < a.top) buf[tid] = list[tid];
-                if (tid == 0) s_count = min(cnt, a.top);
-                if (cnt >= a.top) {
-                    t_ord = (uint32_t)(list[a.top - 1] >> 32);
-                    strict = true;  // (what comes later has higher ids)
+            again = t_ord <= kMinusInf;  // (a maximum of -inf may stand for NaN or nothing)
+            if (!again) {
+                t_ord -= t_ord == kZero ? 2 : 1;  // the next value below (0 and -0 are one)
+                t = order_value(t_ord);
+                if (cm > t) keep(ring[0], 0);
+                if (chunks > 1) {
+                    __syncthreads();
+                    cut();
                 }
-                __syncthreads();
             }
         }
-#pragma unroll
-        for (int k = 0; k < U; k++) cur[k] = nxt[k];
     }
+    for (int c = 1; c < chunks; c++) {
+#pragma unroll
+        for (int q = 0; q < AHEAD; q++)
+#pragma unroll
+            for (int k = 0; k < U; k++) ring[q][k] = ring[q + 1][k];
+        if (c + AHEAD < chunks) load_chunk(ring[AHEAD], c + AHEAD);
+        const float cm = take(ring[0]);
+        if constexpr (TOP) {
+            if (cm > t) keep(ring[0], c);
+            if ((c & (c - 1)) == 0 && (c & 0x55555554)) {  // 4, 16, 64, ...
+                __syncthreads();
+                cut();
+            }
+        }
+    }
+    if constexpr (TOP) {
+        __syncthreads();
+        if (again || s_count > kBuf) {
+            __syncthreads();
+            if (tid == 0) s_count = 0;
+            bool full = false;  // (as many as asked for are kept: only larger values count)
+            __syncthreads();
+            for (int c = 0; c < chunks; c++) {
+                for (int h = 0; h < kPer; h++) {
+                    const int i = v0 + (c * U + h / VN) * kThreads + tid, e = i * VN - off + h % VN;
+                    if (e < 0 || e >= a.n || i >= v1) continue;
+                    const uint32_t o = order32((float)x0[e]);
+                    if (!full || o > t_ord) buf[atomicAdd(&s_count, 1)] = ((Key)o << 32) | (0xFFFFFFFFu - (uint32_t)e);
+                }
+                if (__syncthreads_or(*(volatile int*)&s_count > kCut)) {
+                    full = true;  // (kCut is above any top)
+                    cut();
+                }
+            }
+            __syncthreads();
+        }
+    }
+    if (sm.top > sm.m) sm.raise(sm.top);
     // the CTA's sums
     float m = sm.m, S = sm.S.x + sm.S.y, Tt = sm.T.x + sm.T.y;
 #pragma unroll
@@ -322,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const LpArgs a) {
         red[warp][2] = Tt;
     }
     __syncthreads();
-    if (TOP) best_keys(buf, s_count, a.top, list, kred);
+    if (TOP) best_keys(buf, s_count, a.top, pick);
     if (warp == 0) {
         const int w = lane < kWarps ? lane : 0;
         m = lane < kWarps ? red[w][0] : -INFINITY;
@@ -360,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const LpArgs a) {
                 join(m, S, Tt, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, S, o),
                      __shfl_xor_sync(0xffffffffu, Tt, o));
         }
-        if (TOP) best_keys(meet, (int)cs * a.top, a.top, list, kred);
+        if (TOP) best_keys(meet, (int)cs * a.top, a.top, pick);
     }
     if (tid == 0) {
         const float ls = m == -INFINITY ? NAN : logf(S);
@@ -386,15 +498,14 @@ int logprobs_launch(cn_ctx* ctx, int type, const void* logits, int64_t stride, i
     const bool half = type == CN_TYPE_F16;
     const Fn fn = half ? (top ? (Fn)logprobs_kernel<__half, true> : (Fn)logprobs_kernel<__half, false>)
                        : (top ? (Fn)logprobs_kernel<float, true> : (Fn)logprobs_kernel<float, false>);
-    const size_t smem = top ? (kBuf + kMaxCluster * kMaxTop) * sizeof(Key) : 0;
-    // CTAs per row: as many as the SMs hold at once (four each), and at least a
-    // quarter of a chunk for each
-    const int64_t room = (int64_t)ctx->sms * 4;
+    const size_t smem = top ? (kBuf + kMaxCluster * kMaxTop) * sizeof(Key) + sizeof(Pick) : 0;
+    // CTAs per row: as many as give every SM two (32 rows of 32000 with 20
+    // alternatives: 13.2 us with 2, 9.8 with 8, 14 with 16), and at least a quarter
+    // of a chunk for each
+    const int64_t room = (int64_t)ctx->sms * 2;
     int cluster = 1;
-    const char* env = getenv("LP_CS");
-    if (env) cluster = atoi(env);
-    else
-    while (cluster < kMaxCluster && 2 * (int64_t)cluster * rows <= room && 2 * cluster * (kChunk / 4) <= vocab) cluster *= 2;
+    while (cluster < kMaxCluster && 2 * (int64_t)cluster * rows <= room && 2 * cluster * (kChunk / 4) <= vocab)
+        cluster *= 2;
     CN_CHECK((int64_t)rows * cluster < (1ll << 31), CN_ERR_INVALID_ARG, "too many rows (%d)", rows);
     const uint32_t bit = 1u << (16 + (half ? 2 : 0) + (top ? 1 : 0));
     if (!(__atomic_load_n(&ctx->kvq4_ready, __ATOMIC_RELAXED) & bit)) {
