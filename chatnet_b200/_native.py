@@ -143,6 +143,8 @@ SIGNATURES: dict[str, tuple] = {
     "cn_kvq4_append_dev": (_i, [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _i, _i, _vp, _i, _vp]),
     "cn_kvq4_attend_dev": (_i, [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i, _i, _i, _f, _vp, _i, _vp]),
     "cn_kvq4_read_dev": (_i, [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _i, _i, _vp]),
+    "cn_llama_logprobs": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp]),
+    "cn_llama_score": (_i, [_vp, _vp, _i, _i, _vp, _vp]),
     "cn_logprobs_dev": (_i, [_vp, _i, _vp, _i64, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp]),
 }
 
@@ -150,6 +152,7 @@ TP_HANDLE_BYTES = 64
 
 KV_F32 = 0
 KV_F16 = 1
+KV_Q4 = 2
 
 
 class LlamaConfigC(C.Structure):

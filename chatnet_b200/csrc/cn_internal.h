@@ -116,6 +116,12 @@ int ensure(void** p, size_t* have, size_t need, bool zero);
 int sample_launch(cn_ctx* ctx, const float* d_logits, int vocab, int batch, float temperature, int top_k,
                   float top_p, const float* r_host, int* tokens_host);
 
+// cn_logprobs_dev's work (logprobs.cu), and its check of what goes together.
+int logprobs_launch(cn_ctx* ctx, int type, const void* logits, int64_t stride, int rows, int vocab, const int* tokens,
+                    int top, float* logprob, float* entropy, int* top_ids, float* top_lp, cudaStream_t st);
+int logprobs_check(int vocab, const void* tokens, int top, const void* logprob, const void* entropy,
+                   const void* top_ids, const void* top_lp);
+
 // Encodes the TMA descriptor a GEMV uses for a [rows][row_bytes] weight
 // matrix, or returns CN_ERR_UNSUPPORTED if the layout cannot be tiled
 // (row_bytes not a multiple of 16, or unaligned base).
@@ -161,6 +167,8 @@ int prefill_norm(cudaStream_t st, const float* x, const float* w, __half* y, flo
                  float eps, __half* ylo = nullptr);
 int prefill_silu(cudaStream_t st, const float* g, const float* u, __half* h, float* inv, int n, int M,
                  __half* hlo = nullptr, int gelu = 0);
+// n fp32 values (n % 4 == 0) as fp16 and, with lo, their fp16 rounding residuals.
+int prefill_halves(cudaStream_t st, const float* x, __half* hi, __half* lo, int64_t n);
 // RoPE of the M prompt tokens' q (in place) and k, k/v into the cache and
 // their fp16 copies into kh/vh [M][kvdim] (with kl/vl, also k's and v's fp16
 // residuals).

@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(kRowThreads)
     const int g = threadIdx.x & 7;
     const int64_t r = (int64_t)blockIdx.x * (kRowThreads / 8) + (threadIdx.x >> 3);
     const bool is_v = blockIdx.y != 0;
-    bool live = r < n_rows;
+    bool live = r < n_rows && (is_v ? v : k) != nullptr;
     int64_t tok = 0, dst = 0;
     int h = 0, p = 0;
     if (live) {

@@ -20,6 +20,7 @@
 
 #include "cn_common.cuh"
 #include "cn_internal.h"
+#include "kvq4.cuh"
 #include "ops.h"
 #include "synth.cuh"
 
@@ -50,6 +51,10 @@ struct cn_llama {
     int kvdim = 0;
     size_t kv_elem = 4;
     int64_t seq_stride = 0;  // KV elements per sequence slot
+    // 4-bit cache (CN_KV_Q4): kc / vc hold the rows' quants and, from q4_scales
+    // on, their scales; rows lie [sequence][layer][kv head][q4_ctx]
+    int q4_ctx = 0;
+    size_t q4_scales = 0;
     void* kc = nullptr;
     void* vc = nullptr;
     float2* rope = nullptr;
@@ -88,6 +93,9 @@ struct cn_llama {
           *pf_u = nullptr;
     __half *pf_h = nullptr, *pf_kh = nullptr, *pf_vh = nullptr;
     int* pf_tok = nullptr;
+    float* pf_att = nullptr;      // fp32 attention output (4-bit cache)
+    int* q4_pos = nullptr;        // position of a call that works on one sequence (4-bit cache)
+    float* score_logits = nullptr;  // [kMaxBatch][vocab], cn_llama_score
     float* pf_xs = nullptr;  // [pf_cap] inverse row scales of pf_h
     // row-padded copies of projections whose rows are not 16-byte multiples
     // (pad_rows); they replace the caller's tensors in t
@@ -105,6 +113,39 @@ static const float* norm_w(const cn_llama* m, int l, int which) {
     if (m->normw) return m->normw + (l < 0 ? (size_t)2 * m->cfg.n_layers * dim : ((size_t)2 * l + which) * dim);
     return static_cast<const float*>(l < 0 ? m->t[2]->d : LT(m, l, which ? 5 : 0)->d);
 }
+
+__global__ void set_int_kernel(int* p, int v) { *p = v; }
+
+// The position a call on one sequence's 4-bit cache works at.
+static int set_q4_pos(cn_llama* m, int pos) {
+    set_int_kernel<<<1, 1, 0, m->ctx->stream>>>(m->q4_pos, pos);
+    CN_CUDA(cudaGetLastError());
+    return CN_OK;
+}
+
+static bool kv_q4(const cn_llama* m) { return m->cfg.kv_dtype == CN_KV_Q4; }
+
+// Layer l's 4-bit cache, from sequence slot seq on.
+static cn_kvq4 q4_layer(const cn_llama* m, int l, int seq = 0) {
+    const int hd = m->cfg.head_dim;
+    const int64_t per_seq = (int64_t)m->cfg.n_layers * m->nkv * m->q4_ctx;
+    const int64_t row = seq * per_seq + (int64_t)l * m->nkv * m->q4_ctx;
+    auto at = [&](void* base, size_t off, int bytes) { return static_cast<uint8_t*>(base) + off + row * bytes; };
+    cn_kvq4 c;
+    c.k_quants = at(m->kc, 0, hd / 2);
+    c.k_scales = at(m->kc, m->q4_scales, hd / 16);
+    c.v_quants = at(m->vc, 0, hd / 2);
+    c.v_scales = at(m->vc, m->q4_scales, hd / 16);
+    c.n_seqs = m->cfg.max_batch - seq;
+    c.n_kv_heads = m->nkv;
+    c.head_dim = hd;
+    c.ctx_len = m->q4_ctx;
+    c.seq_rows = per_seq;
+    return c;
+}
+
+// The reference scales scores by 1 / sqrt(head_dim) (LlamaModel.cs:262).
+static float q4_score_scale(const cn_llama* m) { return 1.0f / sqrtf((float)m->cfg.head_dim); }
 
 static int check_shape(const cn_tensor* t, const char* name, int64_t rows, int64_t cols,
                        bool f32_vector) {
@@ -158,10 +199,11 @@ static int build_step(cn_llama* m, int B) {
         if (gemv_group_make(m->ctx, o + 4, 2, &st.gu[l]) != CN_OK) st.gu[l].n = 0;
     }
     set_error(CN_OK, "");
-    int rc = attention_plan(m->nh, m->nkv, c.head_dim, c.ctx_len, B, m->ctx->sms,
-                            c.kv_dtype == CN_KV_F16, &st.ap);
-    if (rc) return rc;
-    if ((rc = attention_prepare(st.ap))) return rc;
+    if (!kv_q4(m)) {
+        int rc = attention_plan(m->nh, m->nkv, c.head_dim, c.ctx_len, B, m->ctx->sms, c.kv_dtype == CN_KV_F16, &st.ap);
+        if (rc) return rc;
+        if ((rc = attention_prepare(st.ap))) return rc;
+    }
     st.built = true;
     return CN_OK;
 }
@@ -279,38 +321,49 @@ static int enqueue_step(cn_llama* m, int B, cudaStream_t s) {
             if ((rc = gemv(m, s, ops[2], m->xn, m->v, pc))) return rc;
         }
         if ((rc = mark(s, P_QKV))) return rc;
-        AttnArgs aa;
-        aa.q = m->q;
-        aa.kcache = m->kc;
-        aa.vcache = m->vc;
-        aa.pos_dev = m->pos;
-        aa.pos_host = 0;
-        aa.batch = B;
-        aa.n_heads = m->nh;
-        aa.n_kv = m->nkv;
-        aa.hd = c.head_dim;
-        aa.q_stride = qdim;
-        aa.cache_seq_stride = m->seq_stride;
-        aa.cache_layer_off = (int64_t)l * c.ctx_len * kvd;
-        aa.kv_f16 = c.kv_dtype == CN_KV_F16;
-        aa.ctx_len = c.ctx_len;
-        aa.part = m->part;
-        aa.counters = m->attn_ctr;
-        aa.out = m->att;
-        aa.out_stride = qdim;
-        aa.prep = prep_target(&ops[3], m->gb);
-        // TensorMath.ApplyRoPE of q and the new k row, and the new k/v rows'
-        // cache store, run inside the attention kernel
-        aa.rope.k = m->k;
-        aa.rope.v = m->v;
-        aa.rope.rope = m->rope;
-        aa.rope.kv_stride = kvd;
-        aa.rope.on = 1;
-        aa.rope.neox = c.rope_neox;
-        if ((m->nh / m->nkv) * c.head_dim % 256 != 0) aa.prep.kind = -1;
-        if ((rc = launch_attention(aa, st.ap, s)) || (rc = mark(s, P_ATTN))) return rc;
         pc = PrepCache();
-        if (aa.prep.kind >= 0) pc.set(m->att, ops[3]);
+        if (kv_q4(m)) {
+            const cn_kvq4 q4 = q4_layer(m, l);
+            if ((rc = kvq4_append(q4, m->k, m->v, kvd, m->pos, nullptr, B, 1, m->rope, c.rope_neox, s)) ||
+                (rc = mark(s, P_ROPE)))
+                return rc;
+            if ((rc = kvq4_attend(m->ctx, q4, m->q, qdim, m->att, qdim, m->pos, nullptr, B, 1, m->nh,
+                                  q4_score_scale(m), m->rope, c.rope_neox, s)) ||
+                (rc = mark(s, P_ATTN)))
+                return rc;
+        } else {
+            AttnArgs aa;
+            aa.q = m->q;
+            aa.kcache = m->kc;
+            aa.vcache = m->vc;
+            aa.pos_dev = m->pos;
+            aa.pos_host = 0;
+            aa.batch = B;
+            aa.n_heads = m->nh;
+            aa.n_kv = m->nkv;
+            aa.hd = c.head_dim;
+            aa.q_stride = qdim;
+            aa.cache_seq_stride = m->seq_stride;
+            aa.cache_layer_off = (int64_t)l * c.ctx_len * kvd;
+            aa.kv_f16 = c.kv_dtype == CN_KV_F16;
+            aa.ctx_len = c.ctx_len;
+            aa.part = m->part;
+            aa.counters = m->attn_ctr;
+            aa.out = m->att;
+            aa.out_stride = qdim;
+            aa.prep = prep_target(&ops[3], m->gb);
+            // TensorMath.ApplyRoPE of q and the new k row, and the new k/v rows'
+            // cache store, run inside the attention kernel
+            aa.rope.k = m->k;
+            aa.rope.v = m->v;
+            aa.rope.rope = m->rope;
+            aa.rope.kv_stride = kvd;
+            aa.rope.on = 1;
+            aa.rope.neox = c.rope_neox;
+            if ((m->nh / m->nkv) * c.head_dim % 256 != 0) aa.prep.kind = -1;
+            if ((rc = launch_attention(aa, st.ap, s)) || (rc = mark(s, P_ATTN))) return rc;
+            if (aa.prep.kind >= 0) pc.set(m->att, ops[3]);
+        }
         if (tp) {
             const XchgOut xo = tp_reduce_out(m->tp, uses, 2u * l, 0);
             if ((rc = gemv(m, s, ops[3], m->att, m->tmp, pc, &xo))) return rc;
@@ -408,14 +461,16 @@ static int check_dev_err_reset(cn_llama* m) {
 // Fills the cache's first npos positions with the generator's values of the
 // WHOLE model's cache ([layers*ctx, kvd_full]): a tensor-parallel rank holds
 // columns [col0, col0 + kvd) of it.
+// (with layer0, layers of the whole cache from that one on, packed to npos positions)
 __global__ void kv_synth_kernel(uint64_t seed, int layers, int npos, int ctx, int kvd, int kvd_full, int col0,
-                                int f16, void* out) {
+                                int f16, void* out, int layer0 = -1) {
     const int64_t n = (int64_t)layers * npos * kvd;
     for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n;
          i += (int64_t)gridDim.x * blockDim.x) {
         int64_t l = i / ((int64_t)npos * kvd);
         int64_t r = i % ((int64_t)npos * kvd);
-        int64_t idx = (l * ctx + r / kvd) * kvd + r % kvd;
+        int64_t idx = layer0 >= 0 ? i : (l * ctx + r / kvd) * kvd + r % kvd;
+        if (layer0 >= 0) l += layer0;
         int64_t g = (l * ctx + r / kvd) * kvd_full + col0 + r % kvd;
         float v = synth::normal_elem(seed, (uint64_t)g);
         if (f16) reinterpret_cast<__half*>(out)[idx] = __float2half_rn(v);
@@ -478,7 +533,8 @@ static void free_model(cn_llama* m) {
                     m->gate, m->up, m->logits, m->part, m->tokens, m->pos, m->amax,
                     m->gb.xfrag, m->gb.xsum, m->gb.partials, m->gb.counters, m->gb.xinv,
                     m->pf_x, m->pf_q, m->pf_k, m->pf_v, m->pf_g, m->pf_u, m->pf_h, m->pf_kh, m->pf_vh,
-                    m->pf_tok, m->pf_xs, m->pf_hl, m->pf_kl, m->pf_vl, m->normw};
+                    m->pf_tok, m->pf_xs, m->pf_hl, m->pf_kl, m->pf_vl, m->normw, m->pf_att, m->q4_pos,
+                    m->score_logits};
     for (void* p : bufs) cudaFree(p);
     for (cn_tensor* p : m->pads) {
         cudaFree(p->d);
@@ -579,12 +635,12 @@ static int prefill_reserve(cn_llama* m, int n) {
     if (n <= m->pf_cap) return CN_OK;
     CN_CUDA(cudaStreamSynchronize(m->ctx->stream));
     void* old[] = {m->pf_x, m->pf_q, m->pf_k, m->pf_v, m->pf_g, m->pf_u, m->pf_h, m->pf_kh, m->pf_vh,
-                   m->pf_tok, m->pf_xs, m->pf_hl, m->pf_kl, m->pf_vl};
+                   m->pf_tok, m->pf_xs, m->pf_hl, m->pf_kl, m->pf_vl, m->pf_att};
     for (void* p : old) cudaFree(p);
     m->pf_x = m->pf_q = m->pf_k = m->pf_v = m->pf_g = m->pf_u = nullptr;
     m->pf_h = m->pf_kh = m->pf_vh = m->pf_hl = m->pf_kl = m->pf_vl = nullptr;
     m->pf_tok = nullptr;
-    m->pf_xs = nullptr;
+    m->pf_xs = m->pf_att = nullptr;
     m->pf_cap = 0;
     const cn_llama_config& c = m->cfg;
     const size_t N = (size_t)n;
@@ -603,7 +659,8 @@ static int prefill_reserve(cn_llama* m, int n) {
         (rc = dmalloc((void**)&m->pf_xs, N * 4, false)) ||
         (rc = dmalloc((void**)&m->pf_hl, N * hmax * 2, false)) ||
         (rc = dmalloc((void**)&m->pf_kl, N * m->kvdim * 2, false)) ||
-        (rc = dmalloc((void**)&m->pf_vl, N * m->kvdim * 2, false)))
+        (rc = dmalloc((void**)&m->pf_vl, N * m->kvdim * 2, false)) ||
+        (kv_q4(m) && (rc = dmalloc((void**)&m->pf_att, N * m->qdim * 4, false))))
         return rc;
     m->pf_cap = n;
     return CN_OK;
@@ -628,6 +685,7 @@ static int prefill_layers(cn_llama* m, int n, int pos) {
     __half* vl = attn_split && !kv16 ? m->pf_vl : nullptr;
     int rc;
     if ((attn_split || ffn_split) && (rc = prefill_scales(m))) return rc;
+    if (kv_q4(m) && (rc = set_q4_pos(m, pos))) return rc;
     for (int l = 0; l < c.n_layers; l++) {
         const int64_t cache_off = (int64_t)l * c.ctx_len * kvd;  // sequence slot 0
         if ((rc = prefill_norm(s, m->pf_x, norm_w(m, l, 0), m->pf_h, m->pf_xs, c.dim, n,
@@ -638,13 +696,22 @@ static int prefill_layers(cn_llama* m, int n, int pos) {
             float* y[3] = {m->pf_q, m->pf_k, m->pf_v};
             if ((rc = mm_group(m, l, 3, kSlotsQKV, rows, c.dim, n, y, rows, false, true, false, ns[0]))) return rc;
         }
-        if ((rc = prefill_rope(s, m->pf_q, m->pf_k, m->pf_v, m->rope, pos, n, qd, kvd, c.head_dim, m->kc, m->vc,
-                               cache_off, kv16, m->pf_kh, m->pf_vh, kl, vl, c.rope_neox)))
-            return rc;
-        if ((rc = prefill_attention(s, m->pf_q, qd, m->kc, m->vc, kv16, cache_off, m->nh, m->nkv, c.head_dim, n,
-                                    pos, m->pf_kh, m->pf_vh, m->pf_h, qd, attn_split, kl, vl,
-                                    attn_split ? m->pf_hl : nullptr)))
-            return rc;
+        if (kv_q4(m)) {
+            const cn_kvq4 q4 = q4_layer(m, l);
+            if ((rc = kvq4_append(q4, m->pf_k, m->pf_v, kvd, m->q4_pos, nullptr, 1, n, m->rope, c.rope_neox, s)) ||
+                (rc = kvq4_attend(m->ctx, q4, m->pf_q, qd, m->pf_att, qd, m->q4_pos, nullptr, 1, n, m->nh,
+                                  q4_score_scale(m), m->rope, c.rope_neox, s)) ||
+                (rc = prefill_halves(s, m->pf_att, m->pf_h, attn_split ? m->pf_hl : nullptr, (int64_t)n * qd)))
+                return rc;
+        } else {
+            if ((rc = prefill_rope(s, m->pf_q, m->pf_k, m->pf_v, m->rope, pos, n, qd, kvd, c.head_dim, m->kc, m->vc,
+                                   cache_off, kv16, m->pf_kh, m->pf_vh, kl, vl, c.rope_neox)))
+                return rc;
+            if ((rc = prefill_attention(s, m->pf_q, qd, m->kc, m->vc, kv16, cache_off, m->nh, m->nkv, c.head_dim, n,
+                                        pos, m->pf_kh, m->pf_vh, m->pf_h, qd, attn_split, kl, vl,
+                                        attn_split ? m->pf_hl : nullptr)))
+                return rc;
+        }
         {
             const int64_t rows = c.dim;
             if ((rc = mm_group(m, l, 1, kSlotsO, &rows, qd, n, &m->pf_x, &rows, true, false, false, ns[1]))) return rc;
@@ -669,7 +736,8 @@ static int prefill_layers(cn_llama* m, int n, int pos) {
     return CN_OK;
 }
 
-// Kernels one prefill_layers call launches: 6 per layer besides the matmuls,
+// Kernels one prefill_layers call launches: 6 per layer besides the matmuls (7
+// with a 4-bit cache),
 // and one matmul per same-type run of each projection group (4 per layer
 // when every group's types agree).
 static int prefill_kernels(const cn_llama* m) {
@@ -679,7 +747,7 @@ static int prefill_kernels(const cn_llama* m) {
     int k = 0, ns[4];
     split_counts(m, ns);
     for (int l = 0; l < m->cfg.n_layers; l++)
-        k += 6 + mm_group(mm, l, 3, kSlotsQKV, r, 0, 0, y, r, false, false, true, ns[0]) +
+        k += (kv_q4(m) ? 7 : 6) + mm_group(mm, l, 3, kSlotsQKV, r, 0, 0, y, r, false, false, true, ns[0]) +
              mm_group(mm, l, 1, kSlotsO, r, 0, 0, y, r, false, false, true, ns[1]) +
              mm_group(mm, l, 2, kSlotsGU, r, 0, 0, y, r, false, false, true, ns[2]) +
              mm_group(mm, l, 1, kSlotsDown, r, 0, 0, y, r, false, false, true, ns[3]);
@@ -706,8 +774,10 @@ static int create_model(cn_ctx* ctx, const cn_llama_config* cfg, cn_tensor* cons
     CN_CHECK(c.n_heads % c.n_kv_heads == 0, CN_ERR_INVALID_ARG, "n_heads %% n_kv_heads != 0");
     CN_CHECK(c.max_batch >= 1 && c.max_batch <= kMaxBatch, CN_ERR_INVALID_ARG,
              "max_batch %d outside [1, %d]", c.max_batch, kMaxBatch);
-    CN_CHECK(c.kv_dtype == CN_KV_F32 || c.kv_dtype == CN_KV_F16, CN_ERR_INVALID_ARG,
+    CN_CHECK(c.kv_dtype == CN_KV_F32 || c.kv_dtype == CN_KV_F16 || c.kv_dtype == CN_KV_Q4, CN_ERR_INVALID_ARG,
              "bad kv_dtype %d", c.kv_dtype);
+    CN_CHECK(c.kv_dtype != CN_KV_Q4 || kvq4_head_dim_ok(c.head_dim), CN_ERR_UNSUPPORTED,
+             "4-bit cache: head_dim %d (32, 64, 96, 128 or 256)", c.head_dim);
     CN_CHECK((c.rope_neox == 0 || c.rope_neox == 1) && (c.act_gelu == 0 || c.act_gelu == 1) &&
                  (c.norm_offset == 0 || c.norm_offset == 1),
              CN_ERR_INVALID_ARG, "rope_neox, act_gelu and norm_offset are 0 or 1");
@@ -744,7 +814,7 @@ static int create_model(cn_ctx* ctx, const cn_llama_config* cfg, cn_tensor* cons
     }
     for (int i = 0; i < n_tensors; i++)
         CN_CHECK(tensors[i]->ctx == ctx, CN_ERR_INVALID_ARG, "tensor %d belongs to another context", i);
-    {
+    if (c.kv_dtype != CN_KV_Q4) {
         AttnPlan ap;
         if ((rc = attention_plan(nh, nkv, c.head_dim, c.ctx_len, c.max_batch, ctx->sms,
                                  c.kv_dtype == CN_KV_F16, &ap)))
@@ -769,12 +839,19 @@ static int create_model(cn_ctx* ctx, const cn_llama_config* cfg, cn_tensor* cons
     m->seq_stride = (int64_t)c.n_layers * c.ctx_len * kvd;
     m->use_graph = getenv("CN_NO_GRAPH") == nullptr;
     const int B = c.max_batch;
-    const size_t kvbytes = (size_t)B * m->seq_stride * m->kv_elem;
+    size_t kvbytes = (size_t)B * m->seq_stride * m->kv_elem;
+    if (c.kv_dtype == CN_KV_Q4) {
+        m->q4_ctx = (c.ctx_len + 7) / 8 * 8;
+        const size_t rows = (size_t)B * c.n_layers * nkv * m->q4_ctx;
+        m->q4_scales = (rows * (c.head_dim / 2) + 255) / 256 * 256;
+        kvbytes = m->q4_scales + rows * (c.head_dim / 16);
+    }
     auto fail = [&](int code) {
         free_model(m);
         return code;
     };
     if ((rc = dmalloc(&m->kc, kvbytes)) || (rc = dmalloc(&m->vc, kvbytes))) return fail(rc);
+    if (c.kv_dtype == CN_KV_Q4 && (rc = dmalloc((void**)&m->q4_pos, sizeof(int)))) return fail(rc);
     // RoPE table, computed with the reference's formula and the host libm
     // (TensorMath.ApplyRoPE, TensorMath.cs:418-432).
     {
@@ -825,7 +902,7 @@ static int create_model(cn_ctx* ctx, const cn_llama_config* cfg, cn_tensor* cons
         (rc = dmalloc((void**)&m->tokens, B * 4)) || (rc = dmalloc((void**)&m->pos, B * 4)) ||
         (rc = dmalloc((void**)&m->amax, B * 4)))
         return fail(rc);
-    {
+    if (c.kv_dtype != CN_KV_Q4) {
         // split counts depend on the batch size: size for the largest need
         size_t part = 0;
         for (int b = 1; b <= B; b++) {
@@ -989,6 +1066,90 @@ int cn_llama_sample(cn_llama* m, int batch, float temperature, int top_k, float 
              m->cfg.max_batch);
     cudaSetDevice(m->ctx->device);
     return sample_launch(m->ctx, m->logits, m->cfg.vocab, batch, temperature, top_k, top_p, r_host, tokens_host);
+}
+
+// Log probabilities on device logits with host tokens and results; rows' inputs
+// and outputs pass through ctx's sampler scratch.
+static int logprobs_host(cn_ctx* ctx, const float* d_logits, int vocab, int rows, const int* tokens, int top,
+                         float* logprob, float* entropy, int* top_ids, float* top_lp) {
+    const size_t R = (size_t)rows;
+    int rc = ensure(&ctx->samp, &ctx->samp_bytes, R * (12 + 8 * (size_t)top) + 64, false);
+    if (rc) return rc;
+    int* d_tok = static_cast<int*>(ctx->samp);
+    float* d_lp = reinterpret_cast<float*>(d_tok + R);
+    float* d_ent = d_lp + R;
+    int* d_ids = reinterpret_cast<int*>(d_ent + R);
+    float* d_tlp = reinterpret_cast<float*>(d_ids + R * top);
+    cudaStream_t s = ctx->stream;
+    if (tokens) CN_CUDA(cudaMemcpyAsync(d_tok, tokens, R * 4, cudaMemcpyHostToDevice, s));
+    rc = logprobs_launch(ctx, CN_TYPE_F32, d_logits, vocab, rows, vocab, tokens ? d_tok : nullptr, top,
+                         tokens ? d_lp : nullptr, d_ent, top ? d_ids : nullptr, top ? d_tlp : nullptr, s);
+    if (rc) return rc;
+    if (tokens) CN_CUDA(cudaMemcpyAsync(logprob, d_lp, R * 4, cudaMemcpyDeviceToHost, s));
+    if (entropy) CN_CUDA(cudaMemcpyAsync(entropy, d_ent, R * 4, cudaMemcpyDeviceToHost, s));
+    if (top) CN_CUDA(cudaMemcpyAsync(top_ids, d_ids, R * top * 4, cudaMemcpyDeviceToHost, s));
+    if (top && top_lp) CN_CUDA(cudaMemcpyAsync(top_lp, d_tlp, R * top * 4, cudaMemcpyDeviceToHost, s));
+    CN_CUDA(cudaStreamSynchronize(s));
+    return CN_OK;
+}
+
+int cn_llama_logprobs(cn_llama* m, int batch, const int* tokens, int top_n, float* logprob_host, float* entropy_host,
+                      int* top_ids_host, float* top_logprobs_host) {
+    CN_CHECK(m, CN_ERR_INVALID_ARG, "null model");
+    CN_CHECK(batch >= 1 && batch <= m->cfg.max_batch, CN_ERR_INVALID_ARG, "batch %d outside [1, %d]", batch,
+             m->cfg.max_batch);
+    int rc = logprobs_check(m->cfg.vocab, tokens, top_n, logprob_host, entropy_host, top_ids_host, top_logprobs_host);
+    if (rc) return rc;
+    cudaSetDevice(m->ctx->device);
+    return logprobs_host(m->ctx, m->logits, m->cfg.vocab, batch, tokens, top_n, logprob_host, entropy_host,
+                         top_ids_host, top_logprobs_host);
+}
+
+int cn_llama_score(cn_llama* m, const int* tokens, int n, int pos, float* logprob_host, float* entropy_host) {
+    CN_CHECK(m && tokens && logprob_host, CN_ERR_INVALID_ARG, "null argument");
+    CN_CHECK(n >= 2, CN_ERR_INVALID_ARG, "a text of %d tokens has none to score", n);
+    const cn_llama_config& c = m->cfg;
+    CN_CHECK(pos >= 0 && n - 1 <= c.ctx_len - pos, CN_ERR_INVALID_ARG, "positions [%d, %d + %d) outside the context of %d",
+             pos, pos, n - 1, c.ctx_len);
+    for (int t = 0; t < n; t++)
+        CN_CHECK(tokens[t] >= 0 && tokens[t] < c.vocab, CN_ERR_INVALID_ARG, "token id %d outside [0, %d)", tokens[t],
+                 c.vocab);
+    cudaSetDevice(m->ctx->device);
+    cudaStream_t s = m->ctx->stream;
+    int rc;
+    if (!(m->prefill_min > 0 && n - 1 >= m->prefill_min && prefill_supported(m))) {
+        // one decode step per token, its logits scored where they are
+        for (int t = 0; t + 1 < n; t++) {
+            const int p = pos + t;
+            if ((rc = cn_llama_decode(m, tokens + t, &p, 1, nullptr, nullptr)) ||
+                (rc = logprobs_host(m->ctx, m->logits, c.vocab, 1, tokens + t + 1, 0, logprob_host + t,
+                                    entropy_host ? entropy_host + t : nullptr, nullptr, nullptr)))
+                return rc;
+        }
+        return CN_OK;
+    }
+    const int N = n - 1;
+    if ((rc = prefill_reserve(m, N))) return rc;
+    if (!m->score_logits && (rc = dmalloc((void**)&m->score_logits, (size_t)kMaxBatch * c.vocab * 4, false))) return rc;
+    CN_CUDA(cudaMemcpyAsync(m->pf_tok, tokens, (size_t)N * 4, cudaMemcpyHostToDevice, s));
+    const cn_tensor* emb = m->t[T_EMB];
+    if ((rc = launch_embed(emb->type, emb->d, emb->row_bytes, m->pf_tok, c.vocab, c.dim, N, m->pf_x, m->ctx->dev_err,
+                           s)) ||
+        (rc = prefill_layers(m, N, pos)) ||
+        (rc = launch_rmsnorm(m->pf_x, norm_w(m, -1, 0), m->pf_q, c.dim, N, c.rms_eps, s)))
+        return rc;
+    // (one GPU: pf_q rows have dim values)  the head in the decode GEMV's batches,
+    // each scored before the next
+    const cn_tensor* w = m->t[T_OUT];
+    for (int t = 0; t < N; t += kMaxBatch) {
+        const int b = N - t < kMaxBatch ? N - t : kMaxBatch;
+        if ((rc = gemv_launch(m->ctx, w->type, w->d, w->rows, w->cols, w->has_map ? &w->map : nullptr,
+                              m->pf_q + (size_t)t * c.dim, m->score_logits, b)) ||
+            (rc = logprobs_host(m->ctx, m->score_logits, c.vocab, b, tokens + t + 1, 0, logprob_host + t,
+                                entropy_host ? entropy_host + t : nullptr, nullptr, nullptr)))
+            return rc;
+    }
+    return check_dev_err_reset(m);
 }
 
 int cn_llama_set_inputs(cn_llama* m, const int* tokens, const int* pos, int batch) {
@@ -1251,11 +1412,40 @@ static int kv_check(cn_llama* m, int seq, int layer, int pos0, int npos) {
     return CN_OK;
 }
 
+// Rows of a 4-bit cache as fp32 values from (k_in, v_in) or to (k_out, v_out)
+// host memory; any may be null.
+static int q4_rows(cn_llama* m, int seq, int layer, int pos0, int npos, const void* k_in, const void* v_in,
+                   void* k_out, void* v_out) {
+    if (npos == 0 || !(k_in || v_in || k_out || v_out)) return CN_OK;
+    cudaStream_t s = m->ctx->stream;
+    const size_t bytes = (size_t)npos * m->kvdim * 4;
+    int rc = ensure(&m->ctx->dstage, &m->ctx->dstage_bytes, 2 * bytes, false);
+    if (rc) return rc;
+    float* dk = static_cast<float*>(m->ctx->dstage);
+    float* dv = dk + (size_t)npos * m->kvdim;
+    const cn_kvq4 q4 = q4_layer(m, layer, seq);
+    if ((rc = set_q4_pos(m, pos0))) return rc;
+    if (k_in || v_in) {
+        if (k_in) CN_CUDA(cudaMemcpyAsync(dk, k_in, bytes, cudaMemcpyHostToDevice, s));
+        if (v_in) CN_CUDA(cudaMemcpyAsync(dv, v_in, bytes, cudaMemcpyHostToDevice, s));
+        rc = kvq4_append(q4, k_in ? dk : nullptr, v_in ? dv : nullptr, m->kvdim, m->q4_pos, nullptr, 1, npos, nullptr,
+                         0, s);
+    } else {
+        rc = kvq4_read(q4, k_out ? dk : nullptr, v_out ? dv : nullptr, m->kvdim, m->q4_pos, nullptr, 1, npos, s);
+        if (!rc && k_out) CN_CUDA(cudaMemcpyAsync(k_out, dk, bytes, cudaMemcpyDeviceToHost, s));
+        if (!rc && v_out) CN_CUDA(cudaMemcpyAsync(v_out, dv, bytes, cudaMemcpyDeviceToHost, s));
+    }
+    if (rc) return rc;
+    CN_CUDA(cudaStreamSynchronize(s));
+    return CN_OK;
+}
+
 int cn_llama_kv_write(cn_llama* m, int seq, int layer, int pos0, int npos, const void* k_host,
                       const void* v_host) {
     int rc = kv_check(m, seq, layer, pos0, npos);
     if (rc) return rc;
     cudaSetDevice(m->ctx->device);
+    if (kv_q4(m)) return q4_rows(m, seq, layer, pos0, npos, k_host, v_host, nullptr, nullptr);
     size_t off = ((size_t)seq * m->seq_stride + ((size_t)layer * m->cfg.ctx_len + pos0) * m->kvdim) *
                  m->kv_elem;
     size_t bytes = (size_t)npos * m->kvdim * m->kv_elem;
@@ -1270,6 +1460,7 @@ int cn_llama_kv_read(cn_llama* m, int seq, int layer, int pos0, int npos, void* 
     int rc = kv_check(m, seq, layer, pos0, npos);
     if (rc) return rc;
     cudaSetDevice(m->ctx->device);
+    if (kv_q4(m)) return q4_rows(m, seq, layer, pos0, npos, nullptr, nullptr, k_host, v_host);
     size_t off = ((size_t)seq * m->seq_stride + ((size_t)layer * m->cfg.ctx_len + pos0) * m->kvdim) *
                  m->kv_elem;
     size_t bytes = (size_t)npos * m->kvdim * m->kv_elem;
@@ -1284,6 +1475,33 @@ int cn_llama_kv_synth(cn_llama* m, int seq, int npos, uint64_t seed_k, uint64_t 
     if (rc) return rc;
     cudaSetDevice(m->ctx->device);
     cudaStream_t s = m->ctx->stream;
+    if (kv_q4(m)) {
+        // the rows past npos become zeros (scale 0), the others the rounded values
+        const int hd = m->cfg.head_dim, L = m->cfg.n_layers;
+        const cn_kvq4 first = q4_layer(m, 0, seq);
+        for (void* p : {first.k_quants, first.v_quants}) CN_CUDA(cudaMemsetAsync(p, 0x88, first.seq_rows * (hd / 2), s));
+        for (void* p : {first.k_scales, first.v_scales}) CN_CUDA(cudaMemsetAsync(p, 0, first.seq_rows * (hd / 16), s));
+        if (npos > 0) {
+            const int64_t n = (int64_t)npos * m->kvdim;
+            if ((rc = ensure(&m->ctx->dstage, &m->ctx->dstage_bytes, (size_t)n * 8, false))) return rc;
+            float* dk = static_cast<float*>(m->ctx->dstage);
+            const int blocks = (int)((n + 255) / 256 > 148 * 64 ? 148 * 64 : (n + 255) / 256);
+            const int kvd_full = m->cfg.n_kv_heads * hd, col0 = m->tp_rank * m->kvdim;
+            if ((rc = set_q4_pos(m, 0))) return rc;
+            for (int l = 0; l < L; l++) {
+                kv_synth_kernel<<<blocks, 256, 0, s>>>(seed_k, 1, npos, m->cfg.ctx_len, m->kvdim, kvd_full, col0, 0,
+                                                       dk, l);
+                kv_synth_kernel<<<blocks, 256, 0, s>>>(seed_v, 1, npos, m->cfg.ctx_len, m->kvdim, kvd_full, col0, 0,
+                                                       dk + n, l);
+                CN_CUDA(cudaGetLastError());
+                if ((rc = kvq4_append(q4_layer(m, l, seq), dk, dk + n, m->kvdim, m->q4_pos, nullptr, 1, npos, nullptr,
+                                      0, s)))
+                    return rc;
+            }
+        }
+        CN_CUDA(cudaStreamSynchronize(s));
+        return CN_OK;
+    }
     const size_t seq_bytes = (size_t)m->seq_stride * m->kv_elem;
     uint8_t* kb = (uint8_t*)m->kc + (size_t)seq * seq_bytes;
     uint8_t* vb = (uint8_t*)m->vc + (size_t)seq * seq_bytes;

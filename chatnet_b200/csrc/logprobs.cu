@@ -517,6 +517,17 @@ int logprobs_launch(cn_ctx* ctx, int type, const void* logits, int64_t stride, i
     return CN_OK;
 }
 
+int logprobs_check(int vocab, const void* tokens, int top, const void* logprob, const void* entropy,
+                   const void* top_ids, const void* top_lp) {
+    CN_CHECK(top >= 0 && top <= kMaxTop && top <= vocab, CN_ERR_INVALID_ARG,
+             "top_n %d outside [0, min(%d, vocabulary %d)]", top, kMaxTop, vocab);
+    CN_CHECK(!logprob == !tokens, CN_ERR_INVALID_ARG, "tokens and their log probabilities go together");
+    CN_CHECK((top > 0) == (top_ids != nullptr) && (top > 0 || !top_lp), CN_ERR_INVALID_ARG,
+             "top_n and the outputs of the alternatives go together");
+    CN_CHECK(logprob || entropy || top_ids, CN_ERR_INVALID_ARG, "no output asked for");
+    return CN_OK;
+}
+
 }  // namespace cn
 
 using namespace cn;
@@ -529,12 +540,8 @@ extern "C" int cn_logprobs_dev(cn_ctx* ctx, int type, const void* d_logits, int6
     CN_CHECK(rows >= 1 && vocab >= 1 && row_stride >= vocab, CN_ERR_INVALID_ARG,
              "bad shape (%d rows, vocabulary %d, stride %lld)", rows, vocab, (long long)row_stride);
     CN_CHECK(row_stride < (1ll << 40) && vocab < (1 << 30), CN_ERR_INVALID_ARG, "row too large");
-    CN_CHECK(top_n >= 0 && top_n <= kMaxTop && top_n <= vocab, CN_ERR_INVALID_ARG,
-             "top_n %d outside [0, min(%d, vocabulary %d)]", top_n, kMaxTop, vocab);
-    CN_CHECK(!d_logprob == !d_tokens, CN_ERR_INVALID_ARG, "tokens and their log probabilities go together");
-    CN_CHECK((top_n > 0) == (d_top_ids != nullptr) && (top_n > 0 || !d_top_logprobs), CN_ERR_INVALID_ARG,
-             "top_n and the outputs of the alternatives go together");
-    CN_CHECK(d_logprob || d_entropy || d_top_ids, CN_ERR_INVALID_ARG, "no output asked for");
+    int rc = logprobs_check(vocab, d_tokens, top_n, d_logprob, d_entropy, d_top_ids, d_top_logprobs);
+    if (rc) return rc;
     CN_CHECK((uintptr_t)d_logits % (type == CN_TYPE_F16 ? 2 : 4) == 0, CN_ERR_INVALID_ARG, "misaligned logits");
     DeviceScope ds(ctx->device);
     return logprobs_launch(ctx, type, d_logits, row_stride, rows, vocab, d_tokens, top_n, d_logprob, d_entropy,

@@ -154,6 +154,27 @@ __global__ void half_rows_kernel(const float* __restrict__ x, __half* __restrict
     if (threadIdx.x == 0) inv[blockIdx.x] = iv;
 }
 
+__global__ void halves_kernel(const float* __restrict__ x, __half* __restrict__ hi, __half* __restrict__ lo,
+                              int64_t n4) {
+    const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
+    if (i >= n4) return;
+    const float4 v = reinterpret_cast<const float4*>(x)[i];
+    const uint2 h = make_uint2(pack_half2(v.x, v.y), pack_half2(v.z, v.w));
+    reinterpret_cast<uint2*>(hi)[i] = h;
+    if (lo) {
+        const __half2 a = *reinterpret_cast<const __half2*>(&h.x), b = *reinterpret_cast<const __half2*>(&h.y);
+        reinterpret_cast<uint2*>(lo)[i] = make_uint2(pack_half2(v.x - __low2float(a), v.y - __high2float(a)),
+                                                     pack_half2(v.z - __low2float(b), v.w - __high2float(b)));
+    }
+}
+
+int prefill_halves(cudaStream_t st, const float* x, __half* hi, __half* lo, int64_t n) {
+    const int64_t n4 = n / 4;
+    halves_kernel<<<(unsigned)((n4 + 255) / 256), 256, 0, st>>>(x, hi, lo, n4);
+    CN_CUDA(cudaGetLastError());
+    return CN_OK;
+}
+
 // TensorMath.ApplyRoPE (interleaved pairs) on the q and k rows of the n prompt
 // tokens (token t at position pos0 + t), then k and v into the cache, with
 // the decode attention kernels' arithmetic.  Also leaves fp16 copies of the new k and v

@@ -41,6 +41,7 @@ class LlamaConfig:
     rope_neox: bool = False    # TensorMath.ApplyRoPENeox (split-half pairs)
     act_gelu: bool = False     # TensorMath.GeluElementwiseMul
     norm_offset: bool = False  # TensorMath.RmsNormWithOffset (weights stored as w - 1)
+    kv_q4: bool = False        # 4-bit KV cache (cn_kvq4); overrides kv_f16
 
     @property
     def kv_dim(self) -> int:
@@ -53,7 +54,8 @@ class LlamaConfig:
     def to_c(self) -> N.LlamaConfigC:
         return N.LlamaConfigC(self.dim, self.hidden_dim, self.n_layers, self.n_heads,
                               self.n_kv_heads, self.head_dim, self.vocab, self.ctx_len,
-                              self.rope_base, self.rms_eps, N.KV_F16 if self.kv_f16 else N.KV_F32,
+                              self.rope_base, self.rms_eps,
+                              N.KV_Q4 if self.kv_q4 else N.KV_F16 if self.kv_f16 else N.KV_F32,
                               self.max_batch, int(self.rope_neox), int(self.act_gelu), int(self.norm_offset))
 
 
@@ -184,6 +186,32 @@ class CudaLlamaModel:
                                       rr.ctypes.data, out.ctypes.data), "cn_llama_sample")
         return out
 
+    def logprobs(self, batch: int, tokens=None, top_n: int = 0):
+        """Of the last step's logits on the device (cn_llama_logprobs): the tokens' log probabilities (None without
+        tokens), the entropies, and the top_n alternatives' ids and log probabilities ([batch, top_n])."""
+        tok = None if tokens is None else np.ascontiguousarray(tokens, dtype=np.int32)
+        if tok is not None and tok.size != batch:
+            raise ValueError(f"{tok.size} tokens for a batch of {batch}")
+        lp = None if tok is None else np.empty(max(batch, 0), np.float32)
+        ent = np.empty(max(batch, 0), np.float32)
+        ids = np.empty((max(batch, 0), max(top_n, 0)), np.int32)
+        tlp = np.empty((max(batch, 0), max(top_n, 0)), np.float32)
+
+        def ptr(a):
+            return a.ctypes.data if a is not None and a.size else None
+        check(N.lib().cn_llama_logprobs(self.handle, batch, ptr(tok), top_n, ptr(lp), ptr(ent), ptr(ids), ptr(tlp)),
+              "cn_llama_logprobs")
+        return lp, ent, ids, tlp
+
+    def score(self, token_ids, position: int = 0):
+        """Log probabilities of token_ids[1:] and the entropies of their predictions (cn_llama_score)."""
+        ids = np.ascontiguousarray(token_ids, dtype=np.int32)
+        lp = np.empty(max(ids.size - 1, 1), np.float32)
+        ent = np.empty_like(lp)
+        check(N.lib().cn_llama_score(self.handle, ids.ctypes.data, ids.size, position, lp.ctypes.data,
+                                     ent.ctypes.data), "cn_llama_score")
+        return lp, ent
+
     def step_kernels(self, batch: int) -> int:
         n = C.c_int(0)
         check(N.lib().cn_llama_step_kernels(self.handle, batch, C.byref(n)), "cn_llama_step_kernels")
@@ -215,7 +243,7 @@ class CudaLlamaModel:
         check(N.lib().cn_llama_kv_synth(self.handle, seq, npos, seed_k, seed_v), "cn_llama_kv_synth")
 
     def kv_read(self, seq: int, layer: int, pos0: int, npos: int):
-        dt = np.float16 if self.cfg.kv_f16 else np.float32
+        dt = np.float16 if self.cfg.kv_f16 and not self.cfg.kv_q4 else np.float32
         k = np.empty((npos, self.cfg.kv_dim), dt)
         v = np.empty((npos, self.cfg.kv_dim), dt)
         check(N.lib().cn_llama_kv_read(self.handle, seq, layer, pos0, npos, k.ctypes.data,
@@ -223,7 +251,7 @@ class CudaLlamaModel:
         return k, v
 
     def kv_write(self, seq: int, layer: int, pos0: int, k: np.ndarray, v: np.ndarray) -> None:
-        dt = np.float16 if self.cfg.kv_f16 else np.float32
+        dt = np.float16 if self.cfg.kv_f16 and not self.cfg.kv_q4 else np.float32
         k = np.ascontiguousarray(k, dt)
         v = np.ascontiguousarray(v, dt)
         check(N.lib().cn_llama_kv_write(self.handle, seq, layer, pos0, k.shape[0], k.ctypes.data,

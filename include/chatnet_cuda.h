@@ -318,12 +318,13 @@ typedef struct cn_llama cn_llama;
 
 #define CN_KV_F32 0 /* fp32 KV cache, as LlamaModel allocates (LlamaModel.cs:60-61) */
 #define CN_KV_F16 1 /* fp16 KV cache (rounded to nearest on store)                  */
+#define CN_KV_Q4 2  /* 4-bit KV cache (cn_kvq4; head_dim 32, 64, 96, 128 or 256)    */
 
 /* Hyper-parameters; mirrors LlamaConfig (Models/Llama/LlamaConfig.cs:23-39). */
 typedef struct {
     int dim, hidden_dim, n_layers, n_heads, n_kv_heads, head_dim, vocab, ctx_len;
     float rope_base, rms_eps;
-    int kv_dtype;  /* CN_KV_F32 or CN_KV_F16 */
+    int kv_dtype;  /* CN_KV_F32, CN_KV_F16 or CN_KV_Q4 */
     int max_batch; /* sequences decoded together, 1..32; each owns a KV slot */
     /* Variants other ChatNet models run on the same loop (0 = Llama):
      * rope_neox   split-half RoPE pairs (i, i + head_dim/2), TensorMath.ApplyRoPENeox
@@ -432,6 +433,19 @@ int cn_llama_step(cn_llama* m, int batch);
  * so a draw within rounding of a boundary may pick the neighbouring entry. */
 int cn_llama_sample(cn_llama* m, int batch, float temperature, int top_k, float top_p, const float* r_host,
                     int* tokens_host);
+/* cn_logprobs_dev for the logits the last decode step (or cn_llama_forward,
+ * batch 1) left on the device, with host tokens and results; batch rows.
+ * (no reference counterpart) */
+int cn_llama_logprobs(cn_llama* m, int batch, const int* tokens, int top_n, float* logprob_host, float* entropy_host,
+                      int* top_ids_host, float* top_logprobs_host);
+/* Scores a text: runs tokens[0..n-2] at positions pos.. of KV slot 0 (whose
+ * cache rows are written) and writes, for t < n - 1, the log probability of
+ * tokens[t + 1] after tokens[0..t] to logprob_host[t] and the entropy of that
+ * prediction to entropy_host[t] (may be NULL).  exp(-mean) is the text's
+ * perplexity.  As cn_llama_forward, one prefill pass where the model and the
+ * threshold allow, else one decode step per token.  (no reference
+ * counterpart) */
+int cn_llama_score(cn_llama* m, const int* tokens, int n, int pos, float* logprob_host, float* entropy_host);
 /* Kernel launches one decode step makes for `batch` (nodes of its graph). */
 int cn_llama_step_kernels(cn_llama* m, int batch, int* out_count);
 /* Times one projection's fused dequant-GEMV as the step runs it (activation
@@ -549,7 +563,9 @@ int cn_llama_prepare(cn_llama* m, int batch);
 
 /* KV cache access for seeding and checking (no reference counterpart; the
  * reference fills its cache only through Forward).  Element type follows
- * cfg.kv_dtype (float or uint16 fp16 bits), layout [npos][n_kv*head_dim]. */
+ * cfg.kv_dtype (float or uint16 fp16 bits), layout [npos][n_kv*head_dim];
+ * a 4-bit cache takes floats, which it rounds, and gives the values that it
+ * stands for. */
 int cn_llama_kv_write(cn_llama* m, int seq, int layer, int pos0, int npos, const void* k_host,
                       const void* v_host);
 int cn_llama_kv_read(cn_llama* m, int seq, int layer, int pos0, int npos, void* k_host,
