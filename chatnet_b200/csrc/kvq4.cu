@@ -22,95 +22,131 @@ __device__ __forceinline__ float tame(float x) {
     return x == x ? fminf(fmaxf(x, -kMaxX), kMaxX) : 0.f;
 }
 
-// The nearest level to x / d, halves up.  floor(x / d + 8.5) is off by one at
-// most (the reciprocal, product and sum are each rounded), so the borders
-// d * (q - 8.5) and d * (q - 7.5), exact in fp32 (11 + 5 bits), decide.
-__device__ __forceinline__ uint32_t level(float x, float d, float inv) {
-    float q = floorf(__fadd_rn(__fmul_rn(x, inv), 8.5f));
-    q = fminf(fmaxf(q, 0.f), 15.f);
-    const float s = d < 0.f ? -x : x, a = fabsf(d);
-    if (q < 15.f && s >= __fmul_rn(a, q - 7.5f)) q += 1.f;
-    else if (q > 0.f && s < __fmul_rn(a, q - 8.5f)) q -= 1.f;
-    return (uint32_t)(int)q;
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// The nearest level to x / d, halves up, in the low 16 bits.  x * (1 / d)
+// rounded to a whole number q is off by one at most; the rest x - d q is exact
+// in fp32 there (both terms lie within a factor of two, or q is 0) and decides
+// against half a step.
+__device__ __forceinline__ uint32_t level(float x, float d, float inv) {
+    constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: whole numbers from here on
+    const float f = fmaf(x, inv, kWhole + 8.f), q = f - (kWhole + 8.f);
+    const float rest = __uint_as_float(__float_as_uint(fmaf(-d, q, x)) ^ (__float_as_uint(d) & 0x80000000u));
+    const float half = 0.5f * fabsf(d);
+    int n = __float_as_int(f);
+    if (rest >= half) n++;
+    if (rest < -half) n--;
+    const int zero = __float_as_int(kWhole);
+    return (uint32_t)min(max(n, zero), zero + 15);
+}
+
+// Which row a thread's eight lanes take: four tokens of a head side by side (their
+// rows are neighbours in the cache, their scales one 32-byte sector), then the
+// next head, then the next tokens.  shift: 2, or 0 for fewer than four tokens.
+struct RowAt {
+    int b, i, h;
+    bool in;
+    __device__ RowAt(uint32_t r, uint32_t n_slots, int n_new, int n_kv, int shift) {
+        const uint32_t t = r >> shift, groups = ((uint32_t)n_new + (1u << shift) - 1) >> shift;
+        h = (int)(t % (uint32_t)n_kv);
+        const uint32_t g = t / (uint32_t)n_kv;
+        b = (int)(g / groups);
+        i = (int)(((g % groups) << shift) | (r & ((1u << shift) - 1)));
+        in = r < n_slots && i < n_new;
+    }
+};
 
 }  // namespace
 
-// Eight lanes a row: lane g holds the values 32 b + 8 i + g, so a block's
-// minimum and maximum need three shuffles for four rows at once, a lane's
-// values are exactly the nibbles of its chunk, and a load instruction still
-// fetches whole 32-byte sectors.
+// Eight lanes a row, so that a block's minimum and maximum need three shuffles
+// for four rows at once.  Lane l holds the values 4l .. 4l + 3 of every block (16-byte
+// loads and stores): the nibbles i = l >> 1 of chunks g = 4 (l & 1) .. + 3.  A
+// word holds two 16-bit pieces; the four lanes of one parity OR their nibbles
+// together, and lane l then writes chunk 4 (l & 1) + (l >> 1).  Bound: the fp32
+// rows' bytes.
 template <int NB>
 __global__ void __launch_bounds__(kRowThreads)
     kvq4_append_kernel(const float* __restrict__ k, const float* __restrict__ v, int64_t kv_stride,
                        const int* __restrict__ pos, const int* __restrict__ count, int n_new, int n_kv,
-                       int64_t n_rows, const float2* __restrict__ rope, int neox, uint8_t* __restrict__ kq,
+                       uint32_t n_slots, const float2* __restrict__ rope, int neox, uint8_t* __restrict__ kq,
                        __half* __restrict__ kd, uint8_t* __restrict__ vq, __half* __restrict__ vd, int64_t seq_rows,
-                       int ctx_len) {
-    constexpr int HD = 32 * NB;
-    const int g = threadIdx.x & 7;
-    const int64_t r = (int64_t)blockIdx.x * (kRowThreads / 8) + (threadIdx.x >> 3);
+                       int ctx_len, int wide, int shift) {
+    constexpr int HD = 32 * NB, H = HD / 2;
+    const int l = threadIdx.x & 7;
+    const RowAt at(blockIdx.x * (kRowThreads / 8) + (threadIdx.x >> 3), n_slots, n_new, n_kv, shift);
     const bool is_v = blockIdx.y != 0;
-    bool live = r < n_rows && (is_v ? v : k) != nullptr;
+    bool live = at.in && (is_v ? v : k) != nullptr;
     int64_t tok = 0, dst = 0;
-    int h = 0, p = 0;
+    const int h = at.h;
+    int p = 0;
     if (live) {
-        h = (int)(r % n_kv);
-        tok = r / n_kv;
-        const int b = (int)(tok / n_new), i = (int)(tok % n_new);
+        tok = (int64_t)at.b * n_new + at.i;
         int p0;
-        live = i < kvq4_active(pos, count, b, n_new, ctx_len, p0);
-        p = p0 + i;
-        dst = (int64_t)b * seq_rows + (int64_t)h * ctx_len + p;
+        live = at.i < kvq4_active(pos, count, at.b, n_new, ctx_len, p0);
+        p = p0 + at.i;
+        dst = (int64_t)at.b * seq_rows + (int64_t)h * ctx_len + p;
     }
-    float x[NB][4];
-    if (live) {
-        const float* src = (is_v ? v : k) + tok * kv_stride + (int64_t)h * HD + g;
+    float4 x[NB];
+    const float* src = (is_v ? v : k) + tok * kv_stride + (int64_t)h * HD;
+    auto get = [&](int e) {  // (rows that are not 16-byte aligned: value by value)
+        return wide ? *reinterpret_cast<const float4*>(src + e)
+                    : make_float4(src[e], src[e + 1], src[e + 2], src[e + 3]);
+    };
 #pragma unroll
-        for (int b = 0; b < NB; b++)
+    for (int b = 0; b < NB; b++) x[b] = live ? get(32 * b + 4 * l) : make_float4(0.f, 0.f, 0.f, 0.f);
+    if (!is_v && rope && live) {
+        const float2* tab = rope + (int64_t)p * H;
+        auto lo = [](float a, float c, float2 cs) { return __fsub_rn(__fmul_rn(a, cs.x), __fmul_rn(c, cs.y)); };
+        auto hi = [](float a, float c, float2 cs) { return __fadd_rn(__fmul_rn(a, cs.y), __fmul_rn(c, cs.x)); };
+        if (!neox) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[b][i] = src[32 * b + 8 * i];
-    } else {
+            for (int b = 0; b < NB; b++) {
+                const float2 c0 = tab[16 * b + 2 * l], c1 = tab[16 * b + 2 * l + 1];
+                const float4 y = x[b];
+                x[b] = make_float4(lo(y.x, y.y, c0), hi(y.x, y.y, c0), lo(y.z, y.w, c1), hi(y.z, y.w, c1));
+            }
+        } else if constexpr (NB % 2 == 0) {  // e pairs with e + hd/2: the same lane holds both
 #pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[b][i] = 0.f;
-    }
-    if (!is_v && rope) {
-        const float2* tab = rope + (int64_t)p * (HD / 2);  // (p = 0 for a row that is not live)
-        if (neox) {
-            // e pairs with e + hd/2: a lane holds both (hd/2 is a multiple of 16)
-#pragma unroll
-            for (int n = 0; n < 2 * NB; n++) {
-                const int e0 = n, e1 = n + 2 * NB;  // in units of 8 values
-                const float2 cs = tab[8 * n + g];
-                float &a = x[e0 / 4][e0 % 4], &c = x[e1 / 4][e1 % 4];
-                const float ra = __fsub_rn(__fmul_rn(a, cs.x), __fmul_rn(c, cs.y));
-                const float rc = __fadd_rn(__fmul_rn(a, cs.y), __fmul_rn(c, cs.x));
-                a = ra;
-                c = rc;
+            for (int b = 0; b < NB / 2; b++) {
+                const float2* cs = tab + 32 * b + 4 * l;
+                const float2 c0 = cs[0], c1 = cs[1], c2 = cs[2], c3 = cs[3];
+                const float4 y = x[b], z = x[b + NB / 2];
+                x[b] = make_float4(lo(y.x, z.x, c0), lo(y.y, z.y, c1), lo(y.z, z.z, c2), lo(y.w, z.w, c3));
+                x[b + NB / 2] = make_float4(hi(y.x, z.x, c0), hi(y.y, z.y, c1), hi(y.z, z.z, c2), hi(y.w, z.w, c3));
             }
         } else {
 #pragma unroll
-            for (int n = 0; n < 4 * NB; n++) {
-                const float own = x[n / 4][n % 4];
-                const float oth = __shfl_xor_sync(0xffffffffu, own, 1);
-                const float2 cs = tab[4 * n + (g >> 1)];
-                x[n / 4][n % 4] = (g & 1) ? __fadd_rn(__fmul_rn(oth, cs.y), __fmul_rn(own, cs.x))
-                                          : __fsub_rn(__fmul_rn(own, cs.x), __fmul_rn(oth, cs.y));
+            for (int b = 0; b < NB; b++) {
+                const int e = 32 * b + 4 * l;
+                const bool first = e < H;
+                const float4 y = x[b], z = get(first ? e + H : e - H);
+                const float2* cs = tab + (first ? e : e - H);
+                const float2 c0 = cs[0], c1 = cs[1], c2 = cs[2], c3 = cs[3];
+                x[b] = first ? make_float4(lo(y.x, z.x, c0), lo(y.y, z.y, c1), lo(y.z, z.z, c2), lo(y.w, z.w, c3))
+                             : make_float4(hi(z.x, y.x, c0), hi(z.y, y.y, c1), hi(z.z, y.z, c2), hi(z.w, y.w, c3));
             }
         }
     }
-    uint32_t piece[NB];
-    float scale[NB];
+    uint32_t piece[NB];  // of chunk 4 (l & 1) + (l >> 1)
+    float scale = 0.f;   // of block l
+    const int nib = 4 * (l >> 1);
 #pragma unroll
     for (int b = 0; b < NB; b++) {
-        float lo = 0.f, hi = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            x[b][i] = tame(x[b][i]);
-            lo = i ? fminf(lo, x[b][i]) : x[b][i];
-            hi = i ? fmaxf(hi, x[b][i]) : x[b][i];
+        float4 y = x[b];
+        float lo = min_nan(min_nan(y.x, y.y), min_nan(y.z, y.w)), hi = max_nan(max_nan(y.x, y.y), max_nan(y.z, y.w));
+        if (!(lo >= -kMaxX && hi <= kMaxX)) {  // (rarely)
+            y = make_float4(tame(y.x), tame(y.y), tame(y.z), tame(y.w));
+            lo = fminf(fminf(y.x, y.y), fminf(y.z, y.w));
+            hi = fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w));
         }
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) {
@@ -118,15 +154,23 @@ __global__ void __launch_bounds__(kRowThreads)
             hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         }
         const float d = __half2float(__float2half_rn(__fmul_rn(-lo >= hi ? lo : hi, -0.125f)));
-        const float inv = d == 0.f ? 0.f : __frcp_rn(d);  // (inv 0: level 8 for every value)
-        scale[b] = d;
-        uint32_t w = 0;
+        uint32_t w0 = 0x00080008u << nib, w1 = w0;  // level 8: the value 0
+        if (d != 0.f) {
+            const float inv = __frcp_rn(d);
+            w0 = __byte_perm(level(y.x, d, inv), level(y.y, d, inv), 0x5410) << nib;
+            w1 = __byte_perm(level(y.z, d, inv), level(y.w, d, inv), 0x5410) << nib;
+        }
 #pragma unroll
-        for (int i = 0; i < 4; i++) w |= (d == 0.f ? 8u : level(x[b][i], d, inv)) << (4 * i);
-        piece[b] = w;
+        for (int o = 2; o <= 4; o <<= 1) {
+            w0 |= __shfl_xor_sync(0xffffffffu, w0, o);
+            w1 |= __shfl_xor_sync(0xffffffffu, w1, o);
+        }
+        const uint32_t w = (l >> 2) ? w1 : w0;
+        piece[b] = (l & 2) ? w >> 16 : w & 0xFFFFu;
+        if (l == b) scale = d;
     }
     if (!live) return;
-    uint8_t* q = (is_v ? vq : kq) + dst * (HD / 2) + g * (2 * NB);
+    uint8_t* q = (is_v ? vq : kq) + dst * (HD / 2) + (4 * (l & 1) + (l >> 1)) * (2 * NB);
     if constexpr (NB == 8) {
         *reinterpret_cast<uint4*>(q) = make_uint4(piece[0] | piece[1] << 16, piece[2] | piece[3] << 16,
                                                   piece[4] | piece[5] << 16, piece[6] | piece[7] << 16);
@@ -138,39 +182,58 @@ __global__ void __launch_bounds__(kRowThreads)
 #pragma unroll
         for (int b = 0; b < NB; b++) reinterpret_cast<uint16_t*>(q)[b] = (uint16_t)piece[b];
     }
-    __half* d = (is_v ? vd : kd) + dst * NB;
-#pragma unroll
-    for (int b = 0; b < NB; b++)
-        if (g == b) d[b] = __float2half_rn(scale[b]);
+    if (l < NB) ((is_v ? vd : kd) + dst * NB)[l] = __float2half_rn(scale);
 }
 
 template <int NB>
 __global__ void __launch_bounds__(kRowThreads)
     kvq4_read_kernel(float* __restrict__ k, float* __restrict__ v, int64_t kv_stride, const int* __restrict__ pos,
-                     const int* __restrict__ count, int n_new, int n_kv, int64_t n_rows, const uint8_t* __restrict__ kq,
+                     const int* __restrict__ count, int n_new, int n_kv, uint32_t n_slots,
+                     const uint8_t* __restrict__ kq,
                      const __half* __restrict__ kd, const uint8_t* __restrict__ vq, const __half* __restrict__ vd,
-                     int64_t seq_rows, int ctx_len) {
+                     int64_t seq_rows, int ctx_len, int wide, int shift) {
     constexpr int HD = 32 * NB;
-    const int g = threadIdx.x & 7;
-    const int64_t r = (int64_t)blockIdx.x * (kRowThreads / 8) + (threadIdx.x >> 3);
+    const int l = threadIdx.x & 7;
+    const RowAt at(blockIdx.x * (kRowThreads / 8) + (threadIdx.x >> 3), n_slots, n_new, n_kv, shift);
     const bool is_v = blockIdx.y != 0;
     float* out = is_v ? v : k;
-    if (r >= n_rows || !out) return;
-    const int h = (int)(r % n_kv);
-    const int64_t tok = r / n_kv;
-    const int b = (int)(tok / n_new), i = (int)(tok % n_new);
+    if (!at.in || !out) return;
     int p0;
-    if (i >= kvq4_active(pos, count, b, n_new, ctx_len, p0)) return;
-    const int64_t src = (int64_t)b * seq_rows + (int64_t)h * ctx_len + p0 + i;
-    const uint16_t* q = reinterpret_cast<const uint16_t*>((is_v ? vq : kq) + src * (HD / 2) + g * (2 * NB));
+    if (at.i >= kvq4_active(pos, count, at.b, n_new, ctx_len, p0)) return;
+    const int h = at.h;
+    const int64_t tok = (int64_t)at.b * n_new + at.i;
+    const int64_t src = (int64_t)at.b * seq_rows + (int64_t)h * ctx_len + p0 + at.i;
+    // chunks 4 (l & 1) .. + 3 of the row, 4 NB pieces
+    uint32_t w[2 * NB];
+    const uint8_t* q = (is_v ? vq : kq) + src * (HD / 2) + (l & 1) * (8 * NB);
+    if constexpr (NB % 2 == 0) {
+#pragma unroll
+        for (int j = 0; j < NB / 2; j++) {
+            const uint4 u = reinterpret_cast<const uint4*>(q)[j];
+            w[4 * j] = u.x, w[4 * j + 1] = u.y, w[4 * j + 2] = u.z, w[4 * j + 3] = u.w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 2 * NB; j++) w[j] = reinterpret_cast<const uint32_t*>(q)[j];
+    }
     const __half* d = (is_v ? vd : kd) + src * NB;
-    out += tok * kv_stride + (int64_t)h * HD + g;
+    out += tok * kv_stride + (int64_t)h * HD + 4 * l;
+    const int nib = 4 * (l >> 1);
 #pragma unroll
     for (int bl = 0; bl < NB; bl++) {
-        const uint32_t w = q[bl];
         const float s = __half2float(d[bl]);
+        float x[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) out[32 * bl + 8 * j] = s * (float)((int)((w >> (4 * j)) & 15u) - 8);
+        for (int g = 0; g < 4; g++) {
+            const int piece = g * NB + bl;
+            x[g] = s * (float)((int)((w[piece / 2] >> (16 * (piece % 2) + nib)) & 15u) - 8);
+        }
+        if (wide) {
+            *reinterpret_cast<float4*>(out + 32 * bl) = make_float4(x[0], x[1], x[2], x[3]);
+        } else {
+#pragma unroll
+            for (int g = 0; g < 4; g++) out[32 * bl + g] = x[g];
+        }
     }
 }
 
@@ -196,11 +259,13 @@ int kvq4_check(const cn_ctx* ctx, const cn_kvq4* c, int batch, int n_new) {
     return CN_OK;
 }
 
-static int row_grid(const cn_kvq4& c, int batch, int n_new, int64_t* n_rows, dim3* grid) {
-    *n_rows = (int64_t)batch * n_new * c.n_kv_heads;
-    const int64_t ctas = (*n_rows + kRowThreads / 8 - 1) / (kRowThreads / 8);
-    CN_CHECK(ctas < (1ll << 31), CN_ERR_INVALID_ARG, "too many rows (%lld)", (long long)*n_rows);
-    *grid = dim3((unsigned)ctas, 2);
+static int row_grid(const cn_kvq4& c, int batch, int n_new, uint32_t* n_slots, int* shift, dim3* grid) {
+    *shift = n_new >= 4 ? 2 : 0;
+    const int64_t groups = ((int64_t)n_new + (1 << *shift) - 1) >> *shift;
+    const int64_t n = (groups * batch * c.n_kv_heads) << *shift;
+    CN_CHECK(n < (1ll << 31), CN_ERR_INVALID_ARG, "too many rows (%lld)", (long long)n);
+    *n_slots = (uint32_t)n;
+    *grid = dim3((unsigned)((n + kRowThreads / 8 - 1) / (kRowThreads / 8)), 2);
     return CN_OK;
 }
 
@@ -215,15 +280,17 @@ static int row_grid(const cn_kvq4& c, int batch, int n_new, int64_t* n_rows, dim
 
 int kvq4_append(const cn_kvq4& c, const float* k, const float* v, int64_t kv_stride, const int* pos, const int* count,
                 int batch, int n_new, const float2* rope, int neox, cudaStream_t st) {
-    int64_t n;
+    uint32_t n;
+    int shift;
     dim3 grid;
-    int rc = row_grid(c, batch, n_new, &n, &grid);
+    int rc = row_grid(c, batch, n_new, &n, &shift, &grid);
     if (rc) return rc;
+    const int wide = ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && kv_stride % 4 == 0;
 #define CALL(NB)                                                                                                 \
     kvq4_append_kernel<NB><<<grid, kRowThreads, 0, st>>>(                                                        \
         k, v, kv_stride, pos, count, n_new, c.n_kv_heads, n, rope, neox, static_cast<uint8_t*>(c.k_quants),      \
         static_cast<__half*>(c.k_scales), static_cast<uint8_t*>(c.v_quants), static_cast<__half*>(c.v_scales),   \
-        kvq4_seq_rows(c), c.ctx_len);                                                                            \
+        kvq4_seq_rows(c), c.ctx_len, wide, shift);                                                                            \
     break
     KVQ4_BY_HD(c.head_dim, CALL)
 #undef CALL
@@ -233,15 +300,17 @@ int kvq4_append(const cn_kvq4& c, const float* k, const float* v, int64_t kv_str
 
 int kvq4_read(const cn_kvq4& c, float* k, float* v, int64_t kv_stride, const int* pos, const int* count, int batch,
               int n_new, cudaStream_t st) {
-    int64_t n;
+    uint32_t n;
+    int shift;
     dim3 grid;
-    int rc = row_grid(c, batch, n_new, &n, &grid);
+    int rc = row_grid(c, batch, n_new, &n, &shift, &grid);
     if (rc) return rc;
+    const int wide = ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && kv_stride % 4 == 0;
 #define CALL(NB)                                                                                                     \
     kvq4_read_kernel<NB><<<grid, kRowThreads, 0, st>>>(                                                              \
         k, v, kv_stride, pos, count, n_new, c.n_kv_heads, n, static_cast<const uint8_t*>(c.k_quants),                \
         static_cast<const __half*>(c.k_scales), static_cast<const uint8_t*>(c.v_quants),                             \
-        static_cast<const __half*>(c.v_scales), kvq4_seq_rows(c), c.ctx_len);                                        \
+        static_cast<const __half*>(c.v_scales), kvq4_seq_rows(c), c.ctx_len, wide, shift);                                  \
     break
     KVQ4_BY_HD(c.head_dim, CALL)
 #undef CALL
