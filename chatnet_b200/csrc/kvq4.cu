@@ -15,7 +15,7 @@ namespace cn {
 
 namespace {
 
-constexpr int kRowThreads = 256;  // 8 lanes a row: 32 rows per CTA
+constexpr int kRowThreads = 256;  // 8 lanes a row, 32 rows a CTA
 constexpr float kMaxX = 524032.f;  // 8 * 65504
 
 __device__ __forceinline__ float tame(float x) {
@@ -33,12 +33,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// The nearest level to x / d, halves up, in the low 16 bits.  x * (1 / d)
-// rounded to a whole number q is off by one at most; the rest x - d q is exact
-// in fp32 there (both terms lie within a factor of two, or q is 0) and decides
-// against half a step.
-__device__ __forceinline__ uint32_t level(float x, float d, float inv) {
-    constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: whole numbers from here on
+constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: whole numbers from here on
+
+// The nearest level to x / d, halves up, in the low 16 bits, for any d.  x times
+// the rounded 1 / d, rounded to a whole number q, is off by one at most; the rest
+// x - d q is exact in fp32 there (both terms lie within a factor of two, or q is
+// 0) and decides against half a step.
+__device__ __noinline__ uint32_t level_exact(float x, float d, float inv) {
     const float f = fmaf(x, inv, kWhole + 8.f), q = f - (kWhole + 8.f);
     const float rest = __uint_as_float(__float_as_uint(fmaf(-d, q, x)) ^ (__float_as_uint(d) & 0x80000000u));
     const float half = 0.5f * fabsf(d);
@@ -48,20 +49,33 @@ __device__ __forceinline__ uint32_t level(float x, float d, float inv) {
     const int zero = __float_as_int(kWhole);
     return (uint32_t)min(max(n, zero), zero + 15);
 }
+// The same away from the borders: `near` is set where x / d (known to 2^-21) may
+// be within 10^-5 of one.  d is at least 2^-14, so that x / d is above -8.01.
+__device__ __forceinline__ uint32_t level(float x, float inv, bool& near) {
+    const float f = fmaf(x, inv, kWhole + 8.f), q = f - (kWhole + 8.f);
+    near |= fabsf(fmaf(x, inv, -q)) > 0.49999f;
+    return (uint32_t)min(__float_as_int(f), __float_as_int(kWhole) + 15);
+}
 
-// Which row a thread's eight lanes take: four tokens of a head side by side (their
-// rows are neighbours in the cache, their scales one 32-byte sector), then the
-// next head, then the next tokens.  shift: 2, or 0 for fewer than four tokens.
+// Which row a thread's eight lanes take.  Many tokens: a CTA has 32 tokens of one
+// head of one sequence (their rows are neighbours in the cache), from the block's
+// indexes alone.  Few: rows side by side, heads first.
 struct RowAt {
     int b, i, h;
     bool in;
-    __device__ RowAt(uint32_t r, uint32_t n_slots, int n_new, int n_kv, int shift) {
-        const uint32_t t = r >> shift, groups = ((uint32_t)n_new + (1u << shift) - 1) >> shift;
-        h = (int)(t % (uint32_t)n_kv);
-        const uint32_t g = t / (uint32_t)n_kv;
-        b = (int)(g / groups);
-        i = (int)(((g % groups) << shift) | (r & ((1u << shift) - 1)));
-        in = r < n_slots && i < n_new;
+    __device__ RowAt(uint32_t n_rows, int n_new, int n_kv, bool many) {
+        if (many) {
+            i = blockIdx.x * 32 + (threadIdx.x >> 3);
+            h = blockIdx.y >> 1;
+            b = blockIdx.z;
+            in = i < n_new;
+        } else {
+            const uint32_t r = blockIdx.x * 32 + (threadIdx.x >> 3), t = r / (uint32_t)n_kv;
+            h = (int)(r % (uint32_t)n_kv);
+            b = (int)(t / (uint32_t)n_new);
+            i = (int)(t % (uint32_t)n_new);
+            in = r < n_rows;
+        }
     }
 };
 
@@ -77,13 +91,13 @@ template <int NB>
 __global__ void __launch_bounds__(kRowThreads)
     kvq4_append_kernel(const float* __restrict__ k, const float* __restrict__ v, int64_t kv_stride,
                        const int* __restrict__ pos, const int* __restrict__ count, int n_new, int n_kv,
-                       uint32_t n_slots, const float2* __restrict__ rope, int neox, uint8_t* __restrict__ kq,
+                       uint32_t n_rows, const float2* __restrict__ rope, int neox, uint8_t* __restrict__ kq,
                        __half* __restrict__ kd, uint8_t* __restrict__ vq, __half* __restrict__ vd, int64_t seq_rows,
-                       int ctx_len, int wide, int shift) {
+                       int ctx_len, int wide, int many) {
     constexpr int HD = 32 * NB, H = HD / 2;
     const int l = threadIdx.x & 7;
-    const RowAt at(blockIdx.x * (kRowThreads / 8) + (threadIdx.x >> 3), n_slots, n_new, n_kv, shift);
-    const bool is_v = blockIdx.y != 0;
+    const RowAt at(n_rows, n_new, n_kv, many);
+    const bool is_v = blockIdx.y & 1;
     bool live = at.in && (is_v ? v : k) != nullptr;
     int64_t tok = 0, dst = 0;
     const int h = at.h;
@@ -110,15 +124,17 @@ __global__ void __launch_bounds__(kRowThreads)
         if (!neox) {
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                const float2 c0 = tab[16 * b + 2 * l], c1 = tab[16 * b + 2 * l + 1];
+                const float4 cs = *reinterpret_cast<const float4*>(tab + 16 * b + 2 * l);
+                const float2 c0 = {cs.x, cs.y}, c1 = {cs.z, cs.w};
                 const float4 y = x[b];
                 x[b] = make_float4(lo(y.x, y.y, c0), hi(y.x, y.y, c0), lo(y.z, y.w, c1), hi(y.z, y.w, c1));
             }
         } else if constexpr (NB % 2 == 0) {  // e pairs with e + hd/2: the same lane holds both
 #pragma unroll
             for (int b = 0; b < NB / 2; b++) {
-                const float2* cs = tab + 32 * b + 4 * l;
-                const float2 c0 = cs[0], c1 = cs[1], c2 = cs[2], c3 = cs[3];
+                const float4* cs = reinterpret_cast<const float4*>(tab + 32 * b + 4 * l);
+                const float4 s0 = cs[0], s1 = cs[1];
+                const float2 c0 = {s0.x, s0.y}, c1 = {s0.z, s0.w}, c2 = {s1.x, s1.y}, c3 = {s1.z, s1.w};
                 const float4 y = x[b], z = x[b + NB / 2];
                 x[b] = make_float4(lo(y.x, z.x, c0), lo(y.y, z.y, c1), lo(y.z, z.z, c2), lo(y.w, z.w, c3));
                 x[b + NB / 2] = make_float4(hi(y.x, z.x, c0), hi(y.y, z.y, c1), hi(y.z, z.z, c2), hi(y.w, z.w, c3));
@@ -157,8 +173,15 @@ __global__ void __launch_bounds__(kRowThreads)
         uint32_t w0 = 0x00080008u << nib, w1 = w0;  // level 8: the value 0
         if (d != 0.f) {
             const float inv = __frcp_rn(d);
-            w0 = __byte_perm(level(y.x, d, inv), level(y.y, d, inv), 0x5410) << nib;
-            w1 = __byte_perm(level(y.z, d, inv), level(y.w, d, inv), 0x5410) << nib;
+            bool near = fabsf(d) < 6.103515625e-5f;
+            uint32_t q0 = level(y.x, inv, near), q1 = level(y.y, inv, near), q2 = level(y.z, inv, near),
+                     q3 = level(y.w, inv, near);
+            if (near) {
+                q0 = level_exact(y.x, d, inv), q1 = level_exact(y.y, d, inv), q2 = level_exact(y.z, d, inv),
+                q3 = level_exact(y.w, d, inv);
+            }
+            w0 = __byte_perm(q0, q1, 0x5410) << nib;
+            w1 = __byte_perm(q2, q3, 0x5410) << nib;
         }
 #pragma unroll
         for (int o = 2; o <= 4; o <<= 1) {
@@ -188,14 +211,14 @@ __global__ void __launch_bounds__(kRowThreads)
 template <int NB>
 __global__ void __launch_bounds__(kRowThreads)
     kvq4_read_kernel(float* __restrict__ k, float* __restrict__ v, int64_t kv_stride, const int* __restrict__ pos,
-                     const int* __restrict__ count, int n_new, int n_kv, uint32_t n_slots,
+                     const int* __restrict__ count, int n_new, int n_kv, uint32_t n_rows,
                      const uint8_t* __restrict__ kq,
                      const __half* __restrict__ kd, const uint8_t* __restrict__ vq, const __half* __restrict__ vd,
-                     int64_t seq_rows, int ctx_len, int wide, int shift) {
+                     int64_t seq_rows, int ctx_len, int wide, int many) {
     constexpr int HD = 32 * NB;
     const int l = threadIdx.x & 7;
-    const RowAt at(blockIdx.x * (kRowThreads / 8) + (threadIdx.x >> 3), n_slots, n_new, n_kv, shift);
-    const bool is_v = blockIdx.y != 0;
+    const RowAt at(n_rows, n_new, n_kv, many);
+    const bool is_v = blockIdx.y & 1;
     float* out = is_v ? v : k;
     if (!at.in || !out) return;
     int p0;
@@ -259,13 +282,13 @@ int kvq4_check(const cn_ctx* ctx, const cn_kvq4* c, int batch, int n_new) {
     return CN_OK;
 }
 
-static int row_grid(const cn_kvq4& c, int batch, int n_new, uint32_t* n_slots, int* shift, dim3* grid) {
-    *shift = n_new >= 4 ? 2 : 0;
-    const int64_t groups = ((int64_t)n_new + (1 << *shift) - 1) >> *shift;
-    const int64_t n = (groups * batch * c.n_kv_heads) << *shift;
+static int row_grid(const cn_kvq4& c, int batch, int n_new, uint32_t* n_rows, int* many, dim3* grid) {
+    const int64_t n = (int64_t)batch * n_new * c.n_kv_heads;
     CN_CHECK(n < (1ll << 31), CN_ERR_INVALID_ARG, "too many rows (%lld)", (long long)n);
-    *n_slots = (uint32_t)n;
-    *grid = dim3((unsigned)((n + kRowThreads / 8 - 1) / (kRowThreads / 8)), 2);
+    *n_rows = (uint32_t)n;
+    *many = n_new >= 16 && batch <= 65535 && c.n_kv_heads <= 32767;
+    *grid = *many ? dim3((unsigned)((n_new + 31) / 32), 2 * (unsigned)c.n_kv_heads, (unsigned)batch)
+                  : dim3((unsigned)((n + 31) / 32), 2);
     return CN_OK;
 }
 
@@ -281,16 +304,16 @@ static int row_grid(const cn_kvq4& c, int batch, int n_new, uint32_t* n_slots, i
 int kvq4_append(const cn_kvq4& c, const float* k, const float* v, int64_t kv_stride, const int* pos, const int* count,
                 int batch, int n_new, const float2* rope, int neox, cudaStream_t st) {
     uint32_t n;
-    int shift;
+    int many;
     dim3 grid;
-    int rc = row_grid(c, batch, n_new, &n, &shift, &grid);
+    int rc = row_grid(c, batch, n_new, &n, &many, &grid);
     if (rc) return rc;
     const int wide = ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && kv_stride % 4 == 0;
 #define CALL(NB)                                                                                                 \
     kvq4_append_kernel<NB><<<grid, kRowThreads, 0, st>>>(                                                        \
         k, v, kv_stride, pos, count, n_new, c.n_kv_heads, n, rope, neox, static_cast<uint8_t*>(c.k_quants),      \
         static_cast<__half*>(c.k_scales), static_cast<uint8_t*>(c.v_quants), static_cast<__half*>(c.v_scales),   \
-        kvq4_seq_rows(c), c.ctx_len, wide, shift);                                                                            \
+        kvq4_seq_rows(c), c.ctx_len, wide, many);                                                                            \
     break
     KVQ4_BY_HD(c.head_dim, CALL)
 #undef CALL
@@ -301,16 +324,16 @@ int kvq4_append(const cn_kvq4& c, const float* k, const float* v, int64_t kv_str
 int kvq4_read(const cn_kvq4& c, float* k, float* v, int64_t kv_stride, const int* pos, const int* count, int batch,
               int n_new, cudaStream_t st) {
     uint32_t n;
-    int shift;
+    int many;
     dim3 grid;
-    int rc = row_grid(c, batch, n_new, &n, &shift, &grid);
+    int rc = row_grid(c, batch, n_new, &n, &many, &grid);
     if (rc) return rc;
     const int wide = ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && kv_stride % 4 == 0;
 #define CALL(NB)                                                                                                     \
     kvq4_read_kernel<NB><<<grid, kRowThreads, 0, st>>>(                                                              \
         k, v, kv_stride, pos, count, n_new, c.n_kv_heads, n, static_cast<const uint8_t*>(c.k_quants),                \
         static_cast<const __half*>(c.k_scales), static_cast<const uint8_t*>(c.v_quants),                             \
-        static_cast<const __half*>(c.v_scales), kvq4_seq_rows(c), c.ctx_len, wide, shift);                                  \
+        static_cast<const __half*>(c.v_scales), kvq4_seq_rows(c), c.ctx_len, wide, many);                                  \
     break
     KVQ4_BY_HD(c.head_dim, CALL)
 #undef CALL
@@ -332,8 +355,8 @@ int cn_kvq4_append_dev(cn_ctx* ctx, const cn_kvq4* cache, const float* d_k, cons
     CN_CHECK(d_k && d_v && d_pos, CN_ERR_INVALID_ARG, "null argument");
     CN_CHECK(kv_stride >= (int64_t)cache->n_kv_heads * cache->head_dim, CN_ERR_INVALID_ARG,
              "kv_stride %lld is below %d values", (long long)kv_stride, cache->n_kv_heads * cache->head_dim);
-    CN_CHECK(((uintptr_t)d_k | (uintptr_t)d_v) % 4 == 0 && (uintptr_t)d_rope % 8 == 0, CN_ERR_INVALID_ARG,
-             "misaligned pointer");
+    CN_CHECK(((uintptr_t)d_k | (uintptr_t)d_v) % 4 == 0 && (uintptr_t)d_rope % 16 == 0, CN_ERR_INVALID_ARG,
+             "misaligned pointer (k and v 4 bytes, the rope table 16)");
     CN_CHECK(rope_neox == 0 || rope_neox == 1, CN_ERR_INVALID_ARG, "rope_neox is 0 or 1");
     DeviceScope ds(ctx->device);
     return kvq4_append(*cache, d_k, d_v, kv_stride, d_pos, d_count, batch, n_new,
