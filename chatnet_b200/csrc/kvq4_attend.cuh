@@ -1,0 +1,78 @@
+// kvq4_attend.cuh -- shared by the attention kernels over the 4-bit KV cache
+// (kvq4_attend.cu: few rows; kvq4_prompt.cu: many).
+#pragma once
+
+#include "kvq4.cuh"
+
+namespace cn {
+
+struct AttendArgs {
+    const float* q;
+    float* out;
+    int64_t q_stride, out_stride;
+    const int* pos;
+    const int* count;
+    const float2* rope;
+    const uint8_t *kq, *vq;
+    const __half *kd, *vd;
+    int64_t seq_rows;
+    int batch, n_new, n_heads, n_kv, ctx_len, neox, groups;
+    float scale;
+    uint32_t* err;
+};
+
+// Many rows: 128 (kvq4_prompt_rows) to a CTA, head dimensions kvq4_prompt_ok.
+int kvq4_prompt_rows();
+bool kvq4_prompt_ok(int hd);
+int kvq4_attend_prompt(cn_ctx* ctx, int hd, AttendArgs a, cudaStream_t st);
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+        "l"(src), "r"(bytes), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// D = A B + C on m16n8k16, free to be scheduled
+__device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, const float* c) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+// a b - c
+__device__ __forceinline__ uint32_t h2_fms(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("{\n\t.reg .b32 n;\n\tneg.f16x2 n, %3;\n\tfma.rn.f16x2 %0, %1, %2, n;\n\t}" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr, uint32_t rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(map_rank(addr, rank))
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_rank(addr, rank)) : "memory");
+    return v;
+}
+
+// The halves of hi + lo = x: hi keeps 11 bits (x truncated, so the
+// conversion is exact in fp16's normal range), lo the next 11.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const float2 h = make_float2(__uint_as_float(__float_as_uint(a) & 0xFFFFE000u),
+                                 __uint_as_float(__float_as_uint(b) & 0xFFFFE000u));
+    const float2 l = fma2(h, make_float2(-1.f, -1.f), make_float2(a, b));
+    hi = pack_half2(h.x, h.y);
+    lo = pack_half2(l.x, l.y);
+}
+
+}  // namespace cn

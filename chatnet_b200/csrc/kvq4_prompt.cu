@@ -1,0 +1,587 @@
+// kvq4_prompt.cu -- attention over the 4-bit KV cache for many rows (prompts):
+// the tcgen05 form of cn_kvq4_attend_dev.
+//
+// A CTA takes 128 rows (tokens x the query heads of one kv head) and walks the
+// cache in tiles of 64 positions.  Four warps expand a tile's K and V from
+// nibbles to fp16 in shared memory, one thread issues the MMAs (M = 128) into
+// tensor memory, four warps (one row per thread) turn scores into weights.
+//   S = Q K^T:  Q in tensor memory, K [64 positions][hd] as the B operand;
+//   O = P V:    P in tensor memory, V [hd][64 positions] as the B operand.
+// Precision: q, k, v and the weights are exact or 22-bit pairs of fp16 halves, three
+// MMAs each (lo hi + hi lo + hi hi; k = (level - 8) d and v are 15-bit products,
+// exact as pairs).  O is fresh for every tile and joined in fp32 registers,
+// because the tensor cores' accumulation truncates; that also leaves nothing to
+// rescale in tensor memory.  A row's reference moves only when outgrown by 2^4.
+// Bound: the MMAs, 6 x 64 columns x hd x 128 rows a tile (24 KFLOP a position and
+// row of 128), against which the exponentials and the expansion overlap: the scores of tile
+// i + 1 are computed while tile i's weights are, and tile i's output after them.
+//
+// Order of K's dimensions (any will do, if Q has the same) and V's rows (undone on
+// the way out) follow the nibbles: K position kappa of a 64-wide half is
+// (chunk g, word jj, nibble i, piece b & 1), V row n is (b & 1, i, g, jj), for value
+// 32 b + 8 i + g, b = 2 jj + (b & 1).
+#include "kvq4.cuh"
+#include "kvq4_attend.cuh"
+
+namespace cn {
+
+namespace pr {
+
+constexpr int kRows = 128, kPos = 64;
+constexpr int kThreads = 320;  // warps 0-3 rows, 4-7 expansion, 8 MMA, 9 loads
+constexpr int kRaw = 3;        // raw tiles in flight
+constexpr float kPeak = 9.f, kLazy = 4.f;
+constexpr int kMaxCluster = 8;
+
+template <int HD>
+struct Geo {
+    static constexpr int NB = HD / 32, W = NB / 2;  // blocks; 32-bit words per chunk
+    static constexpr int kTile = kPos * HD * 2;     // bytes of one fp16 K or V tile
+    static constexpr int kStage = 4 * kTile;        // K hi, K lo, V hi, V lo
+    static constexpr int kRawTile = kPos * 36 * NB;
+    static constexpr int kRawOff = 2 * kStage;
+    static constexpr int kBarOff = kRawOff + kRaw * kRawTile;
+    static constexpr int kSmem = kBarOff + 512 + 1024;
+    // tensor-memory columns: Q hi, Q lo, two S, two P (hi, lo), O
+    static constexpr int kQ = 0, kS = HD, kP = kS + 2 * kPos, kO = kP + 2 * kPos;
+    static constexpr int kCols = 512;
+    static_assert(kO + HD <= kCols, "tensor memory");
+    static_assert(kBarOff % 8 == 0 && kSmem <= 227 * 1024, "shared memory");
+};
+
+__device__ __forceinline__ void st32(uint32_t taddr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ void st16(uint32_t taddr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void ld32(uint32_t taddr, float* f) {
+    uint32_t* v = reinterpret_cast<uint32_t*>(f);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+// D (+)= A (tensor memory) x B (shared memory)^T, kind::f16, fp32 accumulation
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// A K-major operand tile: rows of 128 bytes, 16-byte pieces at piece ^ (row & 7)
+// (128-byte swizzle), 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t desc(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
+           (2ull << 61);
+}
+// D fp32, A and B fp16, K-major, N columns, M = 128
+__host__ __device__ constexpr uint32_t idesc(int n) {
+    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+}
+
+// Nibble i of both halves of x as level - 8, times d: hi + lo exactly.
+__device__ __forceinline__ void expand(uint32_t x, int i, uint32_t d, uint32_t& hi, uint32_t& lo) {
+    const uint32_t y = i >= 2 ? x >> 8 : x;
+    const uint32_t v = (i & 1) ? h2_fma(lop3_and_or(y, 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u)
+                               : h2_sub(lop3_and_or(y, 0x000F000Fu, 0x64006400u), 0x64086408u);
+    hi = h2_mul(v, d);
+    lo = h2_fms(v, d, hi);
+}
+
+}  // namespace pr
+
+template <int HD>
+__global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(const AttendArgs a) {
+    using namespace pr;
+    using G = Geo<HD>;
+    constexpr int NB = G::NB, W = G::W, RB = 16 * NB, SB = 2 * NB;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint64_t* raw_full = reinterpret_cast<uint64_t*>(smem + G::kBarOff);
+    uint64_t* raw_empty = raw_full + kRaw;
+    uint64_t* k_full = raw_empty + kRaw;  // [2]
+    uint64_t* v_full = k_full + 2;
+    uint64_t* kv_empty = v_full + 2;
+    uint64_t* s_full = kv_empty + 2;
+    uint64_t* s_empty = s_full + 2;
+    uint64_t* p_full = s_empty + 2;
+    uint64_t* o_full = p_full + 2;
+    uint64_t* o_empty = o_full + 1;
+    uint64_t* q_full = o_empty + 1;
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(q_full + 1);
+    float* undo = reinterpret_cast<float*>(tmem_holder + 2);  // [2][2] what K's and V's tiles were scaled down by
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t cs = cluster_size(), rank = cluster_rank();
+
+    // this cluster's 128 rows; the last tokens, which see most, first
+    const int item = (int)(blockIdx.x / cs);
+    const int bh = item % (a.batch * a.n_kv), grp = a.groups - 1 - item / (a.batch * a.n_kv);
+    const int kvh = bh % a.n_kv, b = bh / a.n_kv;
+    const int mul = a.n_heads / a.n_kv;
+    int p0;
+    const int n = kvq4_active(a.pos, a.count, b, a.n_new, a.ctx_len, p0);
+    const int r0 = kRows * grp, rows = min(n * mul - r0, kRows);
+    if (rows <= 0) return;  // (the whole cluster)
+    const int len = p0 + (r0 + rows - 1) / mul + 1;  // positions any of the rows sees
+    const int all = (len + kPos - 1) / kPos;
+    const int tiles = all > (int)rank ? (all - (int)rank + (int)cs - 1) / (int)cs : 0;  // rank, rank + cs, ...
+    const int64_t base = (int64_t)b * a.seq_rows + (int64_t)kvh * a.ctx_len;
+    auto first_of = [&](int i) { return ((int)rank + i * (int)cs) * kPos; };
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kRaw; s++) {
+            mbar_init(&raw_full[s], 1);
+            mbar_init(&raw_empty[s], 4);
+        }
+        for (int s = 0; s < 2; s++) {
+            mbar_init(&k_full[s], 4);
+            mbar_init(&v_full[s], 4);
+            mbar_init(&kv_empty[s], 1);
+            mbar_init(&s_full[s], 1);
+            mbar_init(&s_empty[s], 4);
+            mbar_init(&p_full[s], 4);
+        }
+        mbar_init(o_full, 1);
+        mbar_init(o_empty, 4);
+        mbar_init(q_full, 4);
+        fence_mbar_init();
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                     "r"(G::kCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_holder;
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (ok && !mbar_wait(bar, parity & 1)) {
+            ok = false;
+            atomicOr(a.err, kErrTimeout);
+        }
+    };
+
+    float o[HD];
+    float R = -1e30f, l = 0.f;
+
+    if (warp == 9) {
+        // ---- raw tiles ----
+        if (lane == 0) {
+            fence_proxy_async();
+            for (int i = 0; i < tiles && ok; i++) {
+                const int s = i % kRaw;
+                if (i >= kRaw) wait(&raw_empty[s], (uint32_t)(i / kRaw - 1));
+                if (!ok) break;
+                const int first = first_of(i);
+                const int64_t row = base + first;
+                const int np = min(kPos, (len - first + 7) & ~7);  // (ctx_len is a multiple of 8)
+                uint8_t* d = smem + G::kRawOff + s * G::kRawTile;
+                mbar_expect_tx(&raw_full[s], (uint32_t)(np * 36 * NB));
+                bulk_load(d, a.kq + row * RB, np * RB, &raw_full[s]);
+                bulk_load(d + kPos * RB, a.vq + row * RB, np * RB, &raw_full[s]);
+                bulk_load(d + 2 * kPos * RB, a.kd + row * NB, np * SB, &raw_full[s]);
+                bulk_load(d + 2 * kPos * RB + kPos * SB, a.vd + row * NB, np * SB, &raw_full[s]);
+            }
+        }
+    } else if (warp == 8) {
+        // ---- MMAs: S(0), then S(i + 1) and O(i) ----
+        if (lane == 0 && tiles > 0) {
+            constexpr uint32_t kS = idesc(kPos), kO = idesc(HD);
+            wait(q_full, 0);
+            auto scores = [&](int i) {
+                const int s = i & 1;
+                const uint32_t ph = (uint32_t)(i >> 1);
+                wait(&k_full[s], ph);
+                if (i >= 2) wait(&s_empty[s], ph - 1);
+                if (!ok) return;
+                fence_after();
+                const uint32_t kt = smem_u32(smem + s * G::kStage), d = tmem + G::kS + s * kPos;
+                auto at = [&](int kk) { return kt + (kk / 4) * (kPos * 128) + 32 * (kk % 4); };
+#pragma unroll
+                for (int kk = 0; kk < HD / 16; kk++) {
+                    mma_ts(d, tmem + G::kQ + HD / 2 + 8 * kk, desc(at(kk)), kS, kk != 0);
+                    mma_ts(d, tmem + G::kQ + 8 * kk, desc(at(kk) + G::kTile), kS, 1u);
+                }
+#pragma unroll
+                for (int kk = 0; kk < HD / 16; kk++) mma_ts(d, tmem + G::kQ + 8 * kk, desc(at(kk)), kS, 1u);
+                commit(&s_full[s]);
+            };
+            scores(0);
+            for (int i = 0; i < tiles && ok; i++) {
+                if (i + 1 < tiles) scores(i + 1);
+                const int s = i & 1;
+                wait(&v_full[s], (uint32_t)(i >> 1));
+                wait(&p_full[s], (uint32_t)(i >> 1));
+                if (i > 0) wait(o_empty, (uint32_t)(i - 1));
+                if (!ok) break;
+                fence_after();
+                const uint32_t vt = smem_u32(smem + s * G::kStage + 2 * G::kTile), d = tmem + G::kO;
+                const uint32_t ph = tmem + G::kP + s * kPos, pl = ph + kPos / 2;
+#pragma unroll
+                for (int kk = 0; kk < kPos / 16; kk++) {
+                    mma_ts(d, pl + 8 * kk, desc(vt + 32 * kk), kO, kk != 0);
+                    mma_ts(d, ph + 8 * kk, desc(vt + G::kTile + 32 * kk), kO, 1u);
+                }
+#pragma unroll
+                for (int kk = 0; kk < kPos / 16; kk++) mma_ts(d, ph + 8 * kk, desc(vt + 32 * kk), kO, 1u);
+                commit(o_full);
+                commit(&kv_empty[s]);
+            }
+        }
+    } else if (warp >= 4) {
+        // ---- expansion ----
+        const int tid = threadIdx.x - 128;
+        for (int i = 0; i < tiles; i++) {
+            const int rs = i % kRaw, s = i & 1, first = first_of(i);
+            const uint8_t* raw = smem + G::kRawOff + rs * G::kRawTile;
+            wait(&raw_full[rs], (uint32_t)(i / kRaw));
+            if (i >= 2) wait(&kv_empty[s], (uint32_t)((i >> 1) - 1));
+            uint8_t* stage = smem + s * G::kStage;
+            // scales from 2^12 on would take fp16 products past its range: such a
+            // tile counts 2^-4 times
+            uint32_t shrink[2];
+#pragma unroll
+            for (int kv = 0; kv < 2; kv++) {
+                uint32_t mx = 0;
+                for (int e = lane; e < kPos * NB / 2; e += 32) {
+                    uint32_t v = reinterpret_cast<const uint32_t*>(raw + 2 * kPos * RB + kv * kPos * SB)[e];
+                    if (first + e / (NB / 2) >= len) v = 0;
+                    mx = __vmaxu2(mx, v & 0x7FFF7FFFu);
+                }
+                const bool big = __any_sync(0xffffffffu, max(mx & 0xFFFFu, mx >> 16) >= 0x6C00u);
+                shrink[kv] = big ? 0x2C002C00u : 0x3C003C00u;
+                if (tid == 0) undo[2 * s + kv] = big ? 16.f : 1.f;
+            }
+            {  // K: position p, chunks 4 hf .. + 3 (each W 16-byte pieces)
+                const int p = tid & 63, hf = tid >> 6;
+                const bool in = first + p < len;
+                const uint32_t* q = reinterpret_cast<const uint32_t*>(raw + p * RB + hf * (RB / 2));
+                const uint32_t* sc = reinterpret_cast<const uint32_t*>(raw + 2 * kPos * RB + p * SB);
+                uint32_t d[W];
+#pragma unroll
+                for (int j = 0; j < W; j++) d[j] = in ? h2_mul(sc[j], shrink[0]) : 0u;
+                uint32_t w[4 * W];
+#pragma unroll
+                for (int j = 0; j < W; j++) {
+                    const uint4 u = reinterpret_cast<const uint4*>(q)[j];
+                    w[4 * j] = u.x, w[4 * j + 1] = u.y, w[4 * j + 2] = u.z, w[4 * j + 3] = u.w;
+                }
+#pragma unroll
+                for (int c = 0; c < 4 * W; c++) {  // piece c of this half: chunk c / W, word c % W
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) expand(w[c], e, d[c % W], hi[e], lo[e]);
+                    const int k16 = hf * 4 * W + c;  // 16-byte piece of the row, 8 to a 64-wide part
+                    uint8_t* t = stage + (k16 >> 3) * (kPos * 128) + p * 128 + (((k16 & 7) ^ (p & 7)) << 4);
+                    *reinterpret_cast<uint4*>(t) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4*>(t + G::kTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&k_full[s]);
+            {  // V: eight positions 8 k .. + 7, word (g, jj); with one word a chunk, nibbles in two halves
+                const int gw = tid & (8 * W - 1), k = (tid / (8 * W)) & 7;
+                constexpr int NI = 2 * W;  // nibbles a thread takes
+                const int i0 = W == 2 ? 0 : (tid >> 6) * 2;
+                const int jj = gw % W;
+                const uint8_t* q = raw + kPos * RB + 8 * k * RB + 4 * gw;
+                const uint8_t* sc = raw + 2 * kPos * RB + kPos * SB + 8 * k * SB + 4 * jj;
+                uint32_t hi[2][NI][4], lo[2][NI][4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const uint32_t w0 = *reinterpret_cast<const uint32_t*>(q + 2 * u * RB);
+                    const uint32_t w1 = *reinterpret_cast<const uint32_t*>(q + (2 * u + 1) * RB);
+                    uint32_t d0 = *reinterpret_cast<const uint32_t*>(sc + 2 * u * SB);
+                    uint32_t d1 = *reinterpret_cast<const uint32_t*>(sc + (2 * u + 1) * SB);
+                    if (first + 8 * k + 2 * u >= len) d0 = 0;  // (rows past the end hold anything)
+                    if (first + 8 * k + 2 * u + 1 >= len) d1 = 0;
+#pragma unroll
+                    for (int pb = 0; pb < 2; pb++) {
+                        const uint32_t x = __byte_perm(w0, w1, pb ? 0x7632u : 0x5410u);
+                        const uint32_t d = h2_mul(__byte_perm(d0, d1, pb ? 0x7632u : 0x5410u), shrink[1]);
+#pragma unroll
+                        for (int e = 0; e < NI; e++) {
+                            if constexpr (W == 2) {
+                                expand(x, e, d, hi[pb][e][u], lo[pb][e][u]);
+                            } else {
+                                if (i0 == 0) expand(x, e, d, hi[pb][e][u], lo[pb][e][u]);
+                                else expand(x, e + 2, d, hi[pb][e][u], lo[pb][e][u]);
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int pb = 0; pb < 2; pb++)
+#pragma unroll
+                    for (int e = 0; e < NI; e++) {
+                        const int row = (pb * 4 + i0 + e) * (8 * W) + gw;
+                        uint8_t* t = stage + 2 * G::kTile + row * 128 + ((k ^ (row & 7)) << 4);
+                        *reinterpret_cast<uint4*>(t) = make_uint4(hi[pb][e][0], hi[pb][e][1], hi[pb][e][2], hi[pb][e][3]);
+                        *reinterpret_cast<uint4*>(t + G::kTile) =
+                            make_uint4(lo[pb][e][0], lo[pb][e][1], lo[pb][e][2], lo[pb][e][3]);
+                    }
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&v_full[s]);
+                mbar_arrive(&raw_empty[rs]);
+            }
+        }
+    } else {
+        // ---- rows: one per thread ----
+        const int r = threadIdx.x;
+        const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+        const int rr = r0 + min(r, rows - 1), tok = rr / mul;
+        const int limit = p0 + tok;
+        float factor;
+        {
+            // the row's query, rotated, scaled to [2^14, 2^15), in K's order
+            const float* x = a.q + ((int64_t)b * a.n_new + tok) * a.q_stride + (int64_t)(kvh * mul + rr % mul) * HD;
+            float amax = 0.f;
+#pragma unroll
+            for (int e = 0; e < HD / 4; e++) {
+                const float4 v = reinterpret_cast<const float4*>(x)[e];
+                o[4 * e] = v.x, o[4 * e + 1] = v.y, o[4 * e + 2] = v.z, o[4 * e + 3] = v.w;
+            }
+            if (a.rope) {
+                const float2* tab = a.rope + (int64_t)limit * (HD / 2);
+                auto turn = [](float& u, float& v, float2 t) {
+                    const float u1 = __fsub_rn(__fmul_rn(u, t.x), __fmul_rn(v, t.y));
+                    v = __fadd_rn(__fmul_rn(u, t.y), __fmul_rn(v, t.x));
+                    u = u1;
+                };
+                if (a.neox) {
+#pragma unroll
+                    for (int e = 0; e < HD / 2; e++) turn(o[e], o[e + HD / 2], tab[e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < HD / 2; e++) turn(o[2 * e], o[2 * e + 1], tab[e]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < HD; e++) amax = fmaxf(amax, fabsf(o[e]));
+            float sc, inv;
+            row_pow2_scale(amax, sc, inv);
+            factor = a.scale * 1.44269504088896341f * inv;
+#pragma unroll
+            for (int part = 0; part < HD / 64; part++) {
+                uint32_t hi[32], lo[32];
+#pragma unroll
+                for (int m = 0; m < 32; m++) {
+                    const int k16 = part * 8 + m / 4, g = k16 / W, jj = k16 % W, i = m % 4;
+                    const int e = 64 * jj + 8 * i + g;  // and the next block's
+                    split2(o[e] * sc, o[e + 32] * sc, hi[m], lo[m]);
+                }
+                st32(tmem + lane_off + G::kQ + 32 * part, hi);
+                st32(tmem + lane_off + G::kQ + HD / 2 + 32 * part, lo);
+            }
+            wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+        }
+#pragma unroll
+        for (int e = 0; e < HD; e++) o[e] = 0.f;
+        const int seen_by_all = p0 + r0 / mul + 1;
+        float al = 1.f, vmul = 1.f;  // of the tile whose output is still to be joined
+        auto join = [&](int i) {  // tile i's output; everything so far times al
+            wait(o_full, (uint32_t)i);
+            fence_after();
+            const bool same = __all_sync(0xffffffffu, al == 1.f && vmul == 1.f);
+#pragma unroll
+            for (int c = 0; c < HD / 32; c++) {
+                float t[32];
+                ld32(tmem + lane_off + G::kO + 32 * c, t);
+                wait_ld();
+                if (same) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const float2 v = add2(make_float2(o[32 * c + e], o[32 * c + e + 1]), make_float2(t[e], t[e + 1]));
+                        o[32 * c + e] = v.x, o[32 * c + e + 1] = v.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[32 * c + e] = al * fmaf(t[e], vmul, o[32 * c + e]);
+                }
+            }
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_empty);
+        };
+        for (int i = 0; i < tiles; i++) {
+            const int s = i & 1, first = first_of(i);
+            wait(&s_full[s], (uint32_t)(i >> 1));
+            fence_after();
+            const float f = factor * undo[2 * s];
+            const float vm = undo[2 * s + 1];
+            const bool hide = first + kPos > seen_by_all;
+            float move = 1.f, top, sum;
+            for (int again = 0;; again++) {
+                top = -INFINITY;
+                sum = 0.f;
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    float x[32];
+                    ld32(tmem + lane_off + G::kS + s * kPos + 32 * c, x);
+                    wait_ld();
+                    if (hide) {
+#pragma unroll
+                        for (int e = 0; e < 32; e++)
+                            if (first + 32 * c + e > limit) x[e] = -INFINITY;
+                    }
+                    uint32_t hi[16], lo[16];
+                    float2 part = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        top = fmaxf(top, fmaxf(x[e], x[e + 1]));
+                        const float2 y = fma2(make_float2(x[e], x[e + 1]), make_float2(f, f), make_float2(-R, -R));
+                        const float2 p = make_float2(ex2(y.x), ex2(y.y));
+                        part = add2(part, p);
+                        split2(p.x, p.y, hi[e / 2], lo[e / 2]);
+                    }
+                    sum += part.x + part.y;
+                    st16(tmem + lane_off + G::kP + s * kPos + 16 * c, hi);
+                    st16(tmem + lane_off + G::kP + s * kPos + kPos / 2 + 16 * c, lo);
+                }
+                const bool out = top * f > R + (kPeak + kLazy);
+                if (again || !__any_sync(0xffffffffu, out)) break;
+                wait_st();
+                if (out) {  // the weights again, from a reference that fits
+                    const float to = top * f - kPeak;
+                    move = ex2(R - to);
+                    R = to;
+                }
+            }
+            l = l * move + sum;
+            wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&s_empty[s]);
+                mbar_arrive(&p_full[s]);
+            }
+            if (i > 0) {
+                al = move;
+                join(i - 1);
+            }
+            vmul = vm;
+        }
+        al = 1.f;
+        if (tiles > 0) join(tiles - 1);
+        if (cs == 1 && r < rows) {
+            float* dst = a.out + ((int64_t)b * a.n_new + tok) * a.out_stride + (int64_t)(kvh * mul + rr % mul) * HD;
+            const float inv = 1.f / l;
+#pragma unroll
+            for (int m = 0; m < HD / 4; m++) {
+                float v[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const int e = 4 * m + u, bl = e / 32, i = (e / 8) % 4, g = e % 8;
+                    v[u] = o[((bl & 1) * 4 + i) * (8 * W) + g * W + (bl >> 1)] * inv;
+                }
+                *reinterpret_cast<float4*>(dst + 4 * m) = make_float4(v[0], v[1], v[2], v[3]);
+            }
+        }
+    }
+    // every MMA is done (its output was waited for) and every copy landed
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 8)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::kCols) : "memory");
+    if (cs > 1) {
+        // the cluster's partials: each CTA leaves its rows in its own shared
+        // memory (in the place of its first K and V tiles), then adds up a share
+        float* mine = reinterpret_cast<float*>(smem);  // [HD][128]
+        float* mR = mine + HD * kRows;
+        float* mL = mR + kRows;
+        if (warp < 4) {
+#pragma unroll
+            for (int e = 0; e < HD; e++) mine[e * kRows + threadIdx.x] = o[e];
+            mR[threadIdx.x] = R;
+            mL[threadIdx.x] = l;
+        }
+        __syncthreads();
+        cluster_arrive();
+        cluster_wait();
+        const uint32_t aO = smem_u32(mine), aR = smem_u32(mR), aL = smem_u32(mL);
+        for (int e = (int)rank * kThreads + threadIdx.x; e < HD * kRows; e += (int)cs * kThreads) {
+            const int r = e % kRows, nn = e / kRows;
+            if (r >= rows) continue;
+            float M = -1e30f, v = 0.f, ls = 0.f;
+            for (uint32_t c = 0; c < cs; c++) M = fmaxf(M, ld_cluster(aR + 4 * r, c));
+            for (uint32_t c = 0; c < cs; c++) {
+                const float f = ex2(ld_cluster(aR + 4 * r, c) - M);
+                v = fmaf(f, ld_cluster(aO + 4 * e, c), v);
+                ls = fmaf(f, ld_cluster(aL + 4 * r, c), ls);
+            }
+            const int hb = nn / (8 * W), lw = nn % (8 * W);
+            const int dim = 32 * (2 * (lw % W) + hb / 4) + 8 * (hb % 4) + lw / W;
+            const int rr = r0 + r;
+            a.out[((int64_t)b * a.n_new + rr / mul) * a.out_stride + (int64_t)(kvh * mul + rr % mul) * HD + dim] = v / ls;
+        }
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+    }
+}
+
+int kvq4_prompt_rows() { return pr::kRows; }
+
+bool kvq4_prompt_ok(int hd) { return hd == 64 || hd == 128; }
+
+int kvq4_attend_prompt(cn_ctx* ctx, int hd, AttendArgs a, cudaStream_t st) {
+    using namespace pr;
+    const int64_t rows = (int64_t)a.n_new * (a.n_heads / a.n_kv), groups = (rows + kRows - 1) / kRows;
+    const int64_t items = groups * a.n_kv * a.batch;
+    CN_CHECK(items < (1ll << 31) / kMaxCluster, CN_ERR_INVALID_ARG, "too many rows (%lld items)", (long long)items);
+    a.groups = (int)groups;
+    // CTAs per item: as many as the SMs hold (one each), four tiles for each at least
+    int cluster = 1;
+    while (cluster < kMaxCluster && 2 * cluster * items <= ctx->sms && 2 * cluster * 4 * kPos <= a.ctx_len) cluster *= 2;
+    using Fn = void (*)(AttendArgs);
+    const Fn fn = hd == 64 ? (Fn)kvq4_attend_prompt_kernel<64> : (Fn)kvq4_attend_prompt_kernel<128>;
+    const int smem = hd == 64 ? Geo<64>::kSmem : Geo<128>::kSmem;
+    const uint32_t bit = 1u << (hd == 64 ? 24 : 25);
+    if (!(__atomic_load_n(&ctx->kvq4_ready, __ATOMIC_RELAXED) & bit)) {
+        CN_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        __atomic_fetch_or(&ctx->kvq4_ready, bit, __ATOMIC_RELAXED);
+    }
+    CN_CUDA(launch_cluster_k(false, cluster, fn, dim3((unsigned)(items * cluster)), dim3(kThreads), (size_t)smem, st, a));
+    return CN_OK;
+}
+
+}  // namespace cn
