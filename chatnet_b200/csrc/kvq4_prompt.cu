@@ -28,7 +28,7 @@ namespace cn {
 namespace pr {
 
 constexpr int kRows = 128, kPos = 64;
-constexpr int kThreads = 320;  // warps 0-3 rows, 4-7 expansion, 8 MMA, 9 loads
+constexpr int kThreads = 640;  // warps 0-3 weights, 4-7 output, 8-11 K, 12-15 V, 16 S, 17 loads, 18 O (19 fills the group)
 constexpr int kRaw = 3;        // raw tiles in flight
 constexpr float kPeak = 9.f, kLazy = 4.f;
 constexpr int kMaxCluster = 8;
@@ -37,28 +37,21 @@ template <int HD>
 struct Geo {
     static constexpr int NB = HD / 32, W = NB / 2;  // blocks; 32-bit words per chunk
     static constexpr int kTile = kPos * HD * 2;     // bytes of one fp16 K or V tile
-    static constexpr int kStage = 4 * kTile;        // K hi, K lo, V hi, V lo
+    static constexpr int kStage = 4 * kTile;        // K (hi, lo of each 64-wide part), V hi, V lo
     static constexpr int kRawTile = kPos * 36 * NB;
     static constexpr int kRawOff = 2 * kStage;
     static constexpr int kBarOff = kRawOff + kRaw * kRawTile;
-    static constexpr int kSmem = kBarOff + 512 + 1024;
-    // tensor-memory columns: Q hi, Q lo, two S, two P (hi, lo), O
-    static constexpr int kQ = 0, kS = HD, kP = kS + 2 * kPos, kO = kP + 2 * kPos;
+    static constexpr int kRowOff = kBarOff + 512;  // per row: four rescalings, the last reference and sum
+    static constexpr int kSmem = kRowOff + kRows * (4 * 4 + 8) + 1024;
+    // tensor-memory columns: Q hi, Q lo; two of S (64 columns of Q Khi, 64 of Qhi
+    // Klo; the weights, 32 columns of halves and 32 of low halves, in the second
+    // half's place); O
+    static constexpr int kQ = 0, kS = HD, kO = kS + 4 * kPos;
     static constexpr int kCols = 512;
     static_assert(kO + HD <= kCols, "tensor memory");
     static_assert(kBarOff % 8 == 0 && kSmem <= 227 * 1024, "shared memory");
 };
 
-__device__ __forceinline__ void st32(uint32_t taddr, const uint32_t* v) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-        : "memory");
-}
 __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t* v) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
@@ -66,6 +59,11 @@ __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t* v) {
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
         "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
+}
+__device__ __forceinline__ void st8(uint32_t taddr, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
 }
 __device__ __forceinline__ void ld32(uint32_t taddr, float* f) {
     uint32_t* v = reinterpret_cast<uint32_t*>(f);
@@ -76,6 +74,16 @@ __device__ __forceinline__ void ld32(uint32_t taddr, float* f) {
           "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
           "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
           "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void ld16(uint32_t taddr, float* f) {
+    uint32_t* v = reinterpret_cast<uint32_t*>(f);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
         : "r"(taddr)
         : "memory");
 }
@@ -129,15 +137,22 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
     uint64_t* raw_empty = raw_full + kRaw;
     uint64_t* k_full = raw_empty + kRaw;  // [2]
     uint64_t* v_full = k_full + 2;
-    uint64_t* kv_empty = v_full + 2;
-    uint64_t* s_full = kv_empty + 2;
-    uint64_t* s_empty = s_full + 2;
-    uint64_t* p_full = s_empty + 2;
-    uint64_t* o_full = p_full + 2;
+    uint64_t* k_empty = v_full + 2;
+    uint64_t* v_empty = k_empty + 2;
+    uint64_t* s_full = v_empty + 2;
+    uint64_t* p_full = s_full + 2;
+    uint64_t* p_empty = p_full + 2;
+    uint64_t* al_full = p_empty + 2;  // [4]
+    uint64_t* o_full = al_full + 4;
     uint64_t* o_empty = o_full + 1;
     uint64_t* q_full = o_empty + 1;
-    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(q_full + 1);
-    float* undo = reinterpret_cast<float*>(tmem_holder + 2);  // [2][2] what K's and V's tiles were scaled down by
+    uint64_t* l_full = q_full + 1;
+    uint64_t* u_full = l_full + 1;  // [2][8]
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(u_full + 16);
+    float* undo = reinterpret_cast<float*>(tmem_holder + 2);  // [2][8] what K's and V's tiles were scaled down by
+    float* slots = reinterpret_cast<float*>(smem + G::kRowOff);    // [4][128] what a tile multiplies the row's output by
+    float* mR = reinterpret_cast<float*>(slots + 4 * kRows);       // [128] references
+    float* mL = mR + kRows;                                        // [128] sums of weights
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t cs = cluster_size(), rank = cluster_rank();
 
@@ -159,22 +174,26 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
     if (threadIdx.x == 0) {
         for (int s = 0; s < kRaw; s++) {
             mbar_init(&raw_full[s], 1);
-            mbar_init(&raw_empty[s], 4);
+            mbar_init(&raw_empty[s], 8);
         }
         for (int s = 0; s < 2; s++) {
             mbar_init(&k_full[s], 4);
             mbar_init(&v_full[s], 4);
-            mbar_init(&kv_empty[s], 1);
+            mbar_init(&k_empty[s], 1);
+            mbar_init(&v_empty[s], 1);
             mbar_init(&s_full[s], 1);
-            mbar_init(&s_empty[s], 4);
             mbar_init(&p_full[s], 4);
+            mbar_init(&p_empty[s], 1);
         }
+        for (int s = 0; s < 4; s++) mbar_init(&al_full[s], 4);
+        for (int s = 0; s < 16; s++) mbar_init(&u_full[s], 1);
+        mbar_init(l_full, 4);
         mbar_init(o_full, 1);
         mbar_init(o_empty, 4);
         mbar_init(q_full, 4);
         fence_mbar_init();
     }
-    if (warp == 8) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
                      "r"(G::kCols)
                      : "memory");
@@ -192,10 +211,15 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
         }
     };
 
-    float o[HD];
-    float R = -1e30f, l = 0.f;
+    // the cluster's partials: each CTA leaves its rows in its own shared memory, in
+    // the place of its first K and V tiles, once its last output is there
+    float* mine = reinterpret_cast<float*>(smem);  // [HD][128]
 
-    if (warp == 9) {
+    // Registers: 96 a thread at launch (480 for the five groups of four warps);
+    // 112 + 184 + 64 + 80 + 32 = 472 once the last three have given theirs up.
+    if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+    if (warp == 17) {
         // ---- raw tiles ----
         if (lane == 0) {
             fence_proxy_async();
@@ -214,327 +238,366 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                 bulk_load(d + 2 * kPos * RB + kPos * SB, a.vd + row * NB, np * SB, &raw_full[s]);
             }
         }
-    } else if (warp == 8) {
-        // ---- MMAs: S(0), then S(i + 1) and O(i) ----
-        if (lane == 0 && tiles > 0) {
-            constexpr uint32_t kS = idesc(kPos), kO = idesc(HD);
-            wait(q_full, 0);
-            auto scores = [&](int i) {
-                const int s = i & 1;
-                const uint32_t ph = (uint32_t)(i >> 1);
-                wait(&k_full[s], ph);
-                if (i >= 2) wait(&s_empty[s], ph - 1);
-                if (!ok) return;
-                fence_after();
-                const uint32_t kt = smem_u32(smem + s * G::kStage), d = tmem + G::kS + s * kPos;
-                auto at = [&](int kk) { return kt + (kk / 4) * (kPos * 128) + 32 * (kk % 4); };
-#pragma unroll
-                for (int kk = 0; kk < HD / 16; kk++) {
-                    mma_ts(d, tmem + G::kQ + HD / 2 + 8 * kk, desc(at(kk)), kS, kk != 0);
-                    mma_ts(d, tmem + G::kQ + 8 * kk, desc(at(kk) + G::kTile), kS, 1u);
-                }
-#pragma unroll
-                for (int kk = 0; kk < HD / 16; kk++) mma_ts(d, tmem + G::kQ + 8 * kk, desc(at(kk)), kS, 1u);
-                commit(&s_full[s]);
-            };
-            scores(0);
+    } else if (warp == 16) {
+        // ---- S.  (The MMA loops stay rolled: their issue, not the tensor cores,
+        // is what a thread of straight-line code would be bound by.) ----
+        if (lane == 0) {
+            constexpr uint32_t kS1 = idesc(kPos), kS2 = idesc(2 * kPos);
+            if (tiles > 0) wait(q_full, 0);
             for (int i = 0; i < tiles && ok; i++) {
-                if (i + 1 < tiles) scores(i + 1);
+                const int s = i & 1;
+                wait(&k_full[s], (uint32_t)(i >> 1));
+                if (i >= 2) wait(&p_empty[s], (uint32_t)((i >> 1) - 1));  // tile i - 2's weights lie there
+                if (!ok) break;
+                fence_after();
+                const uint64_t kt = desc(smem_u32(smem + s * G::kStage));
+                const uint32_t d = tmem + G::kS + s * 2 * kPos, q = tmem + G::kQ;
+                // Qlo Khi (and once Qlo Klo, which starts the second half), then Qhi [Khi | Klo]
+                mma_ts(d, q + HD / 2, kt, kS2, 0u);
+#pragma unroll 1
+                for (int part = 0; part < HD / 64; part++) {
+                    const uint64_t b = kt + part * (2 * kPos * 128 / 16);
+#pragma unroll 1
+                    for (int kk = part ? 0 : 1; kk < 4; kk++)
+                        mma_ts(d, q + HD / 2 + 32 * part + 8 * kk, b + 2 * kk, kS1, 1u);
+                }
+#pragma unroll 1
+                for (int part = 0; part < HD / 64; part++) {
+                    const uint64_t b = kt + part * (2 * kPos * 128 / 16);
+#pragma unroll 1
+                    for (int kk = 0; kk < 4; kk++) mma_ts(d, q + 32 * part + 8 * kk, b + 2 * kk, kS2, 1u);
+                }
+                commit(&s_full[s]);
+                commit(&k_empty[s]);
+            }
+        }
+    } else if (warp == 18) {
+        // ---- O ----
+        if (lane == 0) {
+            constexpr uint32_t kO = idesc(HD);
+            for (int i = 0; i < tiles && ok; i++) {
                 const int s = i & 1;
                 wait(&v_full[s], (uint32_t)(i >> 1));
                 wait(&p_full[s], (uint32_t)(i >> 1));
                 if (i > 0) wait(o_empty, (uint32_t)(i - 1));
                 if (!ok) break;
                 fence_after();
-                const uint32_t vt = smem_u32(smem + s * G::kStage + 2 * G::kTile), d = tmem + G::kO;
-                const uint32_t ph = tmem + G::kP + s * kPos, pl = ph + kPos / 2;
-#pragma unroll
+                const uint64_t vt = desc(smem_u32(smem + s * G::kStage + 2 * G::kTile));
+                const uint32_t d = tmem + G::kO, ph = tmem + G::kS + s * 2 * kPos + kPos, pl = ph + kPos / 2;
+#pragma unroll 1
                 for (int kk = 0; kk < kPos / 16; kk++) {
-                    mma_ts(d, pl + 8 * kk, desc(vt + 32 * kk), kO, kk != 0);
-                    mma_ts(d, ph + 8 * kk, desc(vt + G::kTile + 32 * kk), kO, 1u);
+                    mma_ts(d, pl + 8 * kk, vt + 2 * kk, kO, kk != 0);
+                    mma_ts(d, ph + 8 * kk, vt + G::kTile / 16 + 2 * kk, kO, 1u);
                 }
-#pragma unroll
-                for (int kk = 0; kk < kPos / 16; kk++) mma_ts(d, ph + 8 * kk, desc(vt + 32 * kk), kO, 1u);
+#pragma unroll 1
+                for (int kk = 0; kk < kPos / 16; kk++) mma_ts(d, ph + 8 * kk, vt + 2 * kk, kO, 1u);
                 commit(o_full);
-                commit(&kv_empty[s]);
+                commit(&v_empty[s]);
+                commit(&p_empty[s]);
             }
         }
-    } else if (warp >= 4) {
-        // ---- expansion ----
-        const int tid = threadIdx.x - 128;
-        for (int i = 0; i < tiles; i++) {
-            const int rs = i % kRaw, s = i & 1, first = first_of(i);
-            const uint8_t* raw = smem + G::kRawOff + rs * G::kRawTile;
-            wait(&raw_full[rs], (uint32_t)(i / kRaw));
-            if (i >= 2) wait(&kv_empty[s], (uint32_t)((i >> 1) - 1));
-            uint8_t* stage = smem + s * G::kStage;
-            // scales from 2^12 on would take fp16 products past its range: such a
-            // tile counts 2^-4 times
-            uint32_t shrink[2];
-#pragma unroll
-            for (int kv = 0; kv < 2; kv++) {
-                uint32_t mx = 0;
-                for (int e = lane; e < kPos * NB / 2; e += 32) {
-                    uint32_t v = reinterpret_cast<const uint32_t*>(raw + 2 * kPos * RB + kv * kPos * SB)[e];
-                    if (first + e / (NB / 2) >= len) v = 0;
-                    mx = __vmaxu2(mx, v & 0x7FFF7FFFu);
-                }
-                const bool big = __any_sync(0xffffffffu, max(mx & 0xFFFFu, mx >> 16) >= 0x6C00u);
-                shrink[kv] = big ? 0x2C002C00u : 0x3C003C00u;
-                if (tid == 0) undo[2 * s + kv] = big ? 16.f : 1.f;
+    }
+    } else if (warp >= 8) {
+        // ---- expansion: K by warps 8-11, V by 12-15 ----
+        const int tid = threadIdx.x & 127;
+        const int kv = warp >= 12;
+        // scales from 2^12 on would take fp16 products past its range: a tile that
+        // has one counts 2^-4 times
+        auto shrink_of = [&](const uint8_t* raw, int i) {
+            uint32_t mx = 0;
+            for (int e = lane; e < kPos * NB / 2; e += 32) {
+                uint32_t v = reinterpret_cast<const uint32_t*>(raw + 2 * kPos * RB + kv * kPos * SB)[e];
+                if (first_of(i) + e / (NB / 2) >= len) v = 0;
+                mx = __vmaxu2(mx, v & 0x7FFF7FFFu);
             }
-            {  // K: position p, chunks 4 hf .. + 3 (each W 16-byte pieces)
-                const int p = tid & 63, hf = tid >> 6;
-                const bool in = first + p < len;
-                const uint32_t* q = reinterpret_cast<const uint32_t*>(raw + p * RB + hf * (RB / 2));
+            const bool big = __any_sync(0xffffffffu, max(mx & 0xFFFFu, mx >> 16) >= 0x6C00u);
+            if (tid == 0) {
+                undo[8 * kv + (i & 7)] = big ? 16.f : 1.f;
+                mbar_arrive(&u_full[8 * kv + (i & 7)]);
+            }
+            return big ? 0x2C002C00u : 0x3C003C00u;
+        };
+        if (!kv) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+            // position p, chunks 4 hf .. + 3 (each W 16-byte pieces)
+            const int p = tid & 63, hf = tid >> 6;
+            for (int i = 0; i < tiles; i++) {
+                const int rs = i % kRaw, s = i & 1;
+                const uint8_t* raw = smem + G::kRawOff + rs * G::kRawTile;
+                wait(&raw_full[rs], (uint32_t)(i / kRaw));
+                const uint32_t shrink = shrink_of(raw, i);
+                const bool in = first_of(i) + p < len;
                 const uint32_t* sc = reinterpret_cast<const uint32_t*>(raw + 2 * kPos * RB + p * SB);
-                uint32_t d[W];
-#pragma unroll
-                for (int j = 0; j < W; j++) d[j] = in ? h2_mul(sc[j], shrink[0]) : 0u;
-                uint32_t w[4 * W];
+                uint32_t d[W], w[4 * W];
 #pragma unroll
                 for (int j = 0; j < W; j++) {
-                    const uint4 u = reinterpret_cast<const uint4*>(q)[j];
+                    d[j] = in ? h2_mul(sc[j], shrink) : 0u;
+                    const uint4 u = reinterpret_cast<const uint4*>(raw + p * RB + hf * (RB / 2))[j];
                     w[4 * j] = u.x, w[4 * j + 1] = u.y, w[4 * j + 2] = u.z, w[4 * j + 3] = u.w;
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&raw_empty[rs]);
+                if (i >= 2) wait(&k_empty[s], (uint32_t)((i >> 1) - 1));
+                uint8_t* stage = smem + s * G::kStage + p * 128;
 #pragma unroll
                 for (int c = 0; c < 4 * W; c++) {  // piece c of this half: chunk c / W, word c % W
                     uint32_t hi[4], lo[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) expand(w[c], e, d[c % W], hi[e], lo[e]);
                     const int k16 = hf * 4 * W + c;  // 16-byte piece of the row, 8 to a 64-wide part
-                    uint8_t* t = stage + (k16 >> 3) * (kPos * 128) + p * 128 + (((k16 & 7) ^ (p & 7)) << 4);
+                    uint8_t* t = stage + (k16 >> 3) * (2 * kPos * 128) + (((k16 & 7) ^ (p & 7)) << 4);
                     *reinterpret_cast<uint4*>(t) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    *reinterpret_cast<uint4*>(t + G::kTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    *reinterpret_cast<uint4*>(t + kPos * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&k_full[s]);
             }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&k_full[s]);
-            {  // V: eight positions 8 k .. + 7, word (g, jj); with one word a chunk, nibbles in two halves
-                const int gw = tid & (8 * W - 1), k = (tid / (8 * W)) & 7;
-                constexpr int NI = 2 * W;  // nibbles a thread takes
-                const int i0 = W == 2 ? 0 : (tid >> 6) * 2;
-                const int jj = gw % W;
+        } else {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+            // eight positions 8 k .. + 7, word gw = (g, jj); with one word a chunk,
+            // nibbles in two halves
+            const int gw = tid & (8 * W - 1), k = (tid / (8 * W)) & 7;
+            constexpr int NI = 2 * W;  // nibbles a thread takes
+            const int i0 = W == 2 ? 0 : (tid >> 6) * 2;
+            for (int i = 0; i < tiles; i++) {
+                const int rs = i % kRaw, s = i & 1, first = first_of(i) + 8 * k;
+                const uint8_t* raw = smem + G::kRawOff + rs * G::kRawTile;
+                wait(&raw_full[rs], (uint32_t)(i / kRaw));
+                const uint32_t shrink = shrink_of(raw, i);
                 const uint8_t* q = raw + kPos * RB + 8 * k * RB + 4 * gw;
-                const uint8_t* sc = raw + 2 * kPos * RB + kPos * SB + 8 * k * SB + 4 * jj;
-                uint32_t hi[2][NI][4], lo[2][NI][4];
+                const uint8_t* sc = raw + 2 * kPos * RB + kPos * SB + 8 * k * SB + 4 * (gw % W);
+                uint32_t w[8], d[8];
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const uint32_t w0 = *reinterpret_cast<const uint32_t*>(q + 2 * u * RB);
-                    const uint32_t w1 = *reinterpret_cast<const uint32_t*>(q + (2 * u + 1) * RB);
-                    uint32_t d0 = *reinterpret_cast<const uint32_t*>(sc + 2 * u * SB);
-                    uint32_t d1 = *reinterpret_cast<const uint32_t*>(sc + (2 * u + 1) * SB);
-                    if (first + 8 * k + 2 * u >= len) d0 = 0;  // (rows past the end hold anything)
-                    if (first + 8 * k + 2 * u + 1 >= len) d1 = 0;
-#pragma unroll
-                    for (int pb = 0; pb < 2; pb++) {
-                        const uint32_t x = __byte_perm(w0, w1, pb ? 0x7632u : 0x5410u);
-                        const uint32_t d = h2_mul(__byte_perm(d0, d1, pb ? 0x7632u : 0x5410u), shrink[1]);
-#pragma unroll
-                        for (int e = 0; e < NI; e++) {
-                            if constexpr (W == 2) {
-                                expand(x, e, d, hi[pb][e][u], lo[pb][e][u]);
-                            } else {
-                                if (i0 == 0) expand(x, e, d, hi[pb][e][u], lo[pb][e][u]);
-                                else expand(x, e + 2, d, hi[pb][e][u], lo[pb][e][u]);
-                            }
-                        }
-                    }
+                for (int u = 0; u < 8; u++) {
+                    w[u] = *reinterpret_cast<const uint32_t*>(q + u * RB);
+                    d[u] = *reinterpret_cast<const uint32_t*>(sc + u * SB);
+                    d[u] = first + u < len ? h2_mul(d[u], shrink) : 0u;  // (rows past the end hold anything)
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&raw_empty[rs]);
+                if (i >= 2) wait(&v_empty[s], (uint32_t)((i >> 1) - 1));
+                uint8_t* stage = smem + s * G::kStage + 2 * G::kTile;
 #pragma unroll
                 for (int pb = 0; pb < 2; pb++)
 #pragma unroll
                     for (int e = 0; e < NI; e++) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            uint32_t x = __byte_perm(w[2 * u], w[2 * u + 1], pb ? 0x7632u : 0x5410u);
+                            const uint32_t dd = __byte_perm(d[2 * u], d[2 * u + 1], pb ? 0x7632u : 0x5410u);
+                            if (W == 1 && i0) x >>= 8;  // nibbles 2, 3
+                            expand(x, e, dd, hi[u], lo[u]);
+                        }
                         const int row = (pb * 4 + i0 + e) * (8 * W) + gw;
-                        uint8_t* t = stage + 2 * G::kTile + row * 128 + ((k ^ (row & 7)) << 4);
-                        *reinterpret_cast<uint4*>(t) = make_uint4(hi[pb][e][0], hi[pb][e][1], hi[pb][e][2], hi[pb][e][3]);
-                        *reinterpret_cast<uint4*>(t + G::kTile) =
-                            make_uint4(lo[pb][e][0], lo[pb][e][1], lo[pb][e][2], lo[pb][e][3]);
+                        uint8_t* t = stage + row * 128 + ((k ^ (row & 7)) << 4);
+                        *reinterpret_cast<uint4*>(t) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4*>(t + G::kTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     }
-            }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&v_full[s]);
-                mbar_arrive(&raw_empty[rs]);
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&v_full[s]);
             }
         }
     } else {
-        // ---- rows: one per thread ----
-        const int r = threadIdx.x;
-        const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+        const int r = threadIdx.x & (kRows - 1);  // this thread's row
+        const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
         const int rr = r0 + min(r, rows - 1), tok = rr / mul;
-        const int limit = p0 + tok;
-        float factor;
-        {
-            // the row's query, rotated, scaled to [2^14, 2^15), in K's order
-            const float* x = a.q + ((int64_t)b * a.n_new + tok) * a.q_stride + (int64_t)(kvh * mul + rr % mul) * HD;
-            float amax = 0.f;
+        if (warp >= 4) {
+            // ---- output ----
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+            float o[HD];
+            {
+                // first the row's query: rotated, scaled to [2^14, 2^15), in K's order
+                const float* x = a.q + ((int64_t)b * a.n_new + tok) * a.q_stride + (int64_t)(kvh * mul + rr % mul) * HD;
 #pragma unroll
-            for (int e = 0; e < HD / 4; e++) {
-                const float4 v = reinterpret_cast<const float4*>(x)[e];
-                o[4 * e] = v.x, o[4 * e + 1] = v.y, o[4 * e + 2] = v.z, o[4 * e + 3] = v.w;
-            }
-            if (a.rope) {
-                const float2* tab = a.rope + (int64_t)limit * (HD / 2);
-                auto turn = [](float& u, float& v, float2 t) {
-                    const float u1 = __fsub_rn(__fmul_rn(u, t.x), __fmul_rn(v, t.y));
-                    v = __fadd_rn(__fmul_rn(u, t.y), __fmul_rn(v, t.x));
-                    u = u1;
-                };
-                if (a.neox) {
-#pragma unroll
-                    for (int e = 0; e < HD / 2; e++) turn(o[e], o[e + HD / 2], tab[e]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < HD / 2; e++) turn(o[2 * e], o[2 * e + 1], tab[e]);
+                for (int e = 0; e < HD / 4; e++) {
+                    const float4 v = reinterpret_cast<const float4*>(x)[e];
+                    o[4 * e] = v.x, o[4 * e + 1] = v.y, o[4 * e + 2] = v.z, o[4 * e + 3] = v.w;
                 }
-            }
+                if (a.rope) {
+                    const float4* tab = reinterpret_cast<const float4*>(a.rope + (int64_t)(p0 + tok) * (HD / 2));
+                    auto turn = [](float& u, float& v, float c, float s) {
+                        const float t = __fsub_rn(__fmul_rn(u, c), __fmul_rn(v, s));
+                        v = __fadd_rn(__fmul_rn(u, s), __fmul_rn(v, c));
+                        u = t;
+                    };
+                    if (a.neox) {
 #pragma unroll
-            for (int e = 0; e < HD; e++) amax = fmaxf(amax, fabsf(o[e]));
-            float sc, inv;
-            row_pow2_scale(amax, sc, inv);
-            factor = a.scale * 1.44269504088896341f * inv;
+                        for (int e = 0; e < HD / 2; e += 2) {
+                            const float4 t = tab[e / 2];
+                            turn(o[e], o[e + HD / 2], t.x, t.y);
+                            turn(o[e + 1], o[e + 1 + HD / 2], t.z, t.w);
+                        }
+                    } else {
 #pragma unroll
-            for (int part = 0; part < HD / 64; part++) {
-                uint32_t hi[32], lo[32];
-#pragma unroll
-                for (int m = 0; m < 32; m++) {
-                    const int k16 = part * 8 + m / 4, g = k16 / W, jj = k16 % W, i = m % 4;
-                    const int e = 64 * jj + 8 * i + g;  // and the next block's
-                    split2(o[e] * sc, o[e + 32] * sc, hi[m], lo[m]);
-                }
-                st32(tmem + lane_off + G::kQ + 32 * part, hi);
-                st32(tmem + lane_off + G::kQ + HD / 2 + 32 * part, lo);
-            }
-            wait_st();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_full);
-        }
-#pragma unroll
-        for (int e = 0; e < HD; e++) o[e] = 0.f;
-        const int seen_by_all = p0 + r0 / mul + 1;
-        float al = 1.f, vmul = 1.f;  // of the tile whose output is still to be joined
-        auto join = [&](int i) {  // tile i's output; everything so far times al
-            wait(o_full, (uint32_t)i);
-            fence_after();
-            const bool same = __all_sync(0xffffffffu, al == 1.f && vmul == 1.f);
-#pragma unroll
-            for (int c = 0; c < HD / 32; c++) {
-                float t[32];
-                ld32(tmem + lane_off + G::kO + 32 * c, t);
-                wait_ld();
-                if (same) {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        const float2 v = add2(make_float2(o[32 * c + e], o[32 * c + e + 1]), make_float2(t[e], t[e + 1]));
-                        o[32 * c + e] = v.x, o[32 * c + e + 1] = v.y;
+                        for (int e = 0; e < HD / 2; e += 2) {
+                            const float4 t = tab[e / 2];
+                            turn(o[2 * e], o[2 * e + 1], t.x, t.y);
+                            turn(o[2 * e + 2], o[2 * e + 3], t.z, t.w);
+                        }
                     }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; e++) o[32 * c + e] = al * fmaf(t[e], vmul, o[32 * c + e]);
                 }
-            }
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(o_empty);
-        };
-        for (int i = 0; i < tiles; i++) {
-            const int s = i & 1, first = first_of(i);
-            wait(&s_full[s], (uint32_t)(i >> 1));
-            fence_after();
-            const float f = factor * undo[2 * s];
-            const float vm = undo[2 * s + 1];
-            const bool hide = first + kPos > seen_by_all;
-            float move = 1.f, top, sum;
-            for (int again = 0;; again++) {
-                top = -INFINITY;
-                sum = 0.f;
+                float amax = 0.f, sc, inv;
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    float x[32];
-                    ld32(tmem + lane_off + G::kS + s * kPos + 32 * c, x);
-                    wait_ld();
-                    if (hide) {
+                for (int e = 0; e < HD; e++) amax = fmaxf(amax, fabsf(o[e]));
+                row_pow2_scale(amax, sc, inv);
+                mR[r] = a.scale * 1.44269504088896341f * inv;  // (what a score counts, for the weights' warps)
 #pragma unroll
-                        for (int e = 0; e < 32; e++)
-                            if (first + 32 * c + e > limit) x[e] = -INFINITY;
-                    }
+                for (int part = 0; part < HD / 32; part++) {
                     uint32_t hi[16], lo[16];
-                    float2 part = make_float2(0.f, 0.f);
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        top = fmaxf(top, fmaxf(x[e], x[e + 1]));
-                        const float2 y = fma2(make_float2(x[e], x[e + 1]), make_float2(f, f), make_float2(-R, -R));
-                        const float2 p = make_float2(ex2(y.x), ex2(y.y));
-                        part = add2(part, p);
-                        split2(p.x, p.y, hi[e / 2], lo[e / 2]);
+                    for (int m = 0; m < 16; m++) {
+                        const int k16 = part * 4 + m / 4, g = k16 / W, jj = k16 % W, i = m % 4;
+                        const int e = 64 * jj + 8 * i + g;  // and the next block's
+                        split2(o[e] * sc, o[e + 32] * sc, hi[m], lo[m]);
                     }
-                    sum += part.x + part.y;
-                    st16(tmem + lane_off + G::kP + s * kPos + 16 * c, hi);
-                    st16(tmem + lane_off + G::kP + s * kPos + kPos / 2 + 16 * c, lo);
+                    st16(tmem + lane_off + G::kQ + 16 * part, hi);
+                    st16(tmem + lane_off + G::kQ + HD / 2 + 16 * part, lo);
                 }
-                const bool out = top * f > R + (kPeak + kLazy);
-                if (again || !__any_sync(0xffffffffu, out)) break;
                 wait_st();
-                if (out) {  // the weights again, from a reference that fits
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_full);
+            }
+#pragma unroll
+            for (int e = 0; e < HD; e++) o[e] = 0.f;
+            for (int i = 0; i < tiles; i++) {
+                wait(&al_full[i & 3], (uint32_t)(i >> 2));
+                const float am = slots[(i & 3) * kRows + r];
+                if (!__all_sync(0xffffffffu, am == 1.f)) {
+#pragma unroll
+                    for (int e = 0; e < HD; e++) o[e] *= am;
+                }
+                wait(o_full, (uint32_t)i);
+                wait(&u_full[8 + (i & 7)], (uint32_t)(i >> 3));
+                const float vm = undo[8 + (i & 7)];
+                fence_after();
+                float t[2][16];
+                ld16(tmem + lane_off + G::kO, t[0]);
+#pragma unroll
+                for (int c = 0; c < HD / 16; c++) {
+                    wait_ld();
+                    if (c + 1 < HD / 16) ld16(tmem + lane_off + G::kO + 16 * (c + 1), t[(c + 1) & 1]);
+                    else {
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(o_empty);
+                    }
+                    const float* x = t[c & 1];
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const float2 v = fma2(make_float2(x[e], x[e + 1]), make_float2(vm, vm),
+                                              make_float2(o[16 * c + e], o[16 * c + e + 1]));
+                        o[16 * c + e] = v.x, o[16 * c + e + 1] = v.y;
+                    }
+                }
+            }
+            if (cs > 1) {
+#pragma unroll
+                for (int e = 0; e < HD; e++) mine[e * kRows + r] = o[e];
+            } else {
+                wait(l_full, 0);
+                if (r < rows) {
+                    float* dst =
+                        a.out + ((int64_t)b * a.n_new + tok) * a.out_stride + (int64_t)(kvh * mul + rr % mul) * HD;
+                    const float inv = 1.f / mL[r];
+#pragma unroll
+                    for (int m = 0; m < HD / 4; m++) {
+                        float v[4];
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            const int e = 4 * m + u, bl = e / 32, i = (e / 8) % 4, g = e % 8;
+                            v[u] = o[((bl & 1) * 4 + i) * (8 * W) + g * W + (bl >> 1)] * inv;
+                        }
+                        *reinterpret_cast<float4*>(dst + 4 * m) = make_float4(v[0], v[1], v[2], v[3]);
+                    }
+                }
+            }
+        } else {
+            // ---- weights ----
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+            float R = -1e30f, l = 0.f;
+            const int limit = p0 + tok;
+            wait(q_full, 0);
+            const float factor = mR[r];
+            const int seen_by_all = p0 + r0 / mul + 1;
+            for (int i = 0; i < tiles; i++) {
+                const int s = i & 1, first = first_of(i);
+                wait(&u_full[i & 7], (uint32_t)(i >> 3));
+                const float f = factor * undo[i & 7];
+                wait(&s_full[s], (uint32_t)(i >> 1));
+                fence_after();
+                const uint32_t sc = tmem + lane_off + G::kS + s * 2 * kPos;
+                float x[64];
+                ld32(sc, x);
+                ld32(sc + 32, x + 32);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    float y[16];
+                    ld16(sc + kPos + 16 * c, y);
+                    wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const float2 v =
+                            add2(make_float2(x[16 * c + e], x[16 * c + e + 1]), make_float2(y[e], y[e + 1]));
+                        x[16 * c + e] = v.x, x[16 * c + e + 1] = v.y;
+                    }
+                }
+                if (first + kPos > seen_by_all) {
+#pragma unroll
+                    for (int e = 0; e < 64; e++)
+                        if (first + e > limit) x[e] = -INFINITY;
+                }
+                float top = x[0], move = 1.f;
+#pragma unroll
+                for (int e = 1; e < 64; e++) top = fmaxf(top, x[e]);
+                if (top * f > R + (kPeak + kLazy)) {
                     const float to = top * f - kPeak;
                     move = ex2(R - to);
                     R = to;
                 }
-            }
-            l = l * move + sum;
-            wait_st();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&s_empty[s]);
-                mbar_arrive(&p_full[s]);
-            }
-            if (i > 0) {
-                al = move;
-                join(i - 1);
-            }
-            vmul = vm;
-        }
-        al = 1.f;
-        if (tiles > 0) join(tiles - 1);
-        if (cs == 1 && r < rows) {
-            float* dst = a.out + ((int64_t)b * a.n_new + tok) * a.out_stride + (int64_t)(kvh * mul + rr % mul) * HD;
-            const float inv = 1.f / l;
+                float2 part = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int m = 0; m < HD / 4; m++) {
-                float v[4];
+                for (int c = 0; c < 4; c++) {
+                    uint32_t hi[8], lo[8];
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const int e = 4 * m + u, bl = e / 32, i = (e / 8) % 4, g = e % 8;
-                    v[u] = o[((bl & 1) * 4 + i) * (8 * W) + g * W + (bl >> 1)] * inv;
+                    for (int e = 0; e < 16; e += 2) {
+                        const float2 y =
+                            fma2(make_float2(x[16 * c + e], x[16 * c + e + 1]), make_float2(f, f), make_float2(-R, -R));
+                        const float2 w = make_float2(ex2(y.x), ex2(y.y));
+                        part = add2(part, w);
+                        split2(w.x, w.y, hi[e / 2], lo[e / 2]);
+                    }
+                    st8(sc + kPos + 8 * c, hi);
+                    st8(sc + kPos + kPos / 2 + 8 * c, lo);
                 }
-                *reinterpret_cast<float4*>(dst + 4 * m) = make_float4(v[0], v[1], v[2], v[3]);
+                const float sum = part.x + part.y;
+                l = l * move + sum;
+                slots[(i & 3) * kRows + r] = move;
+                wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&p_full[s]);
+                    mbar_arrive(&al_full[i & 3]);
+                }
             }
+            mR[r] = R;
+            mL[r] = l;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(l_full);
         }
     }
     // every MMA is done (its output was waited for) and every copy landed
     fence_before();
     __syncthreads();
     fence_after();
-    if (warp == 8)
+    if (warp == 16)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::kCols) : "memory");
     if (cs > 1) {
-        // the cluster's partials: each CTA leaves its rows in its own shared
-        // memory (in the place of its first K and V tiles), then adds up a share
-        float* mine = reinterpret_cast<float*>(smem);  // [HD][128]
-        float* mR = mine + HD * kRows;
-        float* mL = mR + kRows;
-        if (warp < 4) {
-#pragma unroll
-            for (int e = 0; e < HD; e++) mine[e * kRows + threadIdx.x] = o[e];
-            mR[threadIdx.x] = R;
-            mL[threadIdx.x] = l;
-        }
-        __syncthreads();
+        // the partials meet, each CTA adding up a share
         cluster_arrive();
         cluster_wait();
         const uint32_t aO = smem_u32(mine), aR = smem_u32(mR), aL = smem_u32(mL);
