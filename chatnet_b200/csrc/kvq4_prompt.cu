@@ -44,8 +44,8 @@ struct Geo {
     static constexpr int kRowOff = kBarOff + 512;  // per row: four rescalings, the last reference and sum
     static constexpr int kSmem = kRowOff + kRows * (4 * 4 + 8) + 1024;
     // tensor-memory columns: Q hi, Q lo; two of S (64 columns of Q Khi, 64 of Qhi
-    // Klo; the weights, 32 columns of halves and 32 of low halves, in the second
-    // half's place); O
+    // Klo; the weights in the second half's place, for 16 positions 8 columns of
+    // halves and 8 of low halves); O
     static constexpr int kQ = 0, kS = HD, kO = kS + 4 * kPos;
     static constexpr int kCols = 512;
     static_assert(kO + HD <= kCols, "tensor memory");
@@ -283,14 +283,14 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                 if (!ok) break;
                 fence_after();
                 const uint64_t vt = desc(smem_u32(smem + s * G::kStage + 2 * G::kTile));
-                const uint32_t d = tmem + G::kO, ph = tmem + G::kS + s * 2 * kPos + kPos, pl = ph + kPos / 2;
+                const uint32_t d = tmem + G::kO, p = tmem + G::kS + s * 2 * kPos + kPos;
 #pragma unroll 1
                 for (int kk = 0; kk < kPos / 16; kk++) {
-                    mma_ts(d, pl + 8 * kk, vt + 2 * kk, kO, kk != 0);
-                    mma_ts(d, ph + 8 * kk, vt + G::kTile / 16 + 2 * kk, kO, 1u);
+                    mma_ts(d, p + 16 * kk + 8, vt + 2 * kk, kO, kk != 0);
+                    mma_ts(d, p + 16 * kk, vt + G::kTile / 16 + 2 * kk, kO, 1u);
                 }
 #pragma unroll 1
-                for (int kk = 0; kk < kPos / 16; kk++) mma_ts(d, ph + 8 * kk, vt + 2 * kk, kO, 1u);
+                for (int kk = 0; kk < kPos / 16; kk++) mma_ts(d, p + 16 * kk, vt + 2 * kk, kO, 1u);
                 commit(o_full);
                 commit(&v_empty[s]);
                 commit(&p_empty[s]);
@@ -328,30 +328,32 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                 const uint32_t shrink = shrink_of(raw, i);
                 const bool in = first_of(i) + p < len;
                 const uint32_t* sc = reinterpret_cast<const uint32_t*>(raw + 2 * kPos * RB + p * SB);
-                uint32_t d[W], w[4 * W];
+                uint32_t d[W];
 #pragma unroll
-                for (int j = 0; j < W; j++) {
-                    d[j] = in ? h2_mul(sc[j], shrink) : 0u;
-                    const uint4 u = reinterpret_cast<const uint4*>(raw + p * RB + hf * (RB / 2))[j];
-                    w[4 * j] = u.x, w[4 * j + 1] = u.y, w[4 * j + 2] = u.z, w[4 * j + 3] = u.w;
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&raw_empty[rs]);
+                for (int j = 0; j < W; j++) d[j] = in ? h2_mul(sc[j], shrink) : 0u;
                 if (i >= 2) wait(&k_empty[s], (uint32_t)((i >> 1) - 1));
                 uint8_t* stage = smem + s * G::kStage + p * 128;
+#pragma unroll 1
+                for (int j = 0; j < W; j++) {
+                    const uint4 u = reinterpret_cast<const uint4*>(raw + p * RB + hf * (RB / 2))[j];
+                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-                for (int c = 0; c < 4 * W; c++) {  // piece c of this half: chunk c / W, word c % W
-                    uint32_t hi[4], lo[4];
+                    for (int c = 0; c < 4; c++) {  // word c % W of chunk (4 j + c) / W of this half
+                        uint32_t hi[4], lo[4];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) expand(w[c], e, d[c % W], hi[e], lo[e]);
-                    const int k16 = hf * 4 * W + c;  // 16-byte piece of the row, 8 to a 64-wide part
-                    uint8_t* t = stage + (k16 >> 3) * (2 * kPos * 128) + (((k16 & 7) ^ (p & 7)) << 4);
-                    *reinterpret_cast<uint4*>(t) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    *reinterpret_cast<uint4*>(t + kPos * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        for (int e = 0; e < 4; e++) expand(w[c], e, d[c % W], hi[e], lo[e]);
+                        const int k16 = hf * 4 * W + 4 * j + c;  // 16-byte piece of the row, 8 to a 64-wide part
+                        uint8_t* t = stage + (k16 >> 3) * (2 * kPos * 128) + (((k16 & 7) ^ (p & 7)) << 4);
+                        *reinterpret_cast<uint4*>(t) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4*>(t + kPos * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
                 }
                 fence_proxy_async();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&k_full[s]);
+                if (lane == 0) {
+                    mbar_arrive(&k_full[s]);
+                    mbar_arrive(&raw_empty[rs]);
+                }
             }
         } else {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
@@ -378,7 +380,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                 if (lane == 0) mbar_arrive(&raw_empty[rs]);
                 if (i >= 2) wait(&v_empty[s], (uint32_t)((i >> 1) - 1));
                 uint8_t* stage = smem + s * G::kStage + 2 * G::kTile;
-#pragma unroll
+#pragma unroll 1
                 for (int pb = 0; pb < 2; pb++)
 #pragma unroll
                     for (int e = 0; e < NI; e++) {
@@ -530,48 +532,52 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                 wait(&s_full[s], (uint32_t)(i >> 1));
                 fence_after();
                 const uint32_t sc = tmem + lane_off + G::kS + s * 2 * kPos;
-                float x[64];
-                ld32(sc, x);
-                ld32(sc + 32, x + 32);
-#pragma unroll
+                const bool hide = first + kPos > seen_by_all;
+                float top = -INFINITY, move = 1.f;
+#pragma unroll 1
                 for (int c = 0; c < 4; c++) {
-                    float y[16];
+                    float x[16], y[16];
+                    ld16(sc + 16 * c, x);
                     ld16(sc + kPos + 16 * c, y);
                     wait_ld();
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
-                        const float2 v =
-                            add2(make_float2(x[16 * c + e], x[16 * c + e + 1]), make_float2(y[e], y[e + 1]));
-                        x[16 * c + e] = v.x, x[16 * c + e + 1] = v.y;
+                        float2 v = add2(make_float2(x[e], x[e + 1]), make_float2(y[e], y[e + 1]));
+                        if (hide) {
+                            if (first + 16 * c + e > limit) v.x = -INFINITY;
+                            if (first + 16 * c + e + 1 > limit) v.y = -INFINITY;
+                        }
+                        top = fmaxf(top, fmaxf(v.x, v.y));
                     }
                 }
-                if (first + kPos > seen_by_all) {
-#pragma unroll
-                    for (int e = 0; e < 64; e++)
-                        if (first + e > limit) x[e] = -INFINITY;
-                }
-                float top = x[0], move = 1.f;
-#pragma unroll
-                for (int e = 1; e < 64; e++) top = fmaxf(top, x[e]);
                 if (top * f > R + (kPeak + kLazy)) {
                     const float to = top * f - kPeak;
                     move = ex2(R - to);
                     R = to;
                 }
+                // 16 scores at a time: their sums, weights, and the halves in the place of
+                // the second summands (8 columns of halves, 8 of low halves)
                 float2 part = make_float2(0.f, 0.f);
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < 4; c++) {
-                    uint32_t hi[8], lo[8];
+                    float x[16], y[16];
+                    ld16(sc + 16 * c, x);
+                    ld16(sc + kPos + 16 * c, y);
+                    wait_ld();
+                    uint32_t w[16];
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
-                        const float2 y =
-                            fma2(make_float2(x[16 * c + e], x[16 * c + e + 1]), make_float2(f, f), make_float2(-R, -R));
-                        const float2 w = make_float2(ex2(y.x), ex2(y.y));
-                        part = add2(part, w);
-                        split2(w.x, w.y, hi[e / 2], lo[e / 2]);
+                        float2 v = add2(make_float2(x[e], x[e + 1]), make_float2(y[e], y[e + 1]));
+                        if (hide) {
+                            if (first + 16 * c + e > limit) v.x = -INFINITY;
+                            if (first + 16 * c + e + 1 > limit) v.y = -INFINITY;
+                        }
+                        v = fma2(v, make_float2(f, f), make_float2(-R, -R));
+                        v = make_float2(ex2(v.x), ex2(v.y));
+                        part = add2(part, v);
+                        split2(v.x, v.y, w[e / 2], w[8 + e / 2]);
                     }
-                    st8(sc + kPos + 8 * c, hi);
-                    st8(sc + kPos + kPos / 2 + 8 * c, lo);
+                    st16(sc + kPos + 16 * c, w);
                 }
                 const float sum = part.x + part.y;
                 l = l * move + sum;
