@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
     int s = 0;
     uint32_t parity = 0;
     for (int tile = tile0; tile < tiles; tile += step) {
-        if (ok && !mbar_wait(&full[warp][s], parity)) {
+        if (ok && !bar_wait(&full[warp][s], parity)) {
             ok = false;
             if (lane == 0) atomicOr(a.err, kErrTimeout);
         }

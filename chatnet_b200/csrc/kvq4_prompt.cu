@@ -30,6 +30,7 @@ namespace pr {
 constexpr int kRows = 128, kPos = 64;
 constexpr int kThreads = 640;  // warps 0-3 weights, 4-7 output, 8-11 K, 12-15 V, 16 S, 17 loads, 18 O (19 fills the group)
 constexpr int kRaw = 3;        // raw tiles in flight
+constexpr int kBufs = 3;       // tiles between their scores and their output
 constexpr float kPeak = 9.f, kLazy = 4.f;
 constexpr int kMaxCluster = 8;
 
@@ -39,14 +40,15 @@ struct Geo {
     static constexpr int kTile = kPos * HD * 2;     // bytes of one fp16 K or V tile
     static constexpr int kStage = 4 * kTile;        // K (hi, lo of each 64-wide part), V hi, V lo
     static constexpr int kRawTile = kPos * 36 * NB;
-    static constexpr int kRawOff = 2 * kStage;
+    static constexpr int kQOff = 2 * kStage;        // Q: hi and lo of each 64-wide part, 128 rows of 128 bytes
+    static constexpr int kRawOff = kQOff + 2 * HD * kRows * 2;
     static constexpr int kBarOff = kRawOff + kRaw * kRawTile;
     static constexpr int kRowOff = kBarOff + 512;  // per row: four rescalings, the last reference and sum
     static constexpr int kSmem = kRowOff + kRows * (4 * 4 + 8) + 1024;
-    // tensor-memory columns: Q hi, Q lo; two of S (64 columns of Q Khi, 64 of Qhi
-    // Klo; the weights in the second half's place, for 16 positions 8 columns of
-    // halves and 8 of low halves); O
-    static constexpr int kQ = 0, kS = HD, kO = kS + 4 * kPos;
+    // tensor-memory columns: kBufs of S (64 columns of Q Khi, 64 of Qhi Klo; the
+    // weights in the second half's place, for 16 positions 8 columns of halves and
+    // 8 of low halves); O
+    static constexpr int kS = 0, kO = kBufs * 2 * kPos;
     static constexpr int kCols = 512;
     static_assert(kO + HD <= kCols, "tensor memory");
     static_assert(kBarOff % 8 == 0 && kSmem <= 227 * 1024, "shared memory");
@@ -104,6 +106,15 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
         "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// both operands from shared memory
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
 // A K-major operand tile: rows of 128 bytes, 16-byte pieces at piece ^ (row & 7)
 // (128-byte swizzle), 8-row groups 1024 bytes apart.
 __device__ __forceinline__ uint64_t desc(uint32_t addr) {
@@ -140,9 +151,9 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
     uint64_t* k_empty = v_full + 2;
     uint64_t* v_empty = k_empty + 2;
     uint64_t* s_full = v_empty + 2;
-    uint64_t* p_full = s_full + 2;
-    uint64_t* p_empty = p_full + 2;
-    uint64_t* al_full = p_empty + 2;  // [4]
+    uint64_t* p_full = s_full + kBufs;
+    uint64_t* p_empty = p_full + kBufs;
+    uint64_t* al_full = p_empty + kBufs;  // [4]
     uint64_t* o_full = al_full + 4;
     uint64_t* o_empty = o_full + 1;
     uint64_t* q_full = o_empty + 1;
@@ -181,6 +192,8 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
             mbar_init(&v_full[s], 4);
             mbar_init(&k_empty[s], 1);
             mbar_init(&v_empty[s], 1);
+        }
+        for (int s = 0; s < kBufs; s++) {
             mbar_init(&s_full[s], 1);
             mbar_init(&p_full[s], 4);
             mbar_init(&p_empty[s], 1);
@@ -205,7 +218,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
     const uint32_t tmem = *tmem_holder;
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (ok && !mbar_wait(bar, parity & 1)) {
+        if (ok && !bar_wait(bar, parity & 1)) {
             ok = false;
             atomicOr(a.err, kErrTimeout);
         }
@@ -247,27 +260,27 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
             for (int i = 0; i < tiles && ok; i++) {
                 const int s = i & 1;
                 wait(&k_full[s], (uint32_t)(i >> 1));
-                if (i >= 2) wait(&p_empty[s], (uint32_t)((i >> 1) - 1));  // tile i - 2's weights lie there
+                const int buf = i % kBufs;
+                if (i >= kBufs) wait(&p_empty[buf], (uint32_t)(i / kBufs - 1));  // tile i - 3's weights lie there
                 if (!ok) break;
                 fence_after();
-                const uint64_t kt = desc(smem_u32(smem + s * G::kStage));
-                const uint32_t d = tmem + G::kS + s * 2 * kPos, q = tmem + G::kQ;
+                const uint64_t kt = desc(smem_u32(smem + s * G::kStage)), q = desc(smem_u32(smem + G::kQOff));
+                const uint32_t d = tmem + G::kS + buf * 2 * kPos;
                 // Qlo Khi (and once Qlo Klo, which starts the second half), then Qhi [Khi | Klo]
-                mma_ts(d, q + HD / 2, kt, kS2, 0u);
+                mma_ss(d, q + kRows * 128 / 16, kt, kS2, 0u);
 #pragma unroll 1
                 for (int part = 0; part < HD / 64; part++) {
-                    const uint64_t b = kt + part * (2 * kPos * 128 / 16);
+                    const uint64_t b = kt + part * (2 * kPos * 128 / 16), a = q + (2 * part + 1) * (kRows * 128 / 16);
 #pragma unroll 1
-                    for (int kk = part ? 0 : 1; kk < 4; kk++)
-                        mma_ts(d, q + HD / 2 + 32 * part + 8 * kk, b + 2 * kk, kS1, 1u);
+                    for (int kk = part ? 0 : 1; kk < 4; kk++) mma_ss(d, a + 2 * kk, b + 2 * kk, kS1, 1u);
                 }
 #pragma unroll 1
                 for (int part = 0; part < HD / 64; part++) {
-                    const uint64_t b = kt + part * (2 * kPos * 128 / 16);
+                    const uint64_t b = kt + part * (2 * kPos * 128 / 16), a = q + 2 * part * (kRows * 128 / 16);
 #pragma unroll 1
-                    for (int kk = 0; kk < 4; kk++) mma_ts(d, q + 32 * part + 8 * kk, b + 2 * kk, kS2, 1u);
+                    for (int kk = 0; kk < 4; kk++) mma_ss(d, a + 2 * kk, b + 2 * kk, kS2, 1u);
                 }
-                commit(&s_full[s]);
+                commit(&s_full[buf]);
                 commit(&k_empty[s]);
             }
         }
@@ -277,13 +290,14 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
             constexpr uint32_t kO = idesc(HD);
             for (int i = 0; i < tiles && ok; i++) {
                 const int s = i & 1;
+                const int buf = i % kBufs;
                 wait(&v_full[s], (uint32_t)(i >> 1));
-                wait(&p_full[s], (uint32_t)(i >> 1));
+                wait(&p_full[buf], (uint32_t)(i / kBufs));
                 if (i > 0) wait(o_empty, (uint32_t)(i - 1));
                 if (!ok) break;
                 fence_after();
                 const uint64_t vt = desc(smem_u32(smem + s * G::kStage + 2 * G::kTile));
-                const uint32_t d = tmem + G::kO, p = tmem + G::kS + s * 2 * kPos + kPos;
+                const uint32_t d = tmem + G::kO, p = tmem + G::kS + buf * 2 * kPos + kPos;
 #pragma unroll 1
                 for (int kk = 0; kk < kPos / 16; kk++) {
                     mma_ts(d, p + 16 * kk + 8, vt + 2 * kk, kO, kk != 0);
@@ -293,7 +307,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                 for (int kk = 0; kk < kPos / 16; kk++) mma_ts(d, p + 16 * kk, vt + 2 * kk, kO, 1u);
                 commit(o_full);
                 commit(&v_empty[s]);
-                commit(&p_empty[s]);
+                commit(&p_empty[buf]);
             }
         }
     }
@@ -447,19 +461,19 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                 row_pow2_scale(amax, sc, inv);
                 mR[r] = a.scale * 1.44269504088896341f * inv;  // (what a score counts, for the weights' warps)
 #pragma unroll
-                for (int part = 0; part < HD / 32; part++) {
-                    uint32_t hi[16], lo[16];
+                for (int k16 = 0; k16 < HD / 8; k16++) {
+                    uint32_t hi[4], lo[4];
+                    const int g = k16 / W, jj = k16 % W;
 #pragma unroll
-                    for (int m = 0; m < 16; m++) {
-                        const int k16 = part * 4 + m / 4, g = k16 / W, jj = k16 % W, i = m % 4;
+                    for (int i = 0; i < 4; i++) {
                         const int e = 64 * jj + 8 * i + g;  // and the next block's
-                        split2(o[e] * sc, o[e + 32] * sc, hi[m], lo[m]);
+                        split2(o[e] * sc, o[e + 32] * sc, hi[i], lo[i]);
                     }
-                    st16(tmem + lane_off + G::kQ + 16 * part, hi);
-                    st16(tmem + lane_off + G::kQ + HD / 2 + 16 * part, lo);
+                    uint8_t* t = smem + G::kQOff + (k16 / 8) * (2 * kRows * 128) + r * 128 + (((k16 & 7) ^ (r & 7)) << 4);
+                    *reinterpret_cast<uint4*>(t) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4*>(t + kRows * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
-                wait_st();
-                fence_before();
+                fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_full);
             }
@@ -526,30 +540,35 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
             const float factor = mR[r];
             const int seen_by_all = p0 + r0 / mul + 1;
             for (int i = 0; i < tiles; i++) {
-                const int s = i & 1, first = first_of(i);
+                const int buf = i % kBufs, first = first_of(i);
                 wait(&u_full[i & 7], (uint32_t)(i >> 3));
                 const float f = factor * undo[i & 7];
-                wait(&s_full[s], (uint32_t)(i >> 1));
+                wait(&s_full[buf], (uint32_t)(i / kBufs));
                 fence_after();
-                const uint32_t sc = tmem + lane_off + G::kS + s * 2 * kPos;
+                const uint32_t sc = tmem + lane_off + G::kS + buf * 2 * kPos;
                 const bool hide = first + kPos > seen_by_all;
-                float top = -INFINITY, move = 1.f;
-#pragma unroll 1
+                float x[64], top = -INFINITY, move = 1.f;
+                ld32(sc, x);
+                ld32(sc + 32, x + 32);
+#pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    float x[16], y[16];
-                    ld16(sc + 16 * c, x);
+                    float y[16];
                     ld16(sc + kPos + 16 * c, y);
                     wait_ld();
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
-                        float2 v = add2(make_float2(x[e], x[e + 1]), make_float2(y[e], y[e + 1]));
-                        if (hide) {
-                            if (first + 16 * c + e > limit) v.x = -INFINITY;
-                            if (first + 16 * c + e + 1 > limit) v.y = -INFINITY;
-                        }
-                        top = fmaxf(top, fmaxf(v.x, v.y));
+                        const float2 v =
+                            add2(make_float2(x[16 * c + e], x[16 * c + e + 1]), make_float2(y[e], y[e + 1]));
+                        x[16 * c + e] = v.x, x[16 * c + e + 1] = v.y;
                     }
                 }
+                if (hide) {
+#pragma unroll
+                    for (int e = 0; e < 64; e++)
+                        if (first + e > limit) x[e] = -INFINITY;
+                }
+#pragma unroll
+                for (int e = 0; e < 64; e++) top = fmaxf(top, x[e]);
                 if (top * f > R + (kPeak + kLazy)) {
                     const float to = top * f - kPeak;
                     move = ex2(R - to);
@@ -558,21 +577,12 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                 // 16 scores at a time: their sums, weights, and the halves in the place of
                 // the second summands (8 columns of halves, 8 of low halves)
                 float2 part = make_float2(0.f, 0.f);
-#pragma unroll 1
+#pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    float x[16], y[16];
-                    ld16(sc + 16 * c, x);
-                    ld16(sc + kPos + 16 * c, y);
-                    wait_ld();
                     uint32_t w[16];
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
-                        float2 v = add2(make_float2(x[e], x[e + 1]), make_float2(y[e], y[e + 1]));
-                        if (hide) {
-                            if (first + 16 * c + e > limit) v.x = -INFINITY;
-                            if (first + 16 * c + e + 1 > limit) v.y = -INFINITY;
-                        }
-                        v = fma2(v, make_float2(f, f), make_float2(-R, -R));
+                        float2 v = fma2(make_float2(x[16 * c + e], x[16 * c + e + 1]), make_float2(f, f), make_float2(-R, -R));
                         v = make_float2(ex2(v.x), ex2(v.y));
                         part = add2(part, v);
                         split2(v.x, v.y, w[e / 2], w[8 + e / 2]);
@@ -586,7 +596,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                 fence_before();
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive(&p_full[s]);
+                    mbar_arrive(&p_full[buf]);
                     mbar_arrive(&al_full[i & 3]);
                 }
             }
