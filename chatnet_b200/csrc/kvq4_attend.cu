@@ -6,6 +6,7 @@
 //
 // Rows: the queries that read one kv head of one sequence, row r = token
 // r / mul, query head kvh * mul + r % mul (mul = n_heads / n_kv).
+#include <float.h>
 #include <math.h>
 
 #include "kvq4.cuh"
@@ -29,7 +30,6 @@ __host__ __device__ constexpr int scale_bytes(int nb) { return tile_pos(nb) * 4 
 // the rows' query fragments
 __host__ __device__ constexpr int query_bytes(int nb) { return 32 * 32 * nb; }
 __host__ __device__ constexpr int ctas_per_sm(int nb) { return nb <= 4 ? 3 : 2; }
-
 
 // Rotated query values e, e + 1 (e even) of one row.
 template <int HD>
@@ -96,7 +96,7 @@ __device__ __forceinline__ uint32_t pair16(const uint32_t* a, int i, const uint3
 
 // Few rows against a long cache (decode).  An item is eight rows of one
 // (sequence, kv head); its CTAs form a cluster, and every warp of it takes
-// every so-manieth tile of 48 positions through a ring of bulk copies of its own,
+// its share of the tiles of 48 positions through a ring of bulk copies of its own,
 // with its own running reference, sum and output.  The partials meet in shared
 // memory, first the CTA's, then the cluster's: no workspace, no atomics, one
 // launch.
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         float sc, inv;
         row_pow2_scale(amax, sc, inv);
-        factor = a.scale * 1.44269504088896341f * 16777216.f * inv;
+        factor = fmaxf(a.scale * 1.44269504088896341f * 16777216.f * inv, FLT_MIN);  // (not 0: -inf is a masked score)
 #pragma unroll
         for (int j = 0; j < NB; j++) {
             float sum_hi = 0.f, sum_lo = 0.f;
@@ -251,6 +251,8 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
         if (ok && !bar_wait(&full[warp][s], parity)) {
             ok = false;
             if (lane == 0) atomicOr(a.err, kErrTimeout);
+            bar_wait(&full[warp][s ^ 1], parity ^ s);  // (nor does the other copy outlive the CTA, if there is one)
+            bar_wait(&full[warp][s], parity);
         }
         const uint8_t* sk = ring + s * TB;
         const uint8_t* sv = sk + TP * RB;
@@ -551,7 +553,8 @@ RowsFn rows_fn(int hd) {
 }
 
 size_t rows_smem(int nb) {
-    const size_t ring = (size_t)kWarps * (kRing * tile_bytes(nb) + scale_bytes(nb)) + query_bytes(nb), merge = (size_t)(kWarps + 1) * 8 * 32 * nb * 4;
+    const size_t ring = (size_t)kWarps * (kRing * tile_bytes(nb) + scale_bytes(nb)) + query_bytes(nb);
+    const size_t merge = (size_t)(kWarps + 1) * 8 * 32 * nb * 4;
     return ring > merge ? ring : merge;
 }
 
@@ -582,15 +585,29 @@ int kvq4_attend(cn_ctx* ctx, const cn_kvq4& c, const float* q, int64_t q_stride,
     a.scale = scale;
     a.err = ctx->dev_err;
     const int64_t rows = (int64_t)n_new * (n_heads / c.n_kv_heads);
-    if (kvq4_prompt_ok(c.head_dim) && rows >= 96) return kvq4_attend_prompt(ctx, c.head_dim, a, st);
     const int64_t groups = (rows + 7) / 8, items = groups * c.n_kv_heads * batch;
     CN_CHECK(items < (1ll << 31) / kMaxCluster, CN_ERR_INVALID_ARG, "too many rows (%lld items)", (long long)items);
+    const int nb = c.head_dim / 32;
+    const int64_t room = (int64_t)ctx->sms * ctas_per_sm(nb);
+    if (kvq4_prompt_ok(c.head_dim) && rows > 16) {
+        // Which kernel: both as measured over the cache's length (the positions are
+        // on the device), in ns.  Here: 6 us for each round of CTAs and 23 positions
+        // of 128 values a ns.  There: 14 us, 8 more for clusters, 1.35 us a tile of
+        // 64 x 128 values.  One sequence, 64 heads over 8 of 128, 8 x tokens rows,
+        // here / there: at 2000 positions 64 rows 15 / 30 us, 192 rows 27 / 34; at
+        // 16000 64 rows 52 / 65, 96 rows 72 / 67, 128 rows 93 / 69.  Four sequences
+        // of 32 heads, 64 rows: at 100 28 / 18, at 2000 99 / 63, at 16000 534 / 376.
+        const int64_t there = kvq4_prompt_items(rows, c.n_kv_heads, batch);
+        const int k = kvq4_prompt_cluster(ctx, there, c.ctx_len);
+        const double rounds = (double)((there * k + ctx->sms - 1) / ctx->sms);
+        const double t_there = (k > 1 ? 22e3 : 14e3) + rounds * ((c.ctx_len / 64 + k - 1) / k) * 10.5 * c.head_dim;
+        const double t_here = 6e3 * (double)((items + room - 1) / room) + (double)items * c.ctx_len * c.head_dim / 2944.;
+        if (t_there < t_here) return kvq4_attend_prompt(ctx, c.head_dim, a, st);
+    }
     a.groups = (int)groups;
     // CTAs per item: the most that all run at once (8 x 64 heads of 128 at 131
     // thousand positions, 64 items: 372 us with 4, 301 with 6, 347 with 8), and
     // no more than give every warp a tile of the longest sequence
-    const int nb = c.head_dim / 32;
-    const int64_t room = (int64_t)ctx->sms * ctas_per_sm(nb);
     const int64_t most = (c.ctx_len + kWarps * tile_pos(nb) - 1) / (kWarps * tile_pos(nb));
     int cluster = 1;
     for (int k : {2, 3, 4, 6, 8, kMaxCluster})

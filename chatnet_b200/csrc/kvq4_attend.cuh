@@ -21,9 +21,10 @@ struct AttendArgs {
     uint32_t* err;
 };
 
-// Many rows: 128 (kvq4_prompt_rows) to a CTA, head dimensions kvq4_prompt_ok.
-int kvq4_prompt_rows();
+// Many rows: items of 128, head dimensions kvq4_prompt_ok.
 bool kvq4_prompt_ok(int hd);
+int64_t kvq4_prompt_items(int64_t rows, int n_kv, int batch);
+int kvq4_prompt_cluster(const cn_ctx* ctx, int64_t items, int ctx_len);
 int kvq4_attend_prompt(cn_ctx* ctx, int hd, AttendArgs a, cudaStream_t st);
 
 // mbar_wait as a short loop (the kernels wait in many places, and code beyond the

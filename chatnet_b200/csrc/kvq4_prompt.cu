@@ -2,24 +2,33 @@
 // the tcgen05 form of cn_kvq4_attend_dev.
 //
 // A CTA takes 128 rows (tokens x the query heads of one kv head) and walks the
-// cache in tiles of 64 positions.  Four warps expand a tile's K and V from
-// nibbles to fp16 in shared memory, one thread issues the MMAs (M = 128) into
-// tensor memory, four warps (one row per thread) turn scores into weights.
-//   S = Q K^T:  Q in tensor memory, K [64 positions][hd] as the B operand;
-//   O = P V:    P in tensor memory, V [hd][64 positions] as the B operand.
-// Precision: q, k, v and the weights are exact or 22-bit pairs of fp16 halves, three
-// MMAs each (lo hi + hi lo + hi hi; k = (level - 8) d and v are 15-bit products,
-// exact as pairs).  O is fresh for every tile and joined in fp32 registers,
-// because the tensor cores' accumulation truncates; that also leaves nothing to
-// rescale in tensor memory.  A row's reference moves only when outgrown by 2^4.
-// Bound: the MMAs, 6 x 64 columns x hd x 128 rows a tile (24 KFLOP a position and
-// row of 128), against which the exponentials and the expansion overlap: the scores of tile
-// i + 1 are computed while tile i's weights are, and tile i's output after them.
+// cache in tiles of 64 positions, K and V expanded from nibbles to fp16:
+//   S = Q K^T:  Q [128 rows][hd] and K [64 positions][hd] in shared memory;
+//   O = P V:    P [128 rows][64 positions] in tensor memory, V [hd][64 positions].
+// Precision: q, k, v and the weights are pairs of fp16 halves (q and the weights to
+// 22 bits; k and v, 15-bit products of a level and a scale, exactly), three MMAs each
+// (lo hi + hi lo, then hi hi: the tensor cores truncate as they add, and lose less
+// while the sum is small).  O is fresh for every tile and joined in fp32 registers for
+// the same reason; that also leaves nothing to rescale in tensor memory.  A row's
+// reference moves only when outgrown by 2^4.
+//
+// Bound: for a tile and hd = 128 the MMAs take 1900 cycles (6 x 64 columns x 128 x
+// 128), the weights of 128 rows about as many instruction slots, the expansion half.
+// So each has warps of its own, three tiles are between their scores and their
+// output, and a tile takes 2700 cycles: what is left is the way of one tile through
+// all of them (K 600, S 950, weights 2100, O 950), two thirds covered.  Weights by eight
+// warps (half the registers each) took 867 us for the 1111 rows at 6000 below
+// instead of 641, P in shared memory 982, MMA loops unrolled (code beyond the
+// instruction caches) 864.  64 query heads over 8, hd 128, 1111 tokens at position
+// 6000: 645 us, 370 TFLOP/s
+// of the formula's 4 hd a pair, three times that as multiplied; 512 tokens at 0: 27.6 us.
 //
 // Order of K's dimensions (any will do, if Q has the same) and V's rows (undone on
 // the way out) follow the nibbles: K position kappa of a 64-wide half is
 // (chunk g, word jj, nibble i, piece b & 1), V row n is (b & 1, i, g, jj), for value
 // 32 b + 8 i + g, b = 2 jj + (b & 1).
+#include <float.h>
+
 #include "kvq4.cuh"
 #include "kvq4_attend.cuh"
 
@@ -28,7 +37,9 @@ namespace cn {
 namespace pr {
 
 constexpr int kRows = 128, kPos = 64;
-constexpr int kThreads = 640;  // warps 0-3 weights, 4-7 output, 8-11 K, 12-15 V, 16 S, 17 loads, 18 O (19 fills the group)
+// warps 0-3 weights (a row a thread), 4-7 queries, then output, 8-11 K's expansion,
+// 12-15 V's, 16 S, 17 loads, 18 O (19 fills the group)
+constexpr int kThreads = 640;
 constexpr int kRaw = 3;        // raw tiles in flight
 constexpr int kBufs = 3;       // tiles between their scores and their output
 constexpr float kPeak = 9.f, kLazy = 4.f;
@@ -61,11 +72,6 @@ __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t* v) {
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
         "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
-}
-__device__ __forceinline__ void st8(uint32_t taddr, const uint32_t* v) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(v[0]),
-                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-                 : "memory");
 }
 __device__ __forceinline__ void ld32(uint32_t taddr, float* f) {
     uint32_t* v = reinterpret_cast<uint32_t*>(f);
@@ -231,86 +237,93 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
     // Registers: 96 a thread at launch (480 for the five groups of four warps);
     // 112 + 184 + 64 + 80 + 32 = 472 once the last three have given theirs up.
     if (warp >= 16) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
-    if (warp == 17) {
-        // ---- raw tiles ----
-        if (lane == 0) {
-            fence_proxy_async();
-            for (int i = 0; i < tiles && ok; i++) {
-                const int s = i % kRaw;
-                if (i >= kRaw) wait(&raw_empty[s], (uint32_t)(i / kRaw - 1));
-                if (!ok) break;
-                const int first = first_of(i);
-                const int64_t row = base + first;
-                const int np = min(kPos, (len - first + 7) & ~7);  // (ctx_len is a multiple of 8)
-                uint8_t* d = smem + G::kRawOff + s * G::kRawTile;
-                mbar_expect_tx(&raw_full[s], (uint32_t)(np * 36 * NB));
-                bulk_load(d, a.kq + row * RB, np * RB, &raw_full[s]);
-                bulk_load(d + kPos * RB, a.vq + row * RB, np * RB, &raw_full[s]);
-                bulk_load(d + 2 * kPos * RB, a.kd + row * NB, np * SB, &raw_full[s]);
-                bulk_load(d + 2 * kPos * RB + kPos * SB, a.vd + row * NB, np * SB, &raw_full[s]);
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+        if (warp == 17) {
+            // ---- raw tiles ----
+            if (lane == 0) {
+                fence_proxy_async();
+                int i = 0;
+                for (; i < tiles; i++) {
+                    const int s = i % kRaw;
+                    if (i >= kRaw) wait(&raw_empty[s], (uint32_t)(i / kRaw - 1));
+                    if (!ok) break;
+                    const int first = first_of(i);
+                    const int64_t row = base + first;
+                    const int np = min(kPos, (len - first + 7) & ~7);  // (ctx_len is a multiple of 8)
+                    uint8_t* d = smem + G::kRawOff + s * G::kRawTile;
+                    mbar_expect_tx(&raw_full[s], (uint32_t)(np * 36 * NB));
+                    bulk_load(d, a.kq + row * RB, np * RB, &raw_full[s]);
+                    bulk_load(d + kPos * RB, a.vq + row * RB, np * RB, &raw_full[s]);
+                    bulk_load(d + 2 * kPos * RB, a.kd + row * NB, np * SB, &raw_full[s]);
+                    bulk_load(d + 2 * kPos * RB + kPos * SB, a.vd + row * NB, np * SB, &raw_full[s]);
+                }
+                // (whoever gave up, no copy outlives the CTA)
+                for (int j = max(i - kRaw, 0); j < i; j++) bar_wait(&raw_full[j % kRaw], (uint32_t)(j / kRaw) & 1);
+            }
+        } else if (warp == 16) {
+            // ---- S.  (The MMA loops stay rolled: their issue, not the tensor cores,
+            // is what a thread of straight-line code would be bound by.) ----
+            if (lane == 0) {
+                constexpr uint32_t kS1 = idesc(kPos), kS2 = idesc(2 * kPos);
+                if (tiles > 0) wait(q_full, 0);
+                int i = 0;
+                for (; i < tiles; i++) {
+                    const int s = i & 1;
+                    wait(&k_full[s], (uint32_t)(i >> 1));
+                    const int buf = i % kBufs;
+                    if (i >= kBufs) wait(&p_empty[buf], (uint32_t)(i / kBufs - 1));  // tile i - 3's weights lie there
+                    if (!ok) break;
+                    fence_after();
+                    const uint64_t kt = desc(smem_u32(smem + s * G::kStage)), q = desc(smem_u32(smem + G::kQOff));
+                    const uint32_t d = tmem + G::kS + buf * 2 * kPos;
+                    // Qlo Khi (and once Qlo Klo, which starts the second half), then Qhi [Khi | Klo]
+                    mma_ss(d, q + kRows * 128 / 16, kt, kS2, 0u);
+#pragma unroll 1
+                    for (int part = 0; part < HD / 64; part++) {
+                        const uint64_t b = kt + part * (2 * kPos * 128 / 16), a = q + (2 * part + 1) * (kRows * 128 / 16);
+#pragma unroll 1
+                        for (int kk = part ? 0 : 1; kk < 4; kk++) mma_ss(d, a + 2 * kk, b + 2 * kk, kS1, 1u);
+                    }
+#pragma unroll 1
+                    for (int part = 0; part < HD / 64; part++) {
+                        const uint64_t b = kt + part * (2 * kPos * 128 / 16), a = q + 2 * part * (kRows * 128 / 16);
+#pragma unroll 1
+                        for (int kk = 0; kk < 4; kk++) mma_ss(d, a + 2 * kk, b + 2 * kk, kS2, 1u);
+                    }
+                    commit(&s_full[buf]);
+                    commit(&k_empty[s]);
+                }
+                // (nor an MMA its tensor memory)
+                if (i > 0) bar_wait(&s_full[(i - 1) % kBufs], (uint32_t)((i - 1) / kBufs) & 1);
+            }
+        } else if (warp == 18) {
+            // ---- O ----
+            if (lane == 0) {
+                constexpr uint32_t kO = idesc(HD);
+                int i = 0;
+                for (; i < tiles; i++) {
+                    const int s = i & 1, buf = i % kBufs;
+                    wait(&v_full[s], (uint32_t)(i >> 1));
+                    wait(&p_full[buf], (uint32_t)(i / kBufs));
+                    if (i > 0) wait(o_empty, (uint32_t)(i - 1));
+                    if (!ok) break;
+                    fence_after();
+                    const uint64_t vt = desc(smem_u32(smem + s * G::kStage + 2 * G::kTile));
+                    const uint32_t d = tmem + G::kO, p = tmem + G::kS + buf * 2 * kPos + kPos;
+#pragma unroll 1
+                    for (int kk = 0; kk < kPos / 16; kk++) {
+                        mma_ts(d, p + 16 * kk + 8, vt + 2 * kk, kO, kk != 0);
+                        mma_ts(d, p + 16 * kk, vt + G::kTile / 16 + 2 * kk, kO, 1u);
+                    }
+#pragma unroll 1
+                    for (int kk = 0; kk < kPos / 16; kk++) mma_ts(d, p + 16 * kk, vt + 2 * kk, kO, 1u);
+                    commit(o_full);
+                    commit(&v_empty[s]);
+                    commit(&p_empty[buf]);
+                }
+                if (i > 0) bar_wait(o_full, (uint32_t)(i - 1) & 1);
             }
         }
-    } else if (warp == 16) {
-        // ---- S.  (The MMA loops stay rolled: their issue, not the tensor cores,
-        // is what a thread of straight-line code would be bound by.) ----
-        if (lane == 0) {
-            constexpr uint32_t kS1 = idesc(kPos), kS2 = idesc(2 * kPos);
-            if (tiles > 0) wait(q_full, 0);
-            for (int i = 0; i < tiles && ok; i++) {
-                const int s = i & 1;
-                wait(&k_full[s], (uint32_t)(i >> 1));
-                const int buf = i % kBufs;
-                if (i >= kBufs) wait(&p_empty[buf], (uint32_t)(i / kBufs - 1));  // tile i - 3's weights lie there
-                if (!ok) break;
-                fence_after();
-                const uint64_t kt = desc(smem_u32(smem + s * G::kStage)), q = desc(smem_u32(smem + G::kQOff));
-                const uint32_t d = tmem + G::kS + buf * 2 * kPos;
-                // Qlo Khi (and once Qlo Klo, which starts the second half), then Qhi [Khi | Klo]
-                mma_ss(d, q + kRows * 128 / 16, kt, kS2, 0u);
-#pragma unroll 1
-                for (int part = 0; part < HD / 64; part++) {
-                    const uint64_t b = kt + part * (2 * kPos * 128 / 16), a = q + (2 * part + 1) * (kRows * 128 / 16);
-#pragma unroll 1
-                    for (int kk = part ? 0 : 1; kk < 4; kk++) mma_ss(d, a + 2 * kk, b + 2 * kk, kS1, 1u);
-                }
-#pragma unroll 1
-                for (int part = 0; part < HD / 64; part++) {
-                    const uint64_t b = kt + part * (2 * kPos * 128 / 16), a = q + 2 * part * (kRows * 128 / 16);
-#pragma unroll 1
-                    for (int kk = 0; kk < 4; kk++) mma_ss(d, a + 2 * kk, b + 2 * kk, kS2, 1u);
-                }
-                commit(&s_full[buf]);
-                commit(&k_empty[s]);
-            }
-        }
-    } else if (warp == 18) {
-        // ---- O ----
-        if (lane == 0) {
-            constexpr uint32_t kO = idesc(HD);
-            for (int i = 0; i < tiles && ok; i++) {
-                const int s = i & 1;
-                const int buf = i % kBufs;
-                wait(&v_full[s], (uint32_t)(i >> 1));
-                wait(&p_full[buf], (uint32_t)(i / kBufs));
-                if (i > 0) wait(o_empty, (uint32_t)(i - 1));
-                if (!ok) break;
-                fence_after();
-                const uint64_t vt = desc(smem_u32(smem + s * G::kStage + 2 * G::kTile));
-                const uint32_t d = tmem + G::kO, p = tmem + G::kS + buf * 2 * kPos + kPos;
-#pragma unroll 1
-                for (int kk = 0; kk < kPos / 16; kk++) {
-                    mma_ts(d, p + 16 * kk + 8, vt + 2 * kk, kO, kk != 0);
-                    mma_ts(d, p + 16 * kk, vt + G::kTile / 16 + 2 * kk, kO, 1u);
-                }
-#pragma unroll 1
-                for (int kk = 0; kk < kPos / 16; kk++) mma_ts(d, p + 16 * kk, vt + 2 * kk, kO, 1u);
-                commit(o_full);
-                commit(&v_empty[s]);
-                commit(&p_empty[buf]);
-            }
-        }
-    }
     } else if (warp >= 8) {
         // ---- expansion: K by warps 8-11, V by 12-15 ----
         const int tid = threadIdx.x & 127;
@@ -459,7 +472,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
 #pragma unroll
                 for (int e = 0; e < HD; e++) amax = fmaxf(amax, fabsf(o[e]));
                 row_pow2_scale(amax, sc, inv);
-                mR[r] = a.scale * 1.44269504088896341f * inv;  // (what a score counts, for the weights' warps)
+                mR[r] = fmaxf(a.scale * 1.44269504088896341f * inv, FLT_MIN);  // what a score counts, for the weights' warps (not 0: -inf is a masked score)
 #pragma unroll
                 for (int k16 = 0; k16 < HD / 8; k16++) {
                     uint32_t hi[4], lo[4];
@@ -606,7 +619,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
             if (lane == 0) mbar_arrive(l_full);
         }
     }
-    // every MMA is done (its output was waited for) and every copy landed
+    // every MMA is done and every copy landed
     fence_before();
     __syncthreads();
     fence_after();
@@ -638,19 +651,25 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
     }
 }
 
-int kvq4_prompt_rows() { return pr::kRows; }
-
 bool kvq4_prompt_ok(int hd) { return hd == 64 || hd == 128; }
+
+int64_t kvq4_prompt_items(int64_t rows, int n_kv, int batch) { return (rows + pr::kRows - 1) / pr::kRows * n_kv * batch; }
+
+// CTAs per item: as many as the SMs hold (one each), four tiles for each at least
+// (64 query heads over 8, 16 tokens at 30000: 108 us with 8 CTAs, 170 by the
+// kernel for few rows)
+int kvq4_prompt_cluster(const cn_ctx* ctx, int64_t items, int ctx_len) {
+    int k = 1;
+    while (k < pr::kMaxCluster && 2 * k * items <= ctx->sms && 2 * k * 4 * pr::kPos <= ctx_len) k *= 2;
+    return k;
+}
 
 int kvq4_attend_prompt(cn_ctx* ctx, int hd, AttendArgs a, cudaStream_t st) {
     using namespace pr;
-    const int64_t rows = (int64_t)a.n_new * (a.n_heads / a.n_kv), groups = (rows + kRows - 1) / kRows;
-    const int64_t items = groups * a.n_kv * a.batch;
+    const int64_t rows = (int64_t)a.n_new * (a.n_heads / a.n_kv), items = kvq4_prompt_items(rows, a.n_kv, a.batch);
     CN_CHECK(items < (1ll << 31) / kMaxCluster, CN_ERR_INVALID_ARG, "too many rows (%lld items)", (long long)items);
-    a.groups = (int)groups;
-    // CTAs per item: as many as the SMs hold (one each), four tiles for each at least
-    int cluster = 1;
-    while (cluster < kMaxCluster && 2 * cluster * items <= ctx->sms && 2 * cluster * 4 * kPos <= a.ctx_len) cluster *= 2;
+    a.groups = (int)((rows + kRows - 1) / kRows);
+    const int cluster = kvq4_prompt_cluster(ctx, items, a.ctx_len);
     using Fn = void (*)(AttendArgs);
     const Fn fn = hd == 64 ? (Fn)kvq4_attend_prompt_kernel<64> : (Fn)kvq4_attend_prompt_kernel<128>;
     const int smem = hd == 64 ? Geo<64>::kSmem : Geo<128>::kSmem;
