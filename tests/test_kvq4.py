@@ -318,6 +318,94 @@ def test_attend(ctx, hd, kv, mul, ctx_len, n_new, pos, count, rope, neox):
     _check_attend(ctx, box, len(pos), mul * kv, n_new, pos, count, table, neox, gen)
 
 
+PROMPTS = [  # sizes at which rows go 128 to a CTA, in clusters of 1 (the first four), 2, 2, 4, 8, 8
+    (128, 8, 8, 512, 64, [0, 1, 63, 448], None, True, False),
+    (128, 4, 3, 512, 171, [0, 300, 341, -1, 511, 7, 600, 64], [171, 171, 170, 9, 171, 1, 171, 0], True, True),
+    (64, 4, 8, 512, 100, [0, 412, 63, 65], None, True, False),
+    (64, 1, 71, 2048, 40, [2008, 0, 1000, 24, 23, 2047], None, False, False),
+    (128, 8, 8, 8192, 120, [8000], None, True, False),
+    (128, 4, 8, 16384, 90, [16001, 6], [90, 77], False, False),
+    (64, 4, 8, 16384, 120, [16002], None, True, True),
+    (64, 8, 4, 32768, 33, [30001], None, True, True),
+    (128, 1, 8, 16384, 130, [16254, 5], [130, 127], True, False),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,kv,mul,ctx_len,n_new,pos,count,rope,neox", PROMPTS)
+def test_attend_prompts(ctx, hd, kv, mul, ctx_len, n_new, pos, count, rope, neox):
+    gen = _gen(hd * 1000 + n_new + 1)
+    box = Box(len(pos), kv, hd, ctx_len)
+    for b, p in enumerate(pos):
+        if p >= 0:
+            box.fill(b, min(ctx_len, p + n_new), gen)
+    table = ref.rope_table(ctx_len, hd).cuda() if rope else None
+    _check_attend(ctx, box, len(pos), mul * kv, n_new, pos, count, table, neox, gen, q_extra=4, out_extra=8)
+
+
+# one token, a few, a prompt of 128 rows to a CTA (8 sequences: rows enough)
+FORMS = [(1, 1), (1, 24), (8, 130)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("batch,n_new", FORMS)
+def test_attend_peaked_and_flat_prompts(ctx, hd, batch, n_new):
+    """As test_attend_peaked_and_flat, and with products of q and scale below fp32's normal range."""
+    gen = _gen(16)
+    for mul, scale in ((300.0, None), (1e4, None), (0.0, None), (1e-30, None), (1e-40, 1e-20), (1e-3, 1e-38)):
+        box = Box(batch, 4, hd, 512)
+        for b in range(batch):
+            box.fill(b, 512, gen)
+        pos = [(37 * b) % 300 for b in range(batch)]
+        _check_attend(ctx, box, batch, 16, n_new, pos, None, None, False, gen, qmul=mul, scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("batch,n_new", FORMS)
+@pytest.mark.parametrize("lowest", [-20, 0, 10])
+def test_attend_scale_ranges(ctx, hd, batch, n_new, lowest):
+    """Scales of either sign, zero, and powers of two times [1, 2) up to 2^15 for K and V, tile by tile and mixed (a
+    block's values reach 8 * 60000); q small enough for the scores to differ by a few."""
+    gen = _gen(17)
+    box = Box(batch, 4, hd, 512)
+    for b in range(batch):
+        box.fill(b, 512, gen)
+    for w in "kv":
+        shape = box.q[w][1].shape
+        e = torch.randint(lowest, 16, shape, generator=gen, device="cuda")
+        e[:, :, 64:128] = lowest                             # a tile without large ones
+        d = 2.0 ** e * (1 + torch.rand(shape, generator=gen, device="cuda") * 0.8)
+        d = d * torch.randint(-1, 2, shape, generator=gen, device="cuda")
+        box.q[w][1].copy_(d.half())
+    pos = [(37 * b) % 300 for b in range(batch)]
+    _check_attend(ctx, box, batch, 16, n_new, pos, None, None, False, gen, qmul=1e-5)
+
+
+@pytest.mark.gpu
+def test_attend_lone_nan_and_infinite_queries(ctx):
+    """A row whose query is not finite leaves the rows beside it alone."""
+    for batch, n_new in FORMS:
+        gen = _gen(18)
+        box = Box(batch, 4, 128, 512)
+        for b in range(batch):
+            box.fill(b, 512, gen)
+        heads, hd = 16, 128
+        q = torch.randn(batch, n_new, heads * hd, generator=gen, device="cuda")
+        clean, out = (torch.full_like(q, 7.5) for _ in range(2))
+        p = _ints([200] * batch)
+        s = torch.cuda.current_stream().cuda_stream
+        ctx.kvq4_attend_dev(box.cache, q.data_ptr(), clean.data_ptr(), p.data_ptr(), batch, heads, n_new=n_new, stream=s)
+        q[0, 0, 3 * hd + 5], q[-1, -1, 9 * hd] = torch.nan, torch.inf
+        ctx.kvq4_attend_dev(box.cache, q.data_ptr(), out.data_ptr(), p.data_ptr(), batch, heads, n_new=n_new, stream=s)
+        torch.cuda.synchronize()
+        x, y = (t.view(batch, n_new, heads, hd) for t in (out, clean))
+        assert x[0, 0, 3].isnan().all() and x[-1, -1, 9].isnan().all()
+        x[0, 0, 3], x[-1, -1, 9] = y[0, 0, 3], y[-1, -1, 9]
+        assert torch.equal(x, y)
+
+
 @pytest.mark.gpu
 def test_attend_strides_layers_and_scale(ctx):
     gen = _gen(5)
@@ -398,6 +486,51 @@ def test_attend_is_deterministic_on_streams_and_in_graphs(ctx):
     graphs[0].replay()
     torch.cuda.synchronize()
     verify(box, q, outs[2], heads, 1, [100, 10, 1400, 2], None, None, False, hd ** -0.5)
+
+
+@pytest.mark.gpu
+def test_prompts_on_streams_and_in_graphs(ctx):
+    """Two prompt calls at once, captured ones replayed at once and with new inputs; single CTAs and clusters."""
+    for kv, ctx_len, pos, n_new in ((8, 512, [0, 300, 64], 128), (1, 16384, [16000], 130)):
+        gen, hd, heads, batch = _gen(19), 128, 8 * kv, len(pos)
+        box = Box(batch, kv, hd, ctx_len)
+        for b, x in enumerate(pos):
+            box.fill(b, x + n_new, gen)
+        q = torch.randn(batch, n_new, heads * hd, generator=gen, device="cuda")
+        outs = [torch.full_like(q, 7.5) for _ in range(4)]
+        p = _ints(pos)
+        s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+
+        def call(out, stream):
+            ctx.kvq4_attend_dev(box.cache, q.data_ptr(), out.data_ptr(), p.data_ptr(), batch, heads, n_new=n_new,
+                                stream=stream.cuda_stream)
+
+        for _ in range(5):
+            call(outs[0], s1)
+            call(outs[1], s2)
+        graphs = []
+        for k in (2, 3):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                call(outs[k], torch.cuda.current_stream())
+            graphs.append(g)
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for g, s in zip(graphs, (s1, s2)):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        verify(box, q, outs[0], heads, n_new, pos, None, None, False, hd ** -0.5)
+        for o in outs[1:]:
+            assert torch.equal(o, outs[0])
+        q.mul_(0.5)
+        lower = [max(x - 1, 0) for x in pos]
+        p.copy_(_ints(lower))
+        outs[3].fill_(7.5)
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        verify(box, q, outs[3], heads, n_new, lower, None, None, False, hd ** -0.5)
 
 
 @pytest.mark.gpu

@@ -158,6 +158,25 @@ def test_ties_and_masks(ctx, vocab):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("rows", [3, 300])  # a row over several CTAs, and one CTA to a row
+def test_rows_that_rise_or_hide_their_best(ctx, rows, half):
+    """More candidates than a CTA keeps, and first parts of rows that hold nothing to compare with."""
+    vocab = 50001
+    i = torch.arange(vocab, device="cuda")
+    x = torch.randn(rows, vocab, generator=_gen(11), device="cuda")
+    x[0] = (i // 25).float() * 0.01                  # rising
+    x[1, :45000] = -torch.inf                        # nothing at first
+    x[2] = -torch.inf
+    x[2, 49998] = -5.0                               # fewer values than asked for
+    x[-1] = torch.where(i < 4096, -1.0, (i % 7).float())
+    x = x.half() if half else x
+    tok = torch.randint(45000, vocab, (rows,), generator=_gen(12), device="cuda", dtype=torch.int32)
+    for top in (1, 20, 64):
+        check(x, tok, top, run(ctx, x, tok, top))
+
+
+@pytest.mark.gpu
 def test_rows_without_a_distribution(ctx):
     for vocab in (50, 20000):
         x = torch.randn(4, vocab, generator=_gen(1), device="cuda")
