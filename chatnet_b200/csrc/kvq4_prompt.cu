@@ -41,7 +41,9 @@ constexpr int kRows = 128, kPos = 64;
 // 12-15 V's, 16 S, 17 loads, 18 O (19 fills the group)
 constexpr int kThreads = 640;
 constexpr int kRaw = 3;        // raw tiles in flight
-constexpr int kBufs = 3;       // tiles between their scores and their output
+constexpr int kBufs = 4;       // tiles between their scores and their output
+constexpr int kStages = 3;     // expanded tiles
+constexpr int kSlots = 8;      // tiles that words between the warps are kept for: more than any is ahead
 constexpr float kPeak = 9.f, kLazy = 4.f;
 constexpr int kMaxCluster = 8;
 
@@ -51,17 +53,16 @@ struct Geo {
     static constexpr int kTile = kPos * HD * 2;     // bytes of one fp16 K or V tile
     static constexpr int kStage = 4 * kTile;        // K (hi, lo of each 64-wide part), V hi, V lo
     static constexpr int kRawTile = kPos * 36 * NB;
-    static constexpr int kQOff = 2 * kStage;        // Q: hi and lo of each 64-wide part, 128 rows of 128 bytes
-    static constexpr int kRawOff = kQOff + 2 * HD * kRows * 2;
+    static constexpr int kRawOff = kStages * kStage;
     static constexpr int kBarOff = kRawOff + kRaw * kRawTile;
-    static constexpr int kRowOff = kBarOff + 512;  // per row: four rescalings, the last reference and sum
-    static constexpr int kSmem = kRowOff + kRows * (4 * 4 + 8) + 1024;
-    // tensor-memory columns: kBufs of S (64 columns of Q Khi, 64 of Qhi Klo; the
-    // weights in the second half's place, for 16 positions 8 columns of halves and
-    // 8 of low halves); O
-    static constexpr int kS = 0, kO = kBufs * 2 * kPos;
+    static constexpr int kRowOff = kBarOff + 768;  // per row: rescalings, the last reference and sum
+    static constexpr int kSmem = kRowOff + kRows * (4 * kSlots + 8) + 1024;
+    // tensor-memory columns: kBufs of S (the weights in its place, for 16 positions
+    // 8 columns of halves and 8 of low halves); O; Q's halves, Q's low halves
+    static constexpr int kS = 0, kO = kBufs * kPos, kQ = kO + HD;
     static constexpr int kCols = 512;
-    static_assert(kO + HD <= kCols, "tensor memory");
+    static_assert(kQ + HD <= kCols, "tensor memory");
+    static_assert(8 * (2 * kRaw + 4 * kStages + 3 * kBufs + 3 * kSlots + 4) + 8 + 8 * kSlots <= kRowOff - kBarOff, "barriers");
     static_assert(kBarOff % 8 == 0 && kSmem <= 227 * 1024, "shared memory");
 };
 
@@ -112,20 +113,16 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
         "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// both operands from shared memory
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
 // A K-major operand tile: rows of 128 bytes, 16-byte pieces at piece ^ (row & 7)
 // (128-byte swizzle), 8-row groups 1024 bytes apart.
 __device__ __forceinline__ uint64_t desc(uint32_t addr) {
     return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
            (2ull << 61);
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
 }
 // D fp32, A and B fp16, K-major, N columns, M = 128
 __host__ __device__ constexpr uint32_t idesc(int n) {
@@ -152,25 +149,25 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint64_t* raw_full = reinterpret_cast<uint64_t*>(smem + G::kBarOff);
     uint64_t* raw_empty = raw_full + kRaw;
-    uint64_t* k_full = raw_empty + kRaw;  // [2]
-    uint64_t* v_full = k_full + 2;
-    uint64_t* k_empty = v_full + 2;
-    uint64_t* v_empty = k_empty + 2;
-    uint64_t* s_full = v_empty + 2;
+    uint64_t* k_full = raw_empty + kRaw;
+    uint64_t* v_full = k_full + kStages;
+    uint64_t* k_empty = v_full + kStages;
+    uint64_t* v_empty = k_empty + kStages;
+    uint64_t* s_full = v_empty + kStages;
     uint64_t* p_full = s_full + kBufs;
     uint64_t* p_empty = p_full + kBufs;
-    uint64_t* al_full = p_empty + kBufs;  // [4]
-    uint64_t* o_full = al_full + 4;
+    uint64_t* al_full = p_empty + kBufs;
+    uint64_t* o_full = al_full + kSlots;
     uint64_t* o_empty = o_full + 1;
     uint64_t* q_full = o_empty + 1;
     uint64_t* l_full = q_full + 1;
-    uint64_t* u_full = l_full + 1;  // [2][8]
-    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(u_full + 16);
-    float* undo = reinterpret_cast<float*>(tmem_holder + 2);  // [2][8] what K's and V's tiles were scaled down by
-    float* slots = reinterpret_cast<float*>(smem + G::kRowOff);    // [4][128] what a tile multiplies the row's output by
-    float* mR = reinterpret_cast<float*>(slots + 4 * kRows);       // [128] references
+    uint64_t* u_full = l_full + 1;  // [2][kSlots]
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(u_full + 2 * kSlots);
+    float* undo = reinterpret_cast<float*>(tmem_holder + 2);  // [2][kSlots] what K's and V's tiles were scaled down by
+    float* slots = reinterpret_cast<float*>(smem + G::kRowOff);    // [kSlots][128] what a tile multiplies the row's output by
+    float* mR = reinterpret_cast<float*>(slots + kSlots * kRows);       // [128] references
     float* mL = mR + kRows;                                        // [128] sums of weights
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t cs = cluster_size(), rank = cluster_rank();
 
     // this cluster's 128 rows; the last tokens, which see most, first
@@ -193,7 +190,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
             mbar_init(&raw_full[s], 1);
             mbar_init(&raw_empty[s], 8);
         }
-        for (int s = 0; s < 2; s++) {
+        for (int s = 0; s < kStages; s++) {
             mbar_init(&k_full[s], 4);
             mbar_init(&v_full[s], 4);
             mbar_init(&k_empty[s], 1);
@@ -204,8 +201,8 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
             mbar_init(&p_full[s], 4);
             mbar_init(&p_empty[s], 1);
         }
-        for (int s = 0; s < 4; s++) mbar_init(&al_full[s], 4);
-        for (int s = 0; s < 16; s++) mbar_init(&u_full[s], 1);
+        for (int s = 0; s < kSlots; s++) mbar_init(&al_full[s], 4);
+        for (int s = 0; s < 2 * kSlots; s++) mbar_init(&u_full[s], 1);
         mbar_init(l_full, 4);
         mbar_init(o_full, 1);
         mbar_init(o_empty, 4);
@@ -260,66 +257,67 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                 // (whoever gave up, no copy outlives the CTA)
                 for (int j = max(i - kRaw, 0); j < i; j++) bar_wait(&raw_full[j % kRaw], (uint32_t)(j / kRaw) & 1);
             }
-        } else if (warp == 16) {
-            // ---- S.  (The MMA loops stay rolled: their issue, not the tensor cores,
-            // is what a thread of straight-line code would be bound by.) ----
-            if (lane == 0) {
-                constexpr uint32_t kS1 = idesc(kPos), kS2 = idesc(2 * kPos);
-                if (tiles > 0) wait(q_full, 0);
-                int i = 0;
-                for (; i < tiles; i++) {
-                    const int s = i & 1;
-                    wait(&k_full[s], (uint32_t)(i >> 1));
-                    const int buf = i % kBufs;
-                    if (i >= kBufs) wait(&p_empty[buf], (uint32_t)(i / kBufs - 1));  // tile i - 3's weights lie there
-                    if (!ok) break;
+        } else if (warp == 16 || warp == 18) {
+            // ---- S, O.  The whole warp goes through the loops, with values that are
+            // the same in all lanes, and one lane issues: 33 and 65 cycles an MMA of 64
+            // and 128 columns, as the tensor cores take them; a thread by itself
+            // issues one in 84 (50 with the loop unrolled). ----
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const int count = __shfl_sync(0xffffffffu, tiles, 0);
+            const bool lead = elect_one();
+            int i = 0;
+            if (warp == 16) {
+                constexpr uint32_t kN = idesc(kPos);
+                if (count > 0) wait(q_full, 0);
+                for (; i < count; i++) {
+                    const int s = i % kStages, buf = i % kBufs;
+                    wait(&k_full[s], (uint32_t)(i / kStages));
+                    if (i >= kBufs) wait(&p_empty[buf], (uint32_t)(i / kBufs - 1));  // tile i - kBufs' weights lie there
+                    if (!__all_sync(0xffffffffu, ok)) break;
                     fence_after();
-                    const uint64_t kt = desc(smem_u32(smem + s * G::kStage)), q = desc(smem_u32(smem + G::kQOff));
-                    const uint32_t d = tmem + G::kS + buf * 2 * kPos;
-                    // Qlo Khi (and once Qlo Klo, which starts the second half), then Qhi [Khi | Klo]
-                    mma_ss(d, q + kRows * 128 / 16, kt, kS2, 0u);
-#pragma unroll 1
-                    for (int part = 0; part < HD / 64; part++) {
-                        const uint64_t b = kt + part * (2 * kPos * 128 / 16), a = q + (2 * part + 1) * (kRows * 128 / 16);
-#pragma unroll 1
-                        for (int kk = part ? 0 : 1; kk < 4; kk++) mma_ss(d, a + 2 * kk, b + 2 * kk, kS1, 1u);
+                    const uint64_t kt = desc(smem_u32(smem + s * G::kStage));
+                    const uint32_t d = tm + G::kS + buf * kPos;
+                    // Qlo Khi, Qhi Klo, Qhi Khi
+#pragma unroll
+                    for (int m = 0; m < 3; m++)
+#pragma unroll
+                        for (int kk = 0; kk < HD / 16; kk++)
+                            if (lead)
+                                mma_ts(d, tm + G::kQ + (m == 0 ? HD / 2 : 0) + 8 * kk,
+                                       kt + (m == 1 ? kPos * 128 / 16 : 0) + (kk >> 2) * (2 * kPos * 128 / 16) + 2 * (kk & 3),
+                                       kN, m + kk != 0);
+                    if (lead) {
+                        commit(&s_full[buf]);
+                        commit(&k_empty[s]);
                     }
-#pragma unroll 1
-                    for (int part = 0; part < HD / 64; part++) {
-                        const uint64_t b = kt + part * (2 * kPos * 128 / 16), a = q + 2 * part * (kRows * 128 / 16);
-#pragma unroll 1
-                        for (int kk = 0; kk < 4; kk++) mma_ss(d, a + 2 * kk, b + 2 * kk, kS2, 1u);
-                    }
-                    commit(&s_full[buf]);
-                    commit(&k_empty[s]);
+                    __syncwarp();
                 }
-                // (nor an MMA its tensor memory)
+                // (whoever gave up, no MMA outlives its tensor memory)
                 if (i > 0) bar_wait(&s_full[(i - 1) % kBufs], (uint32_t)((i - 1) / kBufs) & 1);
-            }
-        } else if (warp == 18) {
-            // ---- O ----
-            if (lane == 0) {
-                constexpr uint32_t kO = idesc(HD);
-                int i = 0;
-                for (; i < tiles; i++) {
-                    const int s = i & 1, buf = i % kBufs;
-                    wait(&v_full[s], (uint32_t)(i >> 1));
+            } else {
+                constexpr uint32_t kN = idesc(HD);
+                for (; i < count; i++) {
+                    const int s = i % kStages, buf = i % kBufs;
+                    wait(&v_full[s], (uint32_t)(i / kStages));
                     wait(&p_full[buf], (uint32_t)(i / kBufs));
                     if (i > 0) wait(o_empty, (uint32_t)(i - 1));
-                    if (!ok) break;
+                    if (!__all_sync(0xffffffffu, ok)) break;
                     fence_after();
                     const uint64_t vt = desc(smem_u32(smem + s * G::kStage + 2 * G::kTile));
-                    const uint32_t d = tmem + G::kO, p = tmem + G::kS + buf * 2 * kPos + kPos;
-#pragma unroll 1
-                    for (int kk = 0; kk < kPos / 16; kk++) {
-                        mma_ts(d, p + 16 * kk + 8, vt + 2 * kk, kO, kk != 0);
-                        mma_ts(d, p + 16 * kk, vt + G::kTile / 16 + 2 * kk, kO, 1u);
+                    const uint32_t d = tm + G::kO, p = tm + G::kS + buf * kPos;
+#pragma unroll
+                    for (int m = 0; m < 3; m++)
+#pragma unroll
+                        for (int kk = 0; kk < kPos / 16; kk++)
+                            if (lead)
+                                mma_ts(d, p + 16 * kk + (m == 0 ? 8 : 0), vt + (m == 1 ? G::kTile / 16 : 0) + 2 * kk, kN,
+                                       m + kk != 0);
+                    if (lead) {
+                        commit(o_full);
+                        commit(&v_empty[s]);
+                        commit(&p_empty[buf]);
                     }
-#pragma unroll 1
-                    for (int kk = 0; kk < kPos / 16; kk++) mma_ts(d, p + 16 * kk, vt + 2 * kk, kO, 1u);
-                    commit(o_full);
-                    commit(&v_empty[s]);
-                    commit(&p_empty[buf]);
+                    __syncwarp();
                 }
                 if (i > 0) bar_wait(o_full, (uint32_t)(i - 1) & 1);
             }
@@ -339,8 +337,8 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
             }
             const bool big = __any_sync(0xffffffffu, max(mx & 0xFFFFu, mx >> 16) >= 0x6C00u);
             if (tid == 0) {
-                undo[8 * kv + (i & 7)] = big ? 16.f : 1.f;
-                mbar_arrive(&u_full[8 * kv + (i & 7)]);
+                undo[kSlots * kv + i % kSlots] = big ? 16.f : 1.f;
+                mbar_arrive(&u_full[kSlots * kv + i % kSlots]);
             }
             return big ? 0x2C002C00u : 0x3C003C00u;
         };
@@ -349,7 +347,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
             // position p, chunks 4 hf .. + 3 (each W 16-byte pieces)
             const int p = tid & 63, hf = tid >> 6;
             for (int i = 0; i < tiles; i++) {
-                const int rs = i % kRaw, s = i & 1;
+                const int rs = i % kRaw, s = i % kStages;
                 const uint8_t* raw = smem + G::kRawOff + rs * G::kRawTile;
                 wait(&raw_full[rs], (uint32_t)(i / kRaw));
                 const uint32_t shrink = shrink_of(raw, i);
@@ -358,7 +356,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                 uint32_t d[W];
 #pragma unroll
                 for (int j = 0; j < W; j++) d[j] = in ? h2_mul(sc[j], shrink) : 0u;
-                if (i >= 2) wait(&k_empty[s], (uint32_t)((i >> 1) - 1));
+                if (i >= kStages) wait(&k_empty[s], (uint32_t)(i / kStages - 1));
                 uint8_t* stage = smem + s * G::kStage + p * 128;
 #pragma unroll 1
                 for (int j = 0; j < W; j++) {
@@ -390,7 +388,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
             constexpr int NI = 2 * W;  // nibbles a thread takes
             const int i0 = W == 2 ? 0 : (tid >> 6) * 2;
             for (int i = 0; i < tiles; i++) {
-                const int rs = i % kRaw, s = i & 1, first = first_of(i) + 8 * k;
+                const int rs = i % kRaw, s = i % kStages, first = first_of(i) + 8 * k;
                 const uint8_t* raw = smem + G::kRawOff + rs * G::kRawTile;
                 wait(&raw_full[rs], (uint32_t)(i / kRaw));
                 const uint32_t shrink = shrink_of(raw, i);
@@ -405,7 +403,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&raw_empty[rs]);
-                if (i >= 2) wait(&v_empty[s], (uint32_t)((i >> 1) - 1));
+                if (i >= kStages) wait(&v_empty[s], (uint32_t)(i / kStages - 1));
                 uint8_t* stage = smem + s * G::kStage + 2 * G::kTile;
 #pragma unroll 1
                 for (int pb = 0; pb < 2; pb++)
@@ -474,34 +472,37 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                 row_pow2_scale(amax, sc, inv);
                 mR[r] = fmaxf(a.scale * 1.44269504088896341f * inv, FLT_MIN);  // what a score counts, for the weights' warps (not 0: -inf is a masked score)
 #pragma unroll
-                for (int k16 = 0; k16 < HD / 8; k16++) {
-                    uint32_t hi[4], lo[4];
-                    const int g = k16 / W, jj = k16 % W;
+                for (int c = 0; c < HD / 32; c++) {  // 32 dimensions: four pieces of 8
+                    uint32_t hi[16], lo[16];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int e = 64 * jj + 8 * i + g;  // and the next block's
-                        split2(o[e] * sc, o[e + 32] * sc, hi[i], lo[i]);
+                    for (int k = 0; k < 4; k++) {
+                        const int g = (4 * c + k) / W, jj = (4 * c + k) % W;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int e = 64 * jj + 8 * i + g;  // and the next block's
+                            split2(o[e] * sc, o[e + 32] * sc, hi[4 * k + i], lo[4 * k + i]);
+                        }
                     }
-                    uint8_t* t = smem + G::kQOff + (k16 / 8) * (2 * kRows * 128) + r * 128 + (((k16 & 7) ^ (r & 7)) << 4);
-                    *reinterpret_cast<uint4*>(t) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    *reinterpret_cast<uint4*>(t + kRows * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    st16(tmem + lane_off + G::kQ + 16 * c, hi);
+                    st16(tmem + lane_off + G::kQ + HD / 2 + 16 * c, lo);
                 }
-                fence_proxy_async();
+                wait_st();
+                fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_full);
             }
 #pragma unroll
             for (int e = 0; e < HD; e++) o[e] = 0.f;
             for (int i = 0; i < tiles; i++) {
-                wait(&al_full[i & 3], (uint32_t)(i >> 2));
-                const float am = slots[(i & 3) * kRows + r];
+                wait(&al_full[i % kSlots], (uint32_t)(i / kSlots));
+                const float am = slots[(i % kSlots) * kRows + r];
                 if (!__all_sync(0xffffffffu, am == 1.f)) {
 #pragma unroll
                     for (int e = 0; e < HD; e++) o[e] *= am;
                 }
                 wait(o_full, (uint32_t)i);
-                wait(&u_full[8 + (i & 7)], (uint32_t)(i >> 3));
-                const float vm = undo[8 + (i & 7)];
+                wait(&u_full[kSlots + i % kSlots], (uint32_t)(i / kSlots));
+                const float vm = undo[kSlots + i % kSlots];
                 fence_after();
                 float t[2][16];
                 ld16(tmem + lane_off + G::kO, t[0]);
@@ -554,27 +555,16 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
             const int seen_by_all = p0 + r0 / mul + 1;
             for (int i = 0; i < tiles; i++) {
                 const int buf = i % kBufs, first = first_of(i);
-                wait(&u_full[i & 7], (uint32_t)(i >> 3));
-                const float f = factor * undo[i & 7];
+                wait(&u_full[i % kSlots], (uint32_t)(i / kSlots));
+                const float f = factor * undo[i % kSlots];
                 wait(&s_full[buf], (uint32_t)(i / kBufs));
                 fence_after();
-                const uint32_t sc = tmem + lane_off + G::kS + buf * 2 * kPos;
+                const uint32_t sc = tmem + lane_off + G::kS + buf * kPos;
                 const bool hide = first + kPos > seen_by_all;
                 float x[64], top = -INFINITY, move = 1.f;
                 ld32(sc, x);
                 ld32(sc + 32, x + 32);
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    float y[16];
-                    ld16(sc + kPos + 16 * c, y);
-                    wait_ld();
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        const float2 v =
-                            add2(make_float2(x[16 * c + e], x[16 * c + e + 1]), make_float2(y[e], y[e + 1]));
-                        x[16 * c + e] = v.x, x[16 * c + e + 1] = v.y;
-                    }
-                }
+                wait_ld();
                 if (hide) {
 #pragma unroll
                     for (int e = 0; e < 64; e++)
@@ -587,8 +577,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                     move = ex2(R - to);
                     R = to;
                 }
-                // 16 scores at a time: their sums, weights, and the halves in the place of
-                // the second summands (8 columns of halves, 8 of low halves)
+                // 16 scores at a time: weights, and their halves in the scores' place
                 float2 part = make_float2(0.f, 0.f);
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
@@ -600,17 +589,17 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                         part = add2(part, v);
                         split2(v.x, v.y, w[e / 2], w[8 + e / 2]);
                     }
-                    st16(sc + kPos + 16 * c, w);
+                    st16(sc + 16 * c, w);
                 }
                 const float sum = part.x + part.y;
                 l = l * move + sum;
-                slots[(i & 3) * kRows + r] = move;
+                slots[(i % kSlots) * kRows + r] = move;
                 wait_st();
                 fence_before();
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(&p_full[buf]);
-                    mbar_arrive(&al_full[i & 3]);
+                    mbar_arrive(&al_full[i % kSlots]);
                 }
             }
             mR[r] = R;
