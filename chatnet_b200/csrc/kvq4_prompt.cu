@@ -38,12 +38,15 @@ namespace pr {
 
 constexpr int kRows = 128, kPos = 64;
 // warps 0-3 weights (a row a thread), 4-7 queries, then output, 8-11 K's expansion,
-// 12-15 V's, 16 S, 17 loads, 18 O (19 fills the group)
+// 12-15 V's, 16 S, 17 loads, 18 O, 19 scales' ranges
 constexpr int kThreads = 640;
 constexpr int kRaw = 3;        // raw tiles in flight
 constexpr int kBufs = 4;       // tiles between their scores and their output
 constexpr int kStages = 3;     // expanded tiles
-constexpr int kSlots = 8;      // tiles that words between the warps are kept for: more than any is ahead
+// Slots of words that pass between warps, more than any is ahead: a tile's weights
+// are after the output of tile - kBufs, its scales' range after that of
+// tile - kRaw - kStages - kBufs = tile - 10.
+constexpr int kSlots = 8, kUndo = 16;
 constexpr float kPeak = 9.f, kLazy = 4.f;
 constexpr int kMaxCluster = 8;
 
@@ -62,7 +65,7 @@ struct Geo {
     static constexpr int kS = 0, kO = kBufs * kPos, kQ = kO + HD;
     static constexpr int kCols = 512;
     static_assert(kQ + HD <= kCols, "tensor memory");
-    static_assert(8 * (2 * kRaw + 4 * kStages + 3 * kBufs + 3 * kSlots + 4) + 8 + 8 * kSlots <= kRowOff - kBarOff, "barriers");
+    static_assert(8 * (2 * kRaw + 4 * kStages + 3 * kBufs + kSlots + 2 * kUndo + 4) + 8 + 8 * kUndo <= kRowOff - kBarOff, "barriers");
     static_assert(kBarOff % 8 == 0 && kSmem <= 227 * 1024, "shared memory");
 };
 
@@ -161,9 +164,9 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
     uint64_t* o_empty = o_full + 1;
     uint64_t* q_full = o_empty + 1;
     uint64_t* l_full = q_full + 1;
-    uint64_t* u_full = l_full + 1;  // [2][kSlots]
-    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(u_full + 2 * kSlots);
-    float* undo = reinterpret_cast<float*>(tmem_holder + 2);  // [2][kSlots] what K's and V's tiles were scaled down by
+    uint64_t* u_full = l_full + 1;  // [2][kUndo]
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(u_full + 2 * kUndo);
+    float* undo = reinterpret_cast<float*>(tmem_holder + 2);  // [2][kUndo] what K's and V's tiles were scaled down by
     float* slots = reinterpret_cast<float*>(smem + G::kRowOff);    // [kSlots][128] what a tile multiplies the row's output by
     float* mR = reinterpret_cast<float*>(slots + kSlots * kRows);       // [128] references
     float* mL = mR + kRows;                                        // [128] sums of weights
@@ -188,7 +191,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
     if (threadIdx.x == 0) {
         for (int s = 0; s < kRaw; s++) {
             mbar_init(&raw_full[s], 1);
-            mbar_init(&raw_empty[s], 8);
+            mbar_init(&raw_empty[s], 9);
         }
         for (int s = 0; s < kStages; s++) {
             mbar_init(&k_full[s], 4);
@@ -202,7 +205,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
             mbar_init(&p_empty[s], 1);
         }
         for (int s = 0; s < kSlots; s++) mbar_init(&al_full[s], 4);
-        for (int s = 0; s < 2 * kSlots; s++) mbar_init(&u_full[s], 1);
+        for (int s = 0; s < 2 * kUndo; s++) mbar_init(&u_full[s], 1);
         mbar_init(l_full, 4);
         mbar_init(o_full, 1);
         mbar_init(o_empty, 4);
@@ -321,54 +324,74 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                 }
                 if (i > 0) bar_wait(o_full, (uint32_t)(i - 1) & 1);
             }
+        } else {
+            // ---- what a tile's scales are multiplied by: those from 2^12 on would take fp16
+            // products past its range, and a tile of K or V that has one counts 2^-4 times ----
+            for (int i = 0, rs = 0, ph = 0; i < tiles; i++) {
+                wait(&raw_full[rs], ph);
+                const uint4* sc = reinterpret_cast<const uint4*>(smem + G::kRawOff + rs * G::kRawTile + 2 * kPos * RB);
+#pragma unroll
+                for (int kv = 0; kv < 2; kv++) {
+                    uint32_t mx = 0;
+#pragma unroll
+                    for (int e = lane; e < kPos * NB / 8; e += 32) {  // eight scales
+                        const uint4 v = sc[kv * (kPos * NB / 8) + e];
+                        const int n = min(8, (len - first_of(i)) * NB - 8 * e);  // (rows past the end hold anything)
+                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int k = 0; k < 4; k++) mx = __vmaxu2(mx, 2 * k < n ? w[k] & 0x7FFF7FFFu : 0u);
+                    }
+                    const bool big = __any_sync(0xffffffffu, max(mx & 0xFFFFu, mx >> 16) >= 0x6C00u);
+                    if (lane == 0) {
+                        undo[kUndo * kv + i % kUndo] = big ? 16.f : 1.f;
+                        mbar_arrive(&u_full[kUndo * kv + i % kUndo]);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&raw_empty[rs]);
+                if (++rs == kRaw) rs = 0, ph ^= 1;
+            }
         }
     } else if (warp >= 8) {
         // ---- expansion: K by warps 8-11, V by 12-15 ----
         const int tid = threadIdx.x & 127;
         const int kv = warp >= 12;
-        // scales from 2^12 on would take fp16 products past its range: a tile that
-        // has one counts 2^-4 times
-        auto shrink_of = [&](const uint8_t* raw, int i) {
-            uint32_t mx = 0;
-            for (int e = lane; e < kPos * NB / 2; e += 32) {
-                uint32_t v = reinterpret_cast<const uint32_t*>(raw + 2 * kPos * RB + kv * kPos * SB)[e];
-                if (first_of(i) + e / (NB / 2) >= len) v = 0;
-                mx = __vmaxu2(mx, v & 0x7FFF7FFFu);
-            }
-            const bool big = __any_sync(0xffffffffu, max(mx & 0xFFFFu, mx >> 16) >= 0x6C00u);
-            if (tid == 0) {
-                undo[kSlots * kv + i % kSlots] = big ? 16.f : 1.f;
-                mbar_arrive(&u_full[kSlots * kv + i % kSlots]);
-            }
-            return big ? 0x2C002C00u : 0x3C003C00u;
+        auto shrink_of = [&](int i) {  // (rows and their scales have landed)
+            wait(&u_full[kUndo * kv + i % kUndo], (uint32_t)(i / kUndo));
+            return undo[kUndo * kv + i % kUndo] == 1.f ? 0x3C003C00u : 0x2C002C00u;
+        };
+        // the next tile's places in the rings, and the parities of their barriers
+        auto step = [&](int& rs, int& ph, int& s, int& sp) {
+            if (++rs == kRaw) rs = 0, ph ^= 1;
+            if (++s == kStages) s = 0, sp ^= 1;
         };
         if (!kv) {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
             // position p, chunks 4 hf .. + 3 (each W 16-byte pieces)
             const int p = tid & 63, hf = tid >> 6;
-            for (int i = 0; i < tiles; i++) {
-                const int rs = i % kRaw, s = i % kStages;
+            for (int i = 0, rs = 0, ph = 0, s = 0, sp = 1; i < tiles; i++) {
                 const uint8_t* raw = smem + G::kRawOff + rs * G::kRawTile;
-                wait(&raw_full[rs], (uint32_t)(i / kRaw));
-                const uint32_t shrink = shrink_of(raw, i);
+                wait(&raw_full[rs], ph);
+                const uint32_t shrink = shrink_of(i);
                 const bool in = first_of(i) + p < len;
                 const uint32_t* sc = reinterpret_cast<const uint32_t*>(raw + 2 * kPos * RB + p * SB);
                 uint32_t d[W];
 #pragma unroll
                 for (int j = 0; j < W; j++) d[j] = in ? h2_mul(sc[j], shrink) : 0u;
-                if (i >= kStages) wait(&k_empty[s], (uint32_t)(i / kStages - 1));
-                uint8_t* stage = smem + s * G::kStage + p * 128;
+                if (i >= kStages) wait(&k_empty[s], sp);
 #pragma unroll 1
                 for (int j = 0; j < W; j++) {
                     const uint4 u = reinterpret_cast<const uint4*>(raw + p * RB + hf * (RB / 2))[j];
                     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+                    const int first16 = hf * 4 * W + 4 * j;  // the row's 16-byte pieces from here on (8 to a 64-wide part)
+                    uint8_t* stage = smem + s * G::kStage + (first16 >> 3) * (2 * kPos * 128) + p * 128;
+                    const int x = ((first16 & 7) ^ (p & 7)) << 4;
 #pragma unroll
                     for (int c = 0; c < 4; c++) {  // word c % W of chunk (4 j + c) / W of this half
                         uint32_t hi[4], lo[4];
 #pragma unroll
                         for (int e = 0; e < 4; e++) expand(w[c], e, d[c % W], hi[e], lo[e]);
-                        const int k16 = hf * 4 * W + 4 * j + c;  // 16-byte piece of the row, 8 to a 64-wide part
-                        uint8_t* t = stage + (k16 >> 3) * (2 * kPos * 128) + (((k16 & 7) ^ (p & 7)) << 4);
+                        uint8_t* t = stage + (x ^ (c << 4));
                         *reinterpret_cast<uint4*>(t) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                         *reinterpret_cast<uint4*>(t + kPos * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     }
@@ -379,6 +402,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                     mbar_arrive(&k_full[s]);
                     mbar_arrive(&raw_empty[rs]);
                 }
+                step(rs, ph, s, sp);
             }
         } else {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
@@ -387,11 +411,11 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
             const int gw = tid & (8 * W - 1), k = (tid / (8 * W)) & 7;
             constexpr int NI = 2 * W;  // nibbles a thread takes
             const int i0 = W == 2 ? 0 : (tid >> 6) * 2;
-            for (int i = 0; i < tiles; i++) {
-                const int rs = i % kRaw, s = i % kStages, first = first_of(i) + 8 * k;
+            for (int i = 0, rs = 0, ph = 0, s = 0, sp = 1; i < tiles; i++) {
+                const int first = first_of(i) + 8 * k;
                 const uint8_t* raw = smem + G::kRawOff + rs * G::kRawTile;
-                wait(&raw_full[rs], (uint32_t)(i / kRaw));
-                const uint32_t shrink = shrink_of(raw, i);
+                wait(&raw_full[rs], ph);
+                const uint32_t shrink = shrink_of(i);
                 const uint8_t* q = raw + kPos * RB + 8 * k * RB + 4 * gw;
                 const uint8_t* sc = raw + 2 * kPos * RB + kPos * SB + 8 * k * SB + 4 * (gw % W);
                 uint32_t w[8], d[8];
@@ -403,7 +427,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&raw_empty[rs]);
-                if (i >= kStages) wait(&v_empty[s], (uint32_t)(i / kStages - 1));
+                if (i >= kStages) wait(&v_empty[s], sp);
                 uint8_t* stage = smem + s * G::kStage + 2 * G::kTile;
 #pragma unroll 1
                 for (int pb = 0; pb < 2; pb++)
@@ -425,6 +449,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&v_full[s]);
+                step(rs, ph, s, sp);
             }
         }
     } else {
@@ -501,8 +526,8 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                     for (int e = 0; e < HD; e++) o[e] *= am;
                 }
                 wait(o_full, (uint32_t)i);
-                wait(&u_full[kSlots + i % kSlots], (uint32_t)(i / kSlots));
-                const float vm = undo[kSlots + i % kSlots];
+                wait(&u_full[kUndo + i % kUndo], (uint32_t)(i / kUndo));
+                const float vm = undo[kUndo + i % kUndo];
                 fence_after();
                 float t[2][16];
                 ld16(tmem + lane_off + G::kO, t[0]);
@@ -555,13 +580,13 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
             const int seen_by_all = p0 + r0 / mul + 1;
             for (int i = 0; i < tiles; i++) {
                 const int buf = i % kBufs, first = first_of(i);
-                wait(&u_full[i % kSlots], (uint32_t)(i / kSlots));
-                const float f = factor * undo[i % kSlots];
+                wait(&u_full[i % kUndo], (uint32_t)(i / kUndo));
+                const float f = factor * undo[i % kUndo];
                 wait(&s_full[buf], (uint32_t)(i / kBufs));
                 fence_after();
                 const uint32_t sc = tmem + lane_off + G::kS + buf * kPos;
                 const bool hide = first + kPos > seen_by_all;
-                float x[64], top = -INFINITY, move = 1.f;
+                float x[64], top = -INFINITY, top2 = -INFINITY, move = 1.f;
                 ld32(sc, x);
                 ld32(sc + 32, x + 32);
                 wait_ld();
@@ -571,7 +596,8 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                         if (first + e > limit) x[e] = -INFINITY;
                 }
 #pragma unroll
-                for (int e = 0; e < 64; e++) top = fmaxf(top, x[e]);
+                for (int e = 0; e < 32; e++) top = fmaxf(top, x[e]), top2 = fmaxf(top2, x[32 + e]);
+                top = fmaxf(top, top2);
                 if (top * f > R + (kPeak + kLazy)) {
                     const float to = top * f - kPeak;
                     move = ex2(R - to);
