@@ -55,6 +55,12 @@ struct Geo {
     static constexpr int NB = HD / 32, W = NB / 2;  // blocks; 32-bit words per chunk
     static constexpr int kTile = kPos * HD * 2;     // bytes of one fp16 K or V tile
     static constexpr int kStage = 4 * kTile;        // K (hi, lo of each 64-wide part), V hi, V lo
+    // rows of q, of the rope table and of the output in shared memory: 16 bytes
+    // apart in the banks.  q's and the table's lie where the first V tile and what
+    // follows it will; the output's (and a cluster's partials) where the first
+    // stages were.
+    static constexpr int kPitch = 4 * HD + 16, kQOff = 2 * kTile, kTabOff = kQOff + kRows * kPitch;
+    static_assert(kTabOff + kRows * kPitch <= kStages * kStage, "queries");
     static constexpr int kRawTile = kPos * 36 * NB;
     static constexpr int kRawOff = kStages * kStage;
     static constexpr int kBarOff = kRawOff + kRaw * kRawTile;
@@ -65,7 +71,7 @@ struct Geo {
     static constexpr int kS = 0, kO = kBufs * kPos, kQ = kO + HD;
     static constexpr int kCols = 512;
     static_assert(kQ + HD <= kCols, "tensor memory");
-    static_assert(8 * (2 * kRaw + 4 * kStages + 3 * kBufs + kSlots + 2 * kUndo + 4) + 8 + 8 * kUndo <= kRowOff - kBarOff, "barriers");
+    static_assert(8 * (2 * kRaw + 4 * kStages + 3 * kBufs + 2 * kUndo + 6) + 8 + 8 * kUndo <= kRowOff - kBarOff, "barriers");
     static_assert(kBarOff % 8 == 0 && kSmem <= 227 * 1024, "shared memory");
 };
 
@@ -98,6 +104,9 @@ __device__ __forceinline__ void ld16(uint32_t taddr, float* f) {
           "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
         : "r"(taddr)
         : "memory");
+}
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -159,17 +168,16 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
     uint64_t* s_full = v_empty + kStages;
     uint64_t* p_full = s_full + kBufs;
     uint64_t* p_empty = p_full + kBufs;
-    uint64_t* al_full = p_empty + kBufs;
-    uint64_t* o_full = al_full + kSlots;
-    uint64_t* o_empty = o_full + 1;
-    uint64_t* q_full = o_empty + 1;
+    uint64_t* o_full = p_empty + kBufs;  // [2]
+    uint64_t* o_empty = o_full + 2;      // [2]
+    uint64_t* q_full = o_empty + 2;
     uint64_t* l_full = q_full + 1;
     uint64_t* u_full = l_full + 1;  // [2][kUndo]
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(u_full + 2 * kUndo);
     float* undo = reinterpret_cast<float*>(tmem_holder + 2);  // [2][kUndo] what K's and V's tiles were scaled down by
     float* slots = reinterpret_cast<float*>(smem + G::kRowOff);    // [kSlots][128] what a tile multiplies the row's output by
-    float* mR = reinterpret_cast<float*>(slots + kSlots * kRows);       // [128] references
-    float* mL = mR + kRows;                                        // [128] sums of weights
+    float* mR = slots + kSlots * kRows;  // [128] the last references
+    float* mL = mR + kRows;              // [128] sums of weights
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t cs = cluster_size(), rank = cluster_rank();
 
@@ -188,28 +196,22 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
     const int64_t base = (int64_t)b * a.seq_rows + (int64_t)kvh * a.ctx_len;
     auto first_of = [&](int i) { return ((int)rank + i * (int)cs) * kPos; };
 
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < kRaw; s++) {
-            mbar_init(&raw_full[s], 1);
-            mbar_init(&raw_empty[s], 9);
-        }
-        for (int s = 0; s < kStages; s++) {
-            mbar_init(&k_full[s], 4);
-            mbar_init(&v_full[s], 4);
-            mbar_init(&k_empty[s], 1);
-            mbar_init(&v_empty[s], 1);
-        }
-        for (int s = 0; s < kBufs; s++) {
-            mbar_init(&s_full[s], 1);
-            mbar_init(&p_full[s], 4);
-            mbar_init(&p_empty[s], 1);
-        }
-        for (int s = 0; s < kSlots; s++) mbar_init(&al_full[s], 4);
-        for (int s = 0; s < 2 * kUndo; s++) mbar_init(&u_full[s], 1);
-        mbar_init(l_full, 4);
-        mbar_init(o_full, 1);
-        mbar_init(o_empty, 4);
-        mbar_init(q_full, 4);
+    if (warp == 0) {
+        auto init = [&](uint64_t* bars, int n, int count) {
+            if (lane < n) mbar_init(&bars[lane], count);
+        };
+        init(raw_full, kRaw, 1);
+        init(raw_empty, kRaw, 9);
+        init(k_full, 2 * kStages, 4);   // and v_full
+        init(k_empty, 2 * kStages, 1);  // and v_empty
+        init(s_full, kBufs, 1);
+        init(p_full, kBufs, 4);
+        init(p_empty, kBufs, 1);
+        init(o_full, 2, 1);
+        init(o_empty, 2, 4);
+        init(q_full, 1, 4);
+        init(l_full, 1, 4);
+        init(u_full, 2 * kUndo, 1);
         fence_mbar_init();
     }
     if (warp == 16) {
@@ -217,6 +219,21 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                      "r"(G::kCols)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // the rows' queries and their rows of the rope table, a row at a time: on their way
+    const int tok0 = r0 / mul;
+    if (warp >= 4 && warp < 8) {
+        constexpr int kLanes = HD / 4;  // threads to a row
+        const int k0 = (threadIdx.x & 127) / kLanes, e = threadIdx.x % kLanes;
+        const float* q = a.q + (int64_t)b * a.n_new * a.q_stride + (int64_t)kvh * mul * HD + 4 * e;
+        int tok = (r0 + k0) / mul, head = (r0 + k0) % mul;
+        for (int k = k0; k < rows; k += kRows / kLanes) {
+            copy16(smem + G::kQOff + k * G::kPitch + 16 * e, q + tok * a.q_stride + head * HD);
+            for (head += kRows / kLanes; head >= mul; head -= mul) tok++;
+        }
+        if (a.rope)
+            for (int k = k0; k <= (r0 + rows - 1) / mul - tok0; k += kRows / kLanes)
+                copy16(smem + G::kTabOff + k * G::kPitch + 16 * e, a.rope + (int64_t)(p0 + tok0 + k) * (HD / 2) + 2 * e);
     }
     fence_before();
     __syncthreads();
@@ -229,10 +246,6 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
             atomicOr(a.err, kErrTimeout);
         }
     };
-
-    // the cluster's partials: each CTA leaves its rows in its own shared memory, in
-    // the place of its first K and V tiles, once its last output is there
-    float* mine = reinterpret_cast<float*>(smem);  // [HD][128]
 
     // Registers: 96 a thread at launch (480 for the five groups of four warps);
     // 112 + 184 + 64 + 80 + 32 = 472 once the last three have given theirs up.
@@ -298,31 +311,37 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                 // (whoever gave up, no MMA outlives its tensor memory)
                 if (i > 0) bar_wait(&s_full[(i - 1) % kBufs], (uint32_t)((i - 1) / kBufs) & 1);
             } else {
-                constexpr uint32_t kN = idesc(HD);
+                constexpr uint32_t kN = idesc(HD / 2);
                 for (; i < count; i++) {
                     const int s = i % kStages, buf = i % kBufs;
                     wait(&v_full[s], (uint32_t)(i / kStages));
                     wait(&p_full[buf], (uint32_t)(i / kBufs));
-                    if (i > 0) wait(o_empty, (uint32_t)(i - 1));
+                    // the output in halves: one is read while the other is computed
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        if (i > 0) wait(&o_empty[h], (uint32_t)(i - 1));
+                        if (!__all_sync(0xffffffffu, ok)) break;
+                        fence_after();
+                        const uint64_t vt = desc(smem_u32(smem + s * G::kStage + 2 * G::kTile)) + h * (HD / 2 * 128 / 16);
+                        const uint32_t d = tm + G::kO + h * (HD / 2), p = tm + G::kS + buf * kPos;
+#pragma unroll
+                        for (int m = 0; m < 3; m++)
+#pragma unroll
+                            for (int kk = 0; kk < kPos / 16; kk++)
+                                if (lead)
+                                    mma_ts(d, p + 16 * kk + (m == 0 ? 8 : 0), vt + (m == 1 ? G::kTile / 16 : 0) + 2 * kk, kN,
+                                           m + kk != 0);
+                        if (lead) commit(&o_full[h]);
+                    }
                     if (!__all_sync(0xffffffffu, ok)) break;
-                    fence_after();
-                    const uint64_t vt = desc(smem_u32(smem + s * G::kStage + 2 * G::kTile));
-                    const uint32_t d = tm + G::kO, p = tm + G::kS + buf * kPos;
-#pragma unroll
-                    for (int m = 0; m < 3; m++)
-#pragma unroll
-                        for (int kk = 0; kk < kPos / 16; kk++)
-                            if (lead)
-                                mma_ts(d, p + 16 * kk + (m == 0 ? 8 : 0), vt + (m == 1 ? G::kTile / 16 : 0) + 2 * kk, kN,
-                                       m + kk != 0);
                     if (lead) {
-                        commit(o_full);
                         commit(&v_empty[s]);
                         commit(&p_empty[buf]);
                     }
                     __syncwarp();
                 }
-                if (i > 0) bar_wait(o_full, (uint32_t)(i - 1) & 1);
+                if (i > 0) bar_wait(&o_full[1], (uint32_t)(i - 1) & 1);
+                if (i < count) bar_wait(&o_full[0], (uint32_t)i & 1);
             }
         } else {
             // ---- what a tile's scales are multiplied by: those from 2^12 on would take fp16
@@ -378,6 +397,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                 uint32_t d[W];
 #pragma unroll
                 for (int j = 0; j < W; j++) d[j] = in ? h2_mul(sc[j], shrink) : 0u;
+                if (i == 1) wait(q_full, 0);  // (the queries lay there)
                 if (i >= kStages) wait(&k_empty[s], sp);
 #pragma unroll 1
                 for (int j = 0; j < W; j++) {
@@ -427,6 +447,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&raw_empty[rs]);
+                if (i == 0) wait(q_full, 0);
                 if (i >= kStages) wait(&v_empty[s], sp);
                 uint8_t* stage = smem + s * G::kStage + 2 * G::kTile;
 #pragma unroll 1
@@ -462,14 +483,16 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
             float o[HD];
             {
                 // first the row's query: rotated, scaled to [2^14, 2^15), in K's order
-                const float* x = a.q + ((int64_t)b * a.n_new + tok) * a.q_stride + (int64_t)(kvh * mul + rr % mul) * HD;
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                const uint8_t* x = smem + G::kQOff + min(r, rows - 1) * G::kPitch;
 #pragma unroll
                 for (int e = 0; e < HD / 4; e++) {
                     const float4 v = reinterpret_cast<const float4*>(x)[e];
                     o[4 * e] = v.x, o[4 * e + 1] = v.y, o[4 * e + 2] = v.z, o[4 * e + 3] = v.w;
                 }
                 if (a.rope) {
-                    const float4* tab = reinterpret_cast<const float4*>(a.rope + (int64_t)(p0 + tok) * (HD / 2));
+                    const float4* tab = reinterpret_cast<const float4*>(smem + G::kTabOff + (tok - tok0) * G::kPitch);
                     auto turn = [](float& u, float& v, float c, float s) {
                         const float t = __fsub_rn(__fmul_rn(u, c), __fmul_rn(v, s));
                         v = __fadd_rn(__fmul_rn(u, s), __fmul_rn(v, c));
@@ -495,7 +518,8 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
 #pragma unroll
                 for (int e = 0; e < HD; e++) amax = fmaxf(amax, fabsf(o[e]));
                 row_pow2_scale(amax, sc, inv);
-                mR[r] = fmaxf(a.scale * 1.44269504088896341f * inv, FLT_MIN);  // what a score counts, for the weights' warps (not 0: -inf is a masked score)
+                // what a score counts, for the weights' warps (not 0: -inf is a masked score)
+                mR[r] = fmaxf(a.scale * 1.44269504088896341f * inv, FLT_MIN);
 #pragma unroll
                 for (int c = 0; c < HD / 32; c++) {  // 32 dimensions: four pieces of 8
                     uint32_t hi[16], lo[16];
@@ -519,55 +543,64 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
 #pragma unroll
             for (int e = 0; e < HD; e++) o[e] = 0.f;
             for (int i = 0; i < tiles; i++) {
-                wait(&al_full[i % kSlots], (uint32_t)(i / kSlots));
-                const float am = slots[(i % kSlots) * kRows + r];
-                if (!__all_sync(0xffffffffu, am == 1.f)) {
+                float up = 1.f, vm = 1.f;
 #pragma unroll
-                    for (int e = 0; e < HD; e++) o[e] *= am;
-                }
-                wait(o_full, (uint32_t)i);
-                wait(&u_full[kUndo + i % kUndo], (uint32_t)(i / kUndo));
-                const float vm = undo[kUndo + i % kUndo];
-                fence_after();
-                float t[2][16];
-                ld16(tmem + lane_off + G::kO, t[0]);
-#pragma unroll
-                for (int c = 0; c < HD / 16; c++) {
-                    wait_ld();
-                    if (c + 1 < HD / 16) ld16(tmem + lane_off + G::kO + 16 * (c + 1), t[(c + 1) & 1]);
-                    else {
-                        fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(o_empty);
+                for (int h = 0; h < 2; h++) {
+                    wait(&o_full[h], (uint32_t)i);
+                    fence_after();
+                    if (h == 0) {  // (the tile's words are there: the product came after them)
+                        up = slots[(i % kSlots) * kRows + r];
+                        vm = undo[kUndo + i % kUndo];
                     }
-                    const float* x = t[c & 1];
+                    float t[2][16];
+                    const uint32_t col = tmem + lane_off + G::kO + h * (HD / 2);
+                    ld16(col, t[0]);
+                    if (!__all_sync(0xffffffffu, up == 1.f)) {
 #pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        const float2 v = fma2(make_float2(x[e], x[e + 1]), make_float2(vm, vm),
-                                              make_float2(o[16 * c + e], o[16 * c + e + 1]));
-                        o[16 * c + e] = v.x, o[16 * c + e + 1] = v.y;
+                        for (int e = 0; e < HD / 2; e++) o[h * (HD / 2) + e] *= up;
+                    }
+#pragma unroll
+                    for (int c = 0; c < HD / 32; c++) {
+                        wait_ld();
+                        if (c + 1 < HD / 32) ld16(col + 16 * (c + 1), t[(c + 1) & 1]);
+                        else {
+                            fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&o_empty[h]);
+                        }
+                        const float* x = t[c & 1];
+                        float* y = o + h * (HD / 2) + 16 * c;
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) {
+                            const float2 v = fma2(make_float2(x[e], x[e + 1]), make_float2(vm, vm), make_float2(y[e], y[e + 1]));
+                            y[e] = v.x, y[e + 1] = v.y;
+                        }
                     }
                 }
             }
-            if (cs > 1) {
+            wait(l_full, 0);
+            const float inv = cs > 1 ? 1.f : 1.f / mL[r];
+            uint8_t* row = smem + r * G::kPitch;
 #pragma unroll
-                for (int e = 0; e < HD; e++) mine[e * kRows + r] = o[e];
-            } else {
-                wait(l_full, 0);
-                if (r < rows) {
-                    float* dst =
-                        a.out + ((int64_t)b * a.n_new + tok) * a.out_stride + (int64_t)(kvh * mul + rr % mul) * HD;
-                    const float inv = 1.f / mL[r];
+            for (int m = 0; m < HD / 4; m++) {
+                float v[4];
 #pragma unroll
-                    for (int m = 0; m < HD / 4; m++) {
-                        float v[4];
-#pragma unroll
-                        for (int u = 0; u < 4; u++) {
-                            const int e = 4 * m + u, bl = e / 32, i = (e / 8) % 4, g = e % 8;
-                            v[u] = o[((bl & 1) * 4 + i) * (8 * W) + g * W + (bl >> 1)] * inv;
-                        }
-                        *reinterpret_cast<float4*>(dst + 4 * m) = make_float4(v[0], v[1], v[2], v[3]);
-                    }
+                for (int u = 0; u < 4; u++) {
+                    const int e = 4 * m + u, bl = e / 32, i = (e / 8) % 4, g = e % 8;
+                    v[u] = o[((bl & 1) * 4 + i) * (8 * W) + g * W + (bl >> 1)] * inv;
+                }
+                *reinterpret_cast<float4*>(row + 16 * m) = make_float4(v[0], v[1], v[2], v[3]);
+            }
+            if (cs == 1) {  // a row at a time
+                constexpr int kLanes = HD / 4;
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                const int k0 = r / kLanes, e = r % kLanes;
+                float* dst = a.out + (int64_t)b * a.n_new * a.out_stride + (int64_t)kvh * mul * HD + 4 * e;
+                int t = (r0 + k0) / mul, head = (r0 + k0) % mul;
+                for (int k = k0; k < rows; k += kRows / kLanes) {
+                    *reinterpret_cast<float4*>(dst + t * a.out_stride + head * HD) =
+                        *reinterpret_cast<const float4*>(smem + k * G::kPitch + 16 * e);
+                    for (head += kRows / kLanes; head >= mul; head -= mul) t++;
                 }
             }
         } else {
@@ -578,17 +611,21 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
             wait(q_full, 0);
             const float factor = mR[r];
             const int seen_by_all = p0 + r0 / mul + 1;
-            for (int i = 0; i < tiles; i++) {
-                const int buf = i % kBufs, first = first_of(i);
-                wait(&u_full[i % kUndo], (uint32_t)(i / kUndo));
-                const float f = factor * undo[i % kUndo];
-                wait(&s_full[buf], (uint32_t)(i / kBufs));
+            float x[64];  // a tile's scores, on their way while the last tile's weights are stored
+            auto fetch = [&](int i) {
+                wait(&s_full[i % kBufs], (uint32_t)(i / kBufs));
                 fence_after();
-                const uint32_t sc = tmem + lane_off + G::kS + buf * kPos;
-                const bool hide = first + kPos > seen_by_all;
-                float x[64], top = -INFINITY, top2 = -INFINITY, move = 1.f;
+                const uint32_t sc = tmem + lane_off + G::kS + (i % kBufs) * kPos;
                 ld32(sc, x);
                 ld32(sc + 32, x + 32);
+            };
+            if (tiles > 0) fetch(0);
+            for (int i = 0; i < tiles; i++) {
+                const int buf = i % kBufs, first = first_of(i);
+                const uint32_t sc = tmem + lane_off + G::kS + buf * kPos;
+                const float f = factor * undo[i % kUndo];  // (there since before K was expanded)
+                const bool hide = first + kPos > seen_by_all;
+                float top = -INFINITY, top2 = -INFINITY, move = 1.f;
                 wait_ld();
                 if (hide) {
 #pragma unroll
@@ -620,13 +657,11 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
                 const float sum = part.x + part.y;
                 l = l * move + sum;
                 slots[(i % kSlots) * kRows + r] = move;
+                if (i + 1 < tiles) fetch(i + 1);
                 wait_st();
                 fence_before();
                 __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&p_full[buf]);
-                    mbar_arrive(&al_full[i % kSlots]);
-                }
+                if (lane == 0) mbar_arrive(&p_full[buf]);
             }
             mR[r] = R;
             mL[r] = l;
@@ -644,21 +679,23 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
         // the partials meet, each CTA adding up a share
         cluster_arrive();
         cluster_wait();
-        const uint32_t aO = smem_u32(mine), aR = smem_u32(mR), aL = smem_u32(mL);
-        for (int e = (int)rank * kThreads + threadIdx.x; e < HD * kRows; e += (int)cs * kThreads) {
-            const int r = e % kRows, nn = e / kRows;
-            if (r >= rows) continue;
-            float M = -1e30f, v = 0.f, ls = 0.f;
+        const uint32_t aO = smem_u32(smem), aR = smem_u32(mR), aL = smem_u32(mL);
+        for (int e = (int)rank * kThreads + threadIdx.x; e < rows * (HD / 4); e += (int)cs * kThreads) {
+            const int r = e / (HD / 4), at = r * G::kPitch + 16 * (e % (HD / 4)), rr = r0 + r;
+            float M = -1e30f, ls = 0.f;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             for (uint32_t c = 0; c < cs; c++) M = fmaxf(M, ld_cluster(aR + 4 * r, c));
             for (uint32_t c = 0; c < cs; c++) {
                 const float f = ex2(ld_cluster(aR + 4 * r, c) - M);
-                v = fmaf(f, ld_cluster(aO + 4 * e, c), v);
+                const float4 x = ld_cluster4(aO + at, c);
+                v.x = fmaf(f, x.x, v.x);
+                v.y = fmaf(f, x.y, v.y);
+                v.z = fmaf(f, x.z, v.z);
+                v.w = fmaf(f, x.w, v.w);
                 ls = fmaf(f, ld_cluster(aL + 4 * r, c), ls);
             }
-            const int hb = nn / (8 * W), lw = nn % (8 * W);
-            const int dim = 32 * (2 * (lw % W) + hb / 4) + 8 * (hb % 4) + lw / W;
-            const int rr = r0 + r;
-            a.out[((int64_t)b * a.n_new + rr / mul) * a.out_stride + (int64_t)(kvh * mul + rr % mul) * HD + dim] = v / ls;
+            float* dst = a.out + ((int64_t)b * a.n_new + rr / mul) * a.out_stride + (int64_t)(kvh * mul + rr % mul) * HD;
+            reinterpret_cast<float4*>(dst)[e % (HD / 4)] = make_float4(v.x / ls, v.y / ls, v.z / ls, v.w / ls);
         }
         __syncwarp();
         cluster_arrive();
