@@ -3,8 +3,9 @@
 //
 // A CTA takes 128 rows (tokens x the query heads of one kv head) and walks the
 // cache in tiles of 64 positions, K and V expanded from nibbles to fp16:
-//   S = Q K^T:  Q [128 rows][hd] and K [64 positions][hd] in shared memory;
-//   O = P V:    P [128 rows][64 positions] in tensor memory, V [hd][64 positions].
+//   S = Q K^T:  Q [128 rows][hd] in tensor memory, K [64 positions][hd] in shared;
+//   O = P V:    P [128 rows][64 positions] in tensor memory (in the scores' place),
+//               V [hd][64 positions] in shared.
 // Precision: q, k, v and the weights are pairs of fp16 halves (q and the weights to
 // 22 bits; k and v, 15-bit products of a level and a scale, exactly), three MMAs each
 // (lo hi + hi lo, then hi hi: the tensor cores truncate as they add, and lose less
@@ -12,16 +13,19 @@
 // the same reason; that also leaves nothing to rescale in tensor memory.  A row's
 // reference moves only when outgrown by 2^4.
 //
-// Bound: for a tile and hd = 128 the MMAs take 1900 cycles (6 x 64 columns x 128 x
-// 128), the weights of 128 rows about as many instruction slots, the expansion half.
-// So each has warps of its own, three tiles are between their scores and their
-// output, and a tile takes 2700 cycles: what is left is the way of one tile through
-// all of them (K 600, S 950, weights 2100, O 950), two thirds covered.  Weights by eight
-// warps (half the registers each) took 867 us for the 1111 rows at 6000 below
-// instead of 641, P in shared memory 982, MMA loops unrolled (code beyond the
-// instruction caches) 864.  64 query heads over 8, hd 128, 1111 tokens at position
-// 6000: 645 us, 370 TFLOP/s
-// of the formula's 4 hd a pair, three times that as multiplied; 512 tokens at 0: 27.6 us.
+// Bound: the tensor cores.  For a tile and hd = 128 they take 1590 cycles alone (48
+// MMAs of 128 x 64 x 16 at 33) and 1880 next to the loads and stores of tensor memory;
+// a tile takes 2030.  The rest must hide behind them, so each step has warps of its
+// own (the instruction slots are 70 % full), four tiles are between their scores and
+// their output, three expanded, and the output comes in halves, one read while the
+// other is computed.  What it took, 64 query heads over 8 of hd 128, 1111 tokens at
+// position 6000: 507 us, 471 TFLOP/s of the formula's 4 hd a pair, three times that
+// as multiplied.  MMAs issued by a thread by itself, 84 cycles each: 831.  So with Q
+// in shared memory and wide MMAs, fewer to issue: 641.  P in shared memory: 982.
+// Weights by eight warps on alternate tiles: 547.
+// A CTA's first output comes 16600 cycles after its start, most of them the first
+// pass through code that is in no instruction cache yet, and writing it takes 4000:
+// 512 tokens at 0 take 24 us, of which their eight tiles are 9.
 //
 // Order of K's dimensions (any will do, if Q has the same) and V's rows (undone on
 // the way out) follow the nibbles: K position kappa of a 64-wide half is
@@ -708,7 +712,7 @@ bool kvq4_prompt_ok(int hd) { return hd == 64 || hd == 128; }
 int64_t kvq4_prompt_items(int64_t rows, int n_kv, int batch) { return (rows + pr::kRows - 1) / pr::kRows * n_kv * batch; }
 
 // CTAs per item: as many as the SMs hold (one each), four tiles for each at least
-// (64 query heads over 8, 16 tokens at 30000: 108 us with 8 CTAs, 170 by the
+// (64 query heads over 8, 16 tokens at 30000: 81 us with 8 CTAs, 170 by the
 // kernel for few rows)
 int kvq4_prompt_cluster(const cn_ctx* ctx, int64_t items, int ctx_len) {
     int k = 1;
