@@ -255,8 +255,8 @@ int cn_matvec_noalloc_status(void* stream);
  * sequence has.  A sequence with a negative position or no tokens, and tokens
  * past the cache's end, are left out: their cache rows and output rows stay
  * as they were.  Tensors are [batch][n_new] rows of the given stride
- * (in values).  d_rope (may be NULL) is a [ctx_len][head_dim/2] table of
- * (cos, sin) as ApplyRoPE uses it (TensorMath.cs:418-470), rope_neox = 1 pairs
+ * (in values).  d_rope (may be NULL) is a 16-byte aligned [ctx_len][head_dim/2]
+ * table of (cos, sin) as ApplyRoPE uses it (TensorMath.cs:418-470), rope_neox = 1 pairs
  * (i, i + head_dim/2) (TensorMath.cs:475).  The calls run on ctx's device,
  * enqueue on `stream` only, allocate nothing and keep nothing between calls,
  * so they may be captured, replayed and issued from several streams; all
@@ -285,8 +285,8 @@ int cn_kvq4_append_dev(cn_ctx* ctx, const cn_kvq4* cache, const float* d_k, cons
  * . v_p, query head h on kv head h / (n_heads / n_kv_heads) (ComputeAttention +
  * Softmax, LlamaModel.cs:241-346).  q (rotated first when d_rope is given) and
  * out: n_heads * head_dim fp32 values per token, strides multiples of 4, not
- * overlapping; q, out and d_rope 16-byte aligned.  fp32 results (products of q and of the
- * softmax weights carry 22 bits, sums 24). */
+ * overlapping, 16-byte aligned.  fp32 results (products of q and of the softmax
+ * weights carry 22 bits, sums 24). */
 int cn_kvq4_attend_dev(cn_ctx* ctx, const cn_kvq4* cache, const float* d_q, int64_t q_stride, float* d_out,
                        int64_t out_stride, const int* d_pos, const int* d_count, int batch, int n_new, int n_heads,
                        float scale, const float* d_rope, int rope_neox, void* stream);
@@ -304,8 +304,8 @@ int cn_kvq4_read_dev(cn_ctx* ctx, const cn_kvq4* cache, float* d_k, float* d_v, 
  * together; each output but d_top_ids (with top_n > 0) may be NULL.  A token
  * outside [0, vocab) gets NaN.  -inf logits (banned tokens) have probability
  * 0; a row that holds a NaN or +inf, or nothing but -inf, has no distribution:
- * its results are NaN (its alternatives still in order, NaN last).  Enqueues
- * on `stream` only, allocates nothing, keeps nothing between calls.  (no
+ * its results are NaN (its alternatives still in order, NaN last).  vocab is
+ * below 2^30, row_stride below 2^40.  Enqueues on `stream` only, allocates nothing, keeps nothing between calls.  (no
  * reference counterpart: TemperatureSampler discards its probabilities,
  * Samplers/TemperatureSampler.cs:33-113) */
 int cn_logprobs_dev(cn_ctx* ctx, int type, const void* d_logits, int64_t row_stride, int rows, int vocab,
