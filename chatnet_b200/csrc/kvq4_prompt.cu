@@ -25,7 +25,7 @@
 // Weights by eight warps on alternate tiles: 547.
 // A CTA's first output comes 16600 cycles after its start, most of them the first
 // pass through code that is in no instruction cache yet, and writing it takes 4000:
-// 512 tokens at 0 take 24 us, of which their eight tiles are 9.
+// 512 tokens at 0 (32 heads) take 24 us, of which their eight tiles are 9.
 //
 // Order of K's dimensions (any will do, if Q has the same) and V's rows (undone on
 // the way out) follow the nibbles: K position kappa of a 64-wide half is

@@ -18,6 +18,11 @@
 // A row is split over a cluster of CTAs when there are few rows; their sums and
 // lists meet in the first CTA's shared memory.  No workspace, no atomics on
 // global memory, one launch.
+//
+// 4096 rows of 32000 fp32: 87 us, 6.0 TB/s (0.93 of a copy's rate).  300 rows of
+// 131071 fp16 with 8 alternatives: 39 us, 2.0 TB/s, bound by the instructions of twice
+// the values a byte.  Few rows are bound by the choice among the candidates, about
+// 5 us: one row of 32000 with 5 takes 7 us, 32 with 20 10.6.
 #include <float.h>
 
 #include "cn_common.cuh"

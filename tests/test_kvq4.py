@@ -105,7 +105,8 @@ def test_bad_reads_are_refused(bad):
                                  dict(heads=-2), dict(qs=252), dict(qs=258), dict(os=128), dict(q=_P + 4),
                                  dict(out=_P + 8), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
                                  dict(scale=float("inf")), dict(batch=0), dict(batch=5), dict(n_new=65),
-                                 dict(neox=-1), dict(rope=_P + 4)])
+                                 dict(neox=-1), dict(rope=_P + 4),
+                                 dict(heads=1 << 26, n_new=64, qs=1 << 33, os=1 << 33)])
 def test_bad_attends_are_refused(bad):
     assert _attend(**bad) == INVALID
 
