@@ -35,7 +35,8 @@ struct cn_ctx {
     void* samp = nullptr;
     size_t samp_bytes = 0;
 
-    // 4-bit attention kernels (by head_dim / 32) whose launch attributes are set
+    // kernels whose launch attributes are set: bits 1-8 4-bit attention for few rows
+    // (head_dim / 32), 16-19 log probabilities, 24-25 4-bit attention for many rows
     uint32_t kvq4_ready = 0;
 
     // staging for the host-pointer entry points

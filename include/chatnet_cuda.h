@@ -443,7 +443,8 @@ int cn_llama_logprobs(cn_llama* m, int batch, const int* tokens, int top_n, floa
  * tokens[t + 1] after tokens[0..t] to logprob_host[t] and the entropy of that
  * prediction to entropy_host[t] (may be NULL).  exp(-mean) is the text's
  * perplexity.  As cn_llama_forward, one prefill pass where the model and the
- * threshold allow, else one decode step per token.  (no reference
+ * threshold allow, else one decode step per token; which logits it leaves to
+ * cn_llama_sample and cn_llama_logprobs is not defined.  (no reference
  * counterpart) */
 int cn_llama_score(cn_llama* m, const int* tokens, int n, int pos, float* logprob_host, float* entropy_host);
 /* Kernel launches one decode step makes for `batch` (nodes of its graph). */
