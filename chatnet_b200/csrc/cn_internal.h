@@ -38,6 +38,7 @@ struct cn_ctx {
     // kernels whose launch attributes are set: bits 1-8 4-bit attention for few rows
     // (head_dim / 32), 16-19 log probabilities, 24-25 4-bit attention for many rows
     uint32_t kvq4_ready = 0;
+    int kvq4_fit[2][4] = {};  // clusters of 1, 2, 4 and 8 of the latter that run at once (head_dim 64, 128)
 
     // staging for the host-pointer entry points
     void* dstage = nullptr;

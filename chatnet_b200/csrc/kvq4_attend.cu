@@ -596,18 +596,16 @@ int kvq4_attend(cn_ctx* ctx, const cn_kvq4& c, const float* q, int64_t q_stride,
     const int64_t room = (int64_t)ctx->sms * ctas_per_sm(nb);
     if (kvq4_prompt_ok(c.head_dim)) {
         // Which kernel: both as measured over the cache's length (the positions are
-        // on the device), in ns.  Here: 6 us for each round of CTAs and 23 positions
-        // of 128 values a ns.  There: 12 us, 5 more for clusters, 1.08 us a tile of
-        // 64 x 128 values.  One sequence, 64 heads over 8 of 128, 8 x tokens rows,
-        // here / there: at 2000 positions 64 rows 16 / 20 us, 192 rows 27 / 24; at
-        // 16000 64 rows 53 / 49, 96 rows 73 / 50, 192 rows 136 / 97.  Four sequences
-        // of 32 heads, 64 rows: at 100 29 / 16, at 2000 100 / 50, at 16000 540 / 287.
-        const int64_t there = kvq4_prompt_items(rows, c.n_kv_heads, batch);
-        const int k = kvq4_prompt_cluster(ctx, there, c.ctx_len);
-        const double rounds = (double)((there * k + ctx->sms - 1) / ctx->sms);
-        const double t_there = (k > 1 ? 17e3 : 12e3) + rounds * ((c.ctx_len / 64 + k - 1) / k) * 8.4 * c.head_dim;
-        const double t_here = 6e3 * (double)((items + room - 1) / room) + (double)items * c.ctx_len * c.head_dim / 2944.;
-        if (t_there < t_here) return kvq4_attend_prompt(ctx, c.head_dim, a, st);
+        // on the device).  Here: 6 us for each round of CTAs and 23 positions of 128
+        // values a ns.  One sequence, 64 heads over 8 of 128, 8 x tokens rows, here /
+        // there: at 2000 positions 64 rows 16 / 20 us, 192 rows 27 / 24; at 16000 64
+        // rows 53 / 49, 96 rows 73 / 50, 192 rows 136 / 97.  Four sequences of 32
+        // heads, 64 rows: at 100 29 / 16, at 2000 100 / 50, at 16000 540 / 287.
+        int k, rc;
+        double there = 0;
+        if ((rc = kvq4_prompt_plan(ctx, rows, c.n_kv_heads, batch, c.head_dim, c.ctx_len, &k, &there))) return rc;
+        const double here = 6e3 * (double)((items + room - 1) / room) + (double)items * c.ctx_len * c.head_dim / 2944.;
+        if (there < here) return kvq4_attend_prompt(ctx, c.head_dim, k, a, st);
     }
     a.groups = (int)groups;
     // CTAs per item: the most that all run at once (8 x 64 heads of 128 at 131

@@ -23,9 +23,8 @@ struct AttendArgs {
 
 // Many rows: items of 128, head dimensions kvq4_prompt_ok.
 bool kvq4_prompt_ok(int hd);
-int64_t kvq4_prompt_items(int64_t rows, int n_kv, int batch);
-int kvq4_prompt_cluster(const cn_ctx* ctx, int64_t items, int ctx_len);
-int kvq4_attend_prompt(cn_ctx* ctx, int hd, AttendArgs a, cudaStream_t st);
+int kvq4_prompt_plan(cn_ctx* ctx, int64_t rows, int n_kv, int batch, int hd, int ctx_len, int* cluster, double* time);
+int kvq4_attend_prompt(cn_ctx* ctx, int hd, int cluster, AttendArgs a, cudaStream_t st);
 
 // mbar_wait as a short loop (the kernels wait in many places, and code beyond the
 // instruction caches costs more than the waits).

@@ -709,32 +709,63 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
 
 bool kvq4_prompt_ok(int hd) { return hd == 64 || hd == 128; }
 
-int64_t kvq4_prompt_items(int64_t rows, int n_kv, int batch) { return (rows + pr::kRows - 1) / pr::kRows * n_kv * batch; }
-
-// CTAs per item: as many as the SMs hold (one each), four tiles for each at least
-// (64 query heads over 8, 16 tokens at 30000: 81 us with 8 CTAs, 170 by the
-// kernel for few rows)
-int kvq4_prompt_cluster(const cn_ctx* ctx, int64_t items, int ctx_len) {
-    int k = 1;
-    while (k < pr::kMaxCluster && 2 * k * items <= ctx->sms && 2 * k * 4 * pr::kPos <= ctx_len) k *= 2;
-    return k;
+using PromptFn = void (*)(AttendArgs);
+static PromptFn prompt_fn(int hd) { return hd == 64 ? kvq4_attend_prompt_kernel<64> : kvq4_attend_prompt_kernel<128>; }
+static int prompt_smem(int hd) { return hd == 64 ? pr::Geo<64>::kSmem : pr::Geo<128>::kSmem; }
+static int64_t prompt_items(int64_t rows, int n_kv, int batch) {
+    return (rows + pr::kRows - 1) / pr::kRows * n_kv * batch;
 }
 
-int kvq4_attend_prompt(cn_ctx* ctx, int hd, AttendArgs a, cudaStream_t st) {
+// The time in ns that a call takes over the cache's length, and the CTAs per item for
+// which it is shortest (four tiles for each at least): per round of clusters 12 us, 5
+// more above one CTA, and 1.08 us a tile of 64 x 128 values.  64 query heads over 8:
+// 16 tokens at 30000 80 us with 8 CTAs, 170 by the kernel for few rows; 296 at 6000
+// (152 items on 148 SMs) 195 us with 2, 227 with one.
+int kvq4_prompt_plan(cn_ctx* ctx, int64_t rows, int n_kv, int batch, int hd, int ctx_len, int* cluster, double* time) {
+    int* fit = ctx->kvq4_fit[hd == 128];
+    const uint32_t bit = 1u << (hd == 64 ? 24 : 25);
+    if (!(__atomic_load_n(&ctx->kvq4_ready, __ATOMIC_ACQUIRE) & bit)) {
+        const PromptFn fn = prompt_fn(hd);
+        CN_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, prompt_smem(hd)));
+        for (int i = 0; i < 4; i++) {
+            cudaLaunchAttribute at = {};
+            at.id = cudaLaunchAttributeClusterDimension;
+            at.val.clusterDim.x = 1u << i;
+            at.val.clusterDim.y = at.val.clusterDim.z = 1;
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3((unsigned)(ctx->sms + 7) / 8 * 8);
+            cfg.blockDim = dim3(pr::kThreads);
+            cfg.dynamicSmemBytes = (size_t)prompt_smem(hd);
+            cfg.attrs = &at;
+            cfg.numAttrs = 1;
+            int n = 0;
+            CN_CUDA(cudaOccupancyMaxActiveClusters(&n, fn, &cfg));
+            __atomic_store_n(&fit[i], n, __ATOMIC_RELAXED);
+        }
+        __atomic_fetch_or(&ctx->kvq4_ready, bit, __ATOMIC_RELEASE);
+    }
+    const int64_t items = prompt_items(rows, n_kv, batch), tiles = (ctx_len + pr::kPos - 1) / pr::kPos;
+    *cluster = 0;
+    for (int i = 0, k = 1; k <= pr::kMaxCluster && (k == 1 || 4 * k <= tiles); i++, k *= 2) {
+        const int n = __atomic_load_n(&fit[i], __ATOMIC_RELAXED);
+        if (k > 1 && n < 1) continue;
+        const double t = (double)((items + n - 1) / (n > 0 ? n : 1)) *
+                         ((k > 1 ? 17e3 : 12e3) + (double)((tiles + k - 1) / k) * 8.4 * hd);
+        if (*cluster == 0 || t < *time) {
+            *time = t;
+            *cluster = k;
+        }
+    }
+    return CN_OK;
+}
+
+int kvq4_attend_prompt(cn_ctx* ctx, int hd, int cluster, AttendArgs a, cudaStream_t st) {
     using namespace pr;
-    const int64_t rows = (int64_t)a.n_new * (a.n_heads / a.n_kv), items = kvq4_prompt_items(rows, a.n_kv, a.batch);
+    const int64_t rows = (int64_t)a.n_new * (a.n_heads / a.n_kv), items = prompt_items(rows, a.n_kv, a.batch);
     CN_CHECK(items < (1ll << 31) / kMaxCluster, CN_ERR_INVALID_ARG, "too many rows (%lld items)", (long long)items);
     a.groups = (int)((rows + kRows - 1) / kRows);
-    const int cluster = kvq4_prompt_cluster(ctx, items, a.ctx_len);
-    using Fn = void (*)(AttendArgs);
-    const Fn fn = hd == 64 ? (Fn)kvq4_attend_prompt_kernel<64> : (Fn)kvq4_attend_prompt_kernel<128>;
-    const int smem = hd == 64 ? Geo<64>::kSmem : Geo<128>::kSmem;
-    const uint32_t bit = 1u << (hd == 64 ? 24 : 25);
-    if (!(__atomic_load_n(&ctx->kvq4_ready, __ATOMIC_RELAXED) & bit)) {
-        CN_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        __atomic_fetch_or(&ctx->kvq4_ready, bit, __ATOMIC_RELAXED);
-    }
-    CN_CUDA(launch_cluster_k(false, cluster, fn, dim3((unsigned)(items * cluster)), dim3(kThreads), (size_t)smem, st, a));
+    CN_CUDA(launch_cluster_k(false, cluster, prompt_fn(hd), dim3((unsigned)(items * cluster)), dim3(kThreads),
+                             (size_t)prompt_smem(hd), st, a));
     return CN_OK;
 }
 

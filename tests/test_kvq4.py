@@ -319,7 +319,7 @@ def test_attend(ctx, hd, kv, mul, ctx_len, n_new, pos, count, rope, neox):
     _check_attend(ctx, box, len(pos), mul * kv, n_new, pos, count, table, neox, gen)
 
 
-PROMPTS = [  # sizes at which rows go 128 to a CTA, in clusters of 1 (the first four), 2, 2, 4, 8, 8
+PROMPTS = [  # sizes at which rows go 128 to a CTA: single CTAs (the first four), then clusters
     (128, 8, 8, 512, 64, [0, 1, 63, 448], None, True, False),
     (128, 4, 3, 512, 171, [0, 300, 341, -1, 511, 7, 600, 64], [171, 171, 170, 9, 171, 1, 171, 0], True, True),
     (64, 4, 8, 512, 100, [0, 412, 63, 65], None, True, False),
@@ -532,6 +532,29 @@ def test_prompts_on_streams_and_in_graphs(ctx):
         graphs[1].replay()
         torch.cuda.synchronize()
         verify(box, q, outs[3], heads, n_new, lower, None, None, False, hd ** -0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,n_new", FORMS)
+def test_a_contexts_first_call_is_captured(batch, n_new):
+    gen = _gen(20)
+    box = Box(batch, 4, 64, 512)
+    for b in range(batch):
+        box.fill(b, 512, gen)
+    q = torch.randn(batch, n_new, 16 * 64, generator=gen, device="cuda")
+    out = torch.full_like(q, 7.5)
+    pos = [100] * batch
+    p = _ints(pos)
+    torch.cuda.synchronize()
+    with cn.Context(0) as fresh:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            fresh.kvq4_attend_dev(box.cache, q.data_ptr(), out.data_ptr(), p.data_ptr(), batch, 16, n_new=n_new,
+                                  stream=torch.cuda.current_stream().cuda_stream)
+        g.replay()
+        torch.cuda.synchronize()
+        verify(box, q, out, 16, n_new, pos, None, None, False, 0.125)
+        g.reset()
 
 
 @pytest.mark.gpu
