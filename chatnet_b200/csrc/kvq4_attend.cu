@@ -103,12 +103,11 @@ __device__ __forceinline__ uint32_t pair16(const uint32_t* a, int i, const uint3
 //
 // Scores: S = Q K^T on mma.m16n8k16, the eight rows' high halves in the
 // tile's rows 0-7 and their low halves in rows 8-15 (q scaled to [2^14, 2^15)
-// by a power of two: 22 bits).  K's levels go in as fp16 subnormals, level *
-// 2^-24 straight from the nibble (every second nibble as 16 * level, with q
-// divided by 16 there), so a fragment costs one AND per two values; the
-// -8 of a value is added as -8 sum(q) and the block's scale multiplies the
-// block's sum in fp32.  The high halves are whole multiples of 16, so that their
-// products with a block's levels add up exactly.
+// by a power of two, each entry's halves with 11 bits of its own, so that small
+// entries next to a large one keep 22 too).  K's levels go in signed, exact in fp16,
+// two instructions for two values: as the bare nibbles they would take one, but then
+// -8 sum(q) has to be taken off again, whose rounding drowns the small entries beside
+// a large one.  The block's scale multiplies the block's sum in fp32.
 // Output: O = W V with V's signed levels exact in fp16 and w_p d_p,b (weight
 // times the block's scale) as two halves: w's halves hi, lo times the fp16 d
 // give h = hi d rounded, then its exact rounding error and lo d in the second
@@ -121,7 +120,7 @@ __device__ __forceinline__ uint32_t pair16(const uint32_t* a, int i, const uint3
 //
 // Bound: instruction issue and the latency of the MMAs between (about 690 warp
 // instructions for 32 positions; the loads alone run at the copy rate).  8 sequences
-// of 131 thousand positions, 64 heads over 8 of 128: 300 us, 3.15 TB/s; 32 sequences
+// of 131 thousand positions, 64 heads over 8 of 128: 312 us, 3.03 TB/s; 32 sequences
 // to 1001 positions, 32 kv heads: 57 us, 2 TB/s; one of 512, 4 kv heads of 64: 6.2 us.
 template <int NB>
 __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows_kernel(const AttendArgs a) {
@@ -181,7 +180,6 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
     // the rows' queries as A fragments in shared memory (every warp needs a
     // row's maximum, block j is left by warp j % kWarps); limit = last position
     // the row sees
-    float2 bias[NB];
     float factor;
     int limit;
     {
@@ -203,34 +201,22 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         float sc, inv;
         row_pow2_scale(amax, sc, inv);
-        factor = fmaxf(a.scale * 1.44269504088896341f * 16777216.f * inv, FLT_MIN);  // (not 0: -inf is a masked score)
+        factor = fmaxf(a.scale * 1.44269504088896341f * inv, FLT_MIN);  // (not 0: -inf is a masked score)
 #pragma unroll
         for (int j = 0; j < NB; j++) {
-            float sum_hi = 0.f, sum_lo = 0.f;
+            if (j % kWarps != warp) continue;
             uint32_t qa[8];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float m = (i & 1) ? 0.0625f : 1.f;
                 const float x0 = v[j][i].x * sc, x1 = v[j][i].y * sc;
-                const float h0 = rintf(x0 * 0.0625f) * 16.f, h1 = rintf(x1 * 0.0625f) * 16.f;
-                const uint32_t hi = pack_half2(h0 * m, h1 * m), lo = pack_half2((x0 - h0) * m, (x1 - h1) * m);
-                const float2 lf = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-                sum_hi += h0 + h1;
-                sum_lo += (lf.x + lf.y) * ((i & 1) ? 16.f : 1.f);
+                const uint32_t hi = pack_half2(x0, x1);
+                const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&hi));
                 // a0 / a1: high and low halves of k 2t, 2t+1; a2 / a3: of k 2t+8, 2t+9
                 qa[4 * (i >> 1) + 2 * (i & 1)] = hi;
-                qa[4 * (i >> 1) + 2 * (i & 1) + 1] = lo;
+                qa[4 * (i >> 1) + 2 * (i & 1) + 1] = pack_half2(x0 - hf.x, x1 - hf.y);
             }
-            if (j % kWarps == warp) {
-                qs[64 * j + lane] = make_uint4(qa[0], qa[1], qa[2], qa[3]);
-                qs[64 * j + 32 + lane] = make_uint4(qa[4], qa[5], qa[6], qa[7]);
-            }
-#pragma unroll
-            for (int k = 1; k <= 2; k <<= 1) {
-                sum_hi += __shfl_xor_sync(0xffffffffu, sum_hi, k);
-                sum_lo += __shfl_xor_sync(0xffffffffu, sum_lo, k);
-            }
-            bias[j].x = bias[j].y = (sum_hi + sum_lo) * (-8.f / 16777216.f);
+            qs[64 * j + lane] = make_uint4(qa[0], qa[1], qa[2], qa[3]);
+            qs[64 * j + 32 + lane] = make_uint4(qa[4], qa[5], qa[6], qa[7]);
         }
     }
 
@@ -295,16 +281,15 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
                 for (int nt = 0; nt < NT; nt++) {
                     const uint32_t x = pair16(w[nt], j, w[nt], NB + j);
                     c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.f;
-                    mma(c[nt], a0, x & 0x000F000Fu, x & 0x00F000F0u, c[nt]);
+                    mma(c[nt], a0, even_levels(x), odd_levels(x), c[nt]);
                     y[nt] = x >> 8;
                 }
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) mma(c[nt], a1, y[nt] & 0x000F000Fu, y[nt] & 0x00F000F0u, c[nt]);
+                for (int nt = 0; nt < NT; nt++) mma(c[nt], a1, even_levels(y[nt]), odd_levels(y[nt]), c[nt]);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                     const float2 d = reinterpret_cast<const float2*>(fs)[(4 * nt + t) * NB + j];
-                    p[nt] = fma2(d, add2(make_float2(c[nt][0], c[nt][1]), add2(make_float2(c[nt][2], c[nt][3]), bias[j])),
-                                 p[nt]);
+                    p[nt] = fma2(d, add2(make_float2(c[nt][0], c[nt][1]), make_float2(c[nt][2], c[nt][3])), p[nt]);
                 }
             }
         }
@@ -434,15 +419,8 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
                     x1 = pair16(w + 2, jj, w + 3, jj);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        uint32_t b0, b1;
-                        if (i & 1) {  // 1024 + 16 level -> level - 8
-                            b0 = h2_fma(lop3_and_or(x0, 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u);
-                            b1 = h2_fma(lop3_and_or(x1, 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u);
-                        } else {  // 1024 + level -> level - 8
-                            b0 = h2_sub(lop3_and_or(x0, 0x000F000Fu, 0x64006400u), 0x64086408u);
-                            b1 = h2_sub(lop3_and_or(x1, 0x000F000Fu, 0x64006400u), 0x64086408u);
-                        }
-                        mma(c[jj][i], af, b0, b1, c[jj][i]);
+                        if (i & 1) mma(c[jj][i], af, odd_levels(x0), odd_levels(x1), c[jj][i]);
+                        else mma(c[jj][i], af, even_levels(x0), even_levels(x1), c[jj][i]);
                         if (i == 1) {
                             x0 >>= 8;
                             x1 >>= 8;

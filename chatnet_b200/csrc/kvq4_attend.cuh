@@ -64,6 +64,13 @@ __device__ __forceinline__ uint32_t h2_fms(uint32_t a, uint32_t b, uint32_t c) {
     asm("{\n\t.reg .b32 n;\n\tneg.f16x2 n, %3;\n\tfma.rn.f16x2 %0, %1, %2, n;\n\t}" : "=r"(r) : "r"(a), "r"(b), "r"(c));
     return r;
 }
+// Nibbles 0 / 1 of both halves of x as level - 8, exactly (1024 + level, 1024 + 16 level).
+__device__ __forceinline__ uint32_t even_levels(uint32_t x) {
+    return h2_sub(lop3_and_or(x, 0x000F000Fu, 0x64006400u), 0x64086408u);
+}
+__device__ __forceinline__ uint32_t odd_levels(uint32_t x) {
+    return h2_fma(lop3_and_or(x, 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u);
+}
 __device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));

@@ -148,8 +148,7 @@ __host__ __device__ constexpr uint32_t idesc(int n) {
 // Nibble i of both halves of x as level - 8, times d: hi + lo exactly.
 __device__ __forceinline__ void expand(uint32_t x, int i, uint32_t d, uint32_t& hi, uint32_t& lo) {
     const uint32_t y = i >= 2 ? x >> 8 : x;
-    const uint32_t v = (i & 1) ? h2_fma(lop3_and_or(y, 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u)
-                               : h2_sub(lop3_and_or(y, 0x000F000Fu, 0x64006400u), 0x64086408u);
+    const uint32_t v = (i & 1) ? odd_levels(y) : even_levels(y);
     hi = h2_mul(v, d);
     lo = h2_fms(v, d, hi);
 }
