@@ -17,8 +17,6 @@ namespace cn {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr float kPeak = 9.f;     // a weight is 2^9 at the row's reference
-constexpr float kLazy = 4.f;     // a row's reference moves only when the maximum outgrows it by 2^4
 constexpr int kMaxCluster = 16;
 
 // positions of a warp's tile, bytes of a tile in the ring (quants and scales of K and V)
@@ -102,8 +100,8 @@ __device__ __forceinline__ uint32_t pair16(const uint32_t* a, int i, const uint3
 // launch.
 //
 // Scores: S = Q K^T on mma.m16n8k16, the eight rows' high halves in the
-// tile's rows 0-7 and their low halves in rows 8-15 (q scaled to [2^14, 2^15)
-// by a power of two, each entry's halves with 11 bits of its own, so that small
+// tile's rows 0-7 and their low halves in rows 8-15 (q scaled to [2^13, 2^15]
+// as for score_factor, each entry's halves with 11 bits of its own, so that small
 // entries next to a large one keep 22 too).  K's levels go in signed, exact in fp16,
 // two instructions for two values: as the bare nibbles they would take one, but then
 // -8 sum(q) has to be taken off again, whose rounding drowns the small entries beside
@@ -112,8 +110,8 @@ __device__ __forceinline__ uint32_t pair16(const uint32_t* a, int i, const uint3
 // times the block's scale) as two halves: w's halves hi, lo times the fp16 d
 // give h = hi d rounded, then its exact rounding error and lo d in the second
 // half, all in packed fp16 (three instructions for two positions).  A row's
-// weights are 2^9 at its reference (log2 units), a running maximum that moves when
-// outgrown by 2^4, and V's scales count 2^e times where the largest seen
+// weights are 2^9 at its reference (a running maximum in log2 units, moved when
+// outgrown by 2^4), and V's scales count 2^e times where the largest seen
 // lies outside [2^-7, 4), so w d stays below 2^15 and keeps 22 bits down to 2^-25
 // of that, whatever the cache's range.  Each tile's products are summed from
 // zero and joined in fp32 (the tensor cores truncate where fp32 rounds).
@@ -201,7 +199,8 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         float sc, inv;
         row_pow2_scale(amax, sc, inv);
-        factor = fmaxf(a.scale * 1.44269504088896341f * inv, FLT_MIN);  // (not 0: -inf is a masked score)
+        factor = score_factor(inv, a.exp);
+        sc *= a.mant;
 #pragma unroll
         for (int j = 0; j < NB; j++) {
             if (j % kWarps != warp) continue;
@@ -223,7 +222,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
     float2 o[4 * NB];
 #pragma unroll
     for (int j = 0; j < 4 * NB; j++) o[j] = make_float2(0.f, 0.f);
-    float R = -1e30f;
+    float R = -FLT_MAX;
     float2 l2 = make_float2(0.f, 0.f);
     uint32_t dtop = 0;  // bound of the |V scale| seen, fp16 bits
     int e2 = 0;         // V's scales count 2^e2 times
@@ -321,7 +320,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
                 }
             }
             mx = max(mx & 0xFFFFu, mx >> 16);
-            if (__any_sync(0xffffffffu, top > R + (kPeak + kLazy) || mx > dtop)) {
+            if (__any_sync(0xffffffffu, top - R > kPeak + kLazy || mx > dtop)) {
                 float grow = 1.f;
                 mx = __reduce_max_sync(0xffffffffu, mx);
                 if (mx > dtop) {
@@ -335,9 +334,10 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 float al = 1.f;
-                if (top > R + (kPeak + kLazy)) {  // R: the score at which a weight is 1
-                    al = ex2(R - (top - kPeak));
-                    R = top - kPeak;
+                if (top - R > kPeak + kLazy) {
+                    const float to = reference(top);
+                    al = ex2(R - to);
+                    R = to;
                 }
                 l2.x *= al;
                 l2.y *= al;
@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows
     const uint32_t aR = smem_u32(&sR[kWarps][0]), aL = smem_u32(&sL[kWarps][0]), aO = smem_u32(sc);
     for (int e = (int)rank * 32 * kWarps + threadIdx.x; e < min(rows, 8) * (HD / 4); e += (int)cs * 32 * kWarps) {
         const int r = e / (HD / 4);
-        float M = -1e30f;
+        float M = -FLT_MAX;
         for (uint32_t c = 0; c < cs; c++) M = fmaxf(M, ld_cluster(aR + 4 * r, c));
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         float ls = 0.f;
@@ -565,7 +565,7 @@ int kvq4_attend(cn_ctx* ctx, const cn_kvq4& c, const float* q, int64_t q_stride,
     a.n_kv = c.n_kv_heads;
     a.ctx_len = c.ctx_len;
     a.neox = neox;
-    a.scale = scale;
+    a.mant = (float)frexp((double)scale * 1.4426950408889634, &a.exp);
     a.err = ctx->dev_err;
     const int64_t rows = (int64_t)n_new * (n_heads / c.n_kv_heads);
     const int64_t groups = (rows + 7) / 8, items = groups * c.n_kv_heads * batch;

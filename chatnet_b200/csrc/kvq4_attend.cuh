@@ -2,6 +2,8 @@
 // (kvq4_attend.cu: few rows; kvq4_prompt.cu: many).
 #pragma once
 
+#include <float.h>
+
 #include "kvq4.cuh"
 
 namespace cn {
@@ -17,9 +19,28 @@ struct AttendArgs {
     const __half *kd, *vd;
     int64_t seq_rows;
     int batch, n_new, n_heads, n_kv, ctx_len, neox, groups;
-    float scale;
+    float mant;  // the scores' scale in log2 units, scale * log2(e) = mant * 2^exp, mant in [1/2, 1]
+    int exp;
     uint32_t* err;
 };
+
+constexpr float kPeak = 9.f;  // the heaviest weight is 2^9 when a row's reference is set
+constexpr float kLazy = 4.f;  // and the reference moves when a weight would pass 2^(9 + 4)
+
+// What a row's sums count in log2 units, for queries times s * mant with s = 1 / inv
+// a power of two: a power of two as well, so that sum * factor is exact and a
+// score - R as exact as a subtraction, at any size.  Not 0 (-inf is a masked score), nor
+// above 2^84: the sums lie below 2^43, so no score overflows, and scores that this takes
+// down are still 0 or far more than a weight's whole range apart.
+__device__ __forceinline__ float score_factor(float inv, int exp) {
+    return fminf(fmaxf(scalbnf(inv, exp), FLT_MIN), 0x1p84f);
+}
+// The reference R for a maximum (a weight is 2^(score - R)); the maximum itself where
+// scores are 16 apart and more, since one less 9 may come out as one less 16.
+__device__ __forceinline__ float reference(float top) {
+    const float r = top - kPeak;
+    return top - r > 12.f ? top : r;
+}
 
 // Many rows: items of 128, head dimensions kvq4_prompt_ok.
 bool kvq4_prompt_ok(int hd);

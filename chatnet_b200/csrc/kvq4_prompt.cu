@@ -51,7 +51,6 @@ constexpr int kStages = 3;     // expanded tiles
 // are after the output of tile - kBufs, its scales' range after that of
 // tile - kRaw - kStages - kBufs = tile - 10.
 constexpr int kSlots = 8, kUndo = 16;
-constexpr float kPeak = 9.f, kLazy = 4.f;
 constexpr int kMaxCluster = 8;
 
 template <int HD>
@@ -485,7 +484,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
             asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
             float o[HD];
             {
-                // first the row's query: rotated, scaled to [2^14, 2^15), in K's order
+                // first the row's query: rotated, scaled to [2^13, 2^15], in K's order
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 const uint8_t* x = smem + G::kQOff + min(r, rows - 1) * G::kPitch;
@@ -521,8 +520,8 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
 #pragma unroll
                 for (int e = 0; e < HD; e++) amax = fmaxf(amax, fabsf(o[e]));
                 row_pow2_scale(amax, sc, inv);
-                // what a score counts, for the weights' warps (not 0: -inf is a masked score)
-                mR[r] = fmaxf(a.scale * 1.44269504088896341f * inv, FLT_MIN);
+                mR[r] = score_factor(inv, a.exp);  // for the weights' warps
+                sc *= a.mant;
 #pragma unroll
                 for (int c = 0; c < HD / 32; c++) {  // 32 dimensions: four pieces of 8
                     uint32_t hi[16], lo[16];
@@ -609,7 +608,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
         } else {
             // ---- weights ----
             asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
-            float R = -1e30f, l = 0.f;
+            float R = -FLT_MAX, l = 0.f;
             const int limit = p0 + tok;
             wait(q_full, 0);
             const float factor = mR[r];
@@ -638,8 +637,8 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
 #pragma unroll
                 for (int e = 0; e < 32; e++) top = fmaxf(top, x[e]), top2 = fmaxf(top2, x[32 + e]);
                 top = fmaxf(top, top2);
-                if (top * f > R + (kPeak + kLazy)) {
-                    const float to = top * f - kPeak;
+                if (top * f - R > kPeak + kLazy) {
+                    const float to = reference(top * f);
                     move = ex2(R - to);
                     R = to;
                 }
@@ -685,7 +684,7 @@ __global__ void __launch_bounds__(pr::kThreads, 1) kvq4_attend_prompt_kernel(con
         const uint32_t aO = smem_u32(smem), aR = smem_u32(mR), aL = smem_u32(mL);
         for (int e = (int)rank * kThreads + threadIdx.x; e < rows * (HD / 4); e += (int)cs * kThreads) {
             const int r = e / (HD / 4), at = r * G::kPitch + 16 * (e % (HD / 4)), rr = r0 + r;
-            float M = -1e30f, ls = 0.f;
+            float M = -FLT_MAX, ls = 0.f;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             for (uint32_t c = 0; c < cs; c++) M = fmaxf(M, ld_cluster(aR + 4 * r, c));
             for (uint32_t c = 0; c < cs; c++) {

@@ -286,7 +286,7 @@ int cn_kvq4_append_dev(cn_ctx* ctx, const cn_kvq4* cache, const float* d_k, cons
  * Softmax, LlamaModel.cs:241-346).  q (rotated first when d_rope is given) and
  * out: n_heads * head_dim fp32 values per token, strides multiples of 4, not
  * overlapping, 16-byte aligned.  fp32 results (products of q and of the softmax
- * weights carry 22 bits, sums 24). */
+ * weights carry 22 bits, sums 24), for scores of any size that fp32 holds. */
 int cn_kvq4_attend_dev(cn_ctx* ctx, const cn_kvq4* cache, const float* d_q, int64_t q_stride, float* d_out,
                        int64_t out_stride, const int* d_pos, const int* d_count, int batch, int n_new, int n_heads,
                        float scale, const float* d_rope, int rope_neox, void* stream);

@@ -9,7 +9,10 @@ exponential by 8 u more, and against that of the heaviest position m the weight 
 exp(+-(e_p + e_m + 16 u)).  That moves an output by at most
     sum_(p != m) (exp(ln w_p + e_p + e_m + 16 u) - w_p) |v_p - o| / max(w_m, sum w_p exp(-(e_p + e_m + 16 u)));
 weights times V's scales are carried to 2^-22, and sums (of weights, and of products) run over at most 64 positions
-of a tile and then over the tiles: (2^-21 + 2 (136 + positions / 32) u) sum w_p |v_p| more.
+of a tile and then over the tiles: (2^-21 + 2 (136 + positions / 32) u) sum w_p |v_p| more.  That is where the halves
+are normal numbers.  Below, they end at 2^-24, where the heaviest weight is 2^9 or more: each of a weight's two halves is
+off by 2^-25, times |v|; and where the weight is multiplied by V's scale (in 2^-7 .. 4 here) first, so are the product's
+two roundings, times levels of up to 8: positions * w_m (2^-33 max |v| + 2^-30) more.
 """
 from __future__ import annotations
 
@@ -40,12 +43,13 @@ def attend_bound(q, k, v, pos, scale):
         e = e + 2.0 ** -39 * x.abs().amax(-1, keepdim=True) * scale * kk.abs().sum(-1)[None] + 8 * U
         m = logw.argmax(-1, keepdim=True)
         e = (e + e.gather(1, m)).scatter(1, m, 0.0)
-        more = (torch.exp(logw + e) - w).masked_fill(hidden, 0.0)
+        more = (torch.exp((logw + e).clamp(max=0.0)) - w).masked_fill(hidden, 0.0)  # (no weight passes 1)
         least = torch.maximum(w.gather(1, m), (w * torch.exp(-e)).sum(-1, keepdim=True))
         sums = 2.0 ** -21 + 2 * (136 + seen / 32) * U
         for i in range(n):
             off = (vv - out[i, h]).abs()
             tol[i, h] = (more[i] / least[i]) @ off + sums * (w[i] @ vv.abs())
+        tol[:, h] += seen * w.gather(1, m) * (2.0 ** -33 * float(vv.abs().max()) + 2.0 ** -30)
     return out, tol
 
 
@@ -61,13 +65,15 @@ def _rows(shape, gen, ratio=0.0, border=False):
     return x
 
 
-def _cache_values(shape, gen, hole):
-    """K and V rows as (levels, scales); with `hole`, K's entry 5 is 0."""
+def _cache_values(shape, gen, hole, above=False):
+    """K and V rows as (levels, scales); with `hole`, K's entry 5 is 0, and with `above` no value of K is below 0."""
     made = []
     for w in "kv":
         x = torch.randn(*shape, generator=gen, device=gen.device) * 1.5
         if hole and w == "k":
             x[..., 5] = 0.0
+        if above and w == "k":
+            x = x.abs()
         made.append(ref.quantize(x))
     return made
 
@@ -118,14 +124,14 @@ def test_the_bound_tells_lost_bits(hd):
 # ---- GPU -------------------------------------------------------------------------------------------------------------
 
 
-def check(ctx, hd, kv, mul, ctx_len, n_new, pos, gen, q, hole=False, scale=None):
+def check(ctx, hd, kv, mul, ctx_len, n_new, pos, gen, q, hole=False, scale=None, above=False):
     """An attention over a fresh cache against the bound; returns the worst error as a part of it."""
-    scale = hd ** -0.5 if scale is None else scale
+    scale = float(torch.tensor(hd ** -0.5 if scale is None else scale))  # (fp32)
     batch, heads = len(pos), kv * mul
     box = Box(batch, kv, hd, ctx_len)
     for b, p in enumerate(pos):
         n = p + n_new
-        for w, (lv, d) in zip("kv", _cache_values((kv, n, hd), gen, hole)):
+        for w, (lv, d) in zip("kv", _cache_values((kv, n, hd), gen, hole, above)):
             box.q[w][0][b, :, :n] = ref.pack(lv)
             box.q[w][1][b, :, :n] = d
     out = torch.full((batch, n_new, heads * hd), 7.5, device="cuda")
@@ -140,7 +146,7 @@ def check(ctx, hd, kv, mul, ctx_len, n_new, pos, gen, q, hole=False, scale=None)
                                  box.values("v", b)[:, :pos[b] + n_new], pos[b], scale)
         err = (out[b].double().view(n_new, heads, hd) - want).abs()
         assert not err.isnan().any()
-        worst = max(worst, float((err / tol).max()))
+        worst = max(worst, float((err / (tol + 1e-300)).max()))  # (0 / 0: no error)
     return worst
 
 
@@ -168,3 +174,22 @@ def test_queries_with_one_large_entry(ctx, form, ratio, border):
     gen = _gen(31)
     q = _rows((len(pos), n_new, kv * mul, hd), gen, ratio, border).flatten(2)
     assert check(ctx, hd, kv, mul, ctx_len, n_new, pos, gen, q, hole=True) <= 1
+
+
+LARGE = [(30.0, None), (1e4, None), (1e6, None), (1e8, None), (3e8, None), (3e9, None), (1e20, None), (1e31, None),
+         (1e36, None), (1.0, 1e35), (1e-3, 3e38), (1e20, 1e16), (1e36, 1e-38), (1e-38, 1e36)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("signs", ["mixed", "below"])
+@pytest.mark.parametrize("qmul,scale", LARGE)
+@pytest.mark.parametrize("form", FORMS[::2] + FORMS[-1:])
+def test_large_scores(ctx, form, qmul, scale, signs):
+    """Scores up to 1e37 of either sign, and rows with none above -1e31 or so: the heaviest position's values."""
+    hd, kv, mul, ctx_len, n_new, pos = form
+    gen = _gen(32)
+    q = _rows((len(pos), n_new, kv * mul, hd), gen).flatten(2) * qmul
+    assert q.isfinite().all()
+    if signs == "below":
+        q = -q.abs()
+    assert check(ctx, hd, kv, mul, ctx_len, n_new, pos, gen, q, scale=scale, above=signs == "below") <= 1
