@@ -72,11 +72,11 @@ class GgufFile:
         check(N.lib().cn_gguf_get_string(self.handle, key.encode(), C.byref(v)), "cn_gguf_get_string")
         return v.value.decode()
 
-    def llama_config(self, max_batch: int = 1, kv_f16: bool = False) -> LlamaConfig:
+    def llama_config(self, max_batch: int = 1, kv_f16: bool = False, kv_q4: bool = False) -> LlamaConfig:
         c = N.LlamaConfigC()
         check(N.lib().cn_gguf_llama_config(self.handle, C.byref(c)), "cn_gguf_llama_config")
         return LlamaConfig(c.dim, c.hidden_dim, c.n_layers, c.n_heads, c.n_kv_heads, c.head_dim, c.vocab,
-                           c.ctx_len, c.rope_base, c.rms_eps, kv_f16, max_batch)
+                           c.ctx_len, c.rope_base, c.rms_eps, kv_f16, max_batch, kv_q4=kv_q4)
 
     def upload(self, ctx, name: str):
         from . import Tensor
@@ -86,16 +86,18 @@ class GgufFile:
         rows, cols = info.shape
         return ctx._own(Tensor(ctx, h.value, info.type, rows, cols))
 
-    def llama_model(self, ctx, max_batch: int = 1, kv_f16: bool = False, tp=None) -> CudaLlamaModel:
+    def llama_model(self, ctx, max_batch: int = 1, kv_f16: bool = False, tp=None,
+                    kv_q4: bool = False) -> CudaLlamaModel:
         """The whole decoder from this file (cn_llama_create_from_gguf), or,
         with a connected TensorParallel group, this rank's shards of it
-        (cn_llama_create_from_gguf_tp)."""
+        (cn_llama_create_from_gguf_tp).  Its KV cache is fp32, with kv_f16
+        fp16, with kv_q4 (which comes first) 4-bit."""
         from . import Tensor
-        cfg = self.llama_config(max_batch, kv_f16)
+        cfg = self.llama_config(max_batch, kv_f16, kv_q4)
         n = 3 + 9 * cfg.n_layers
         arr = (C.c_void_p * n)()
         h = C.c_void_p()
-        kv = N.KV_F16 if kv_f16 else N.KV_F32
+        kv = cfg.to_c().kv_dtype
         if tp is None:
             check(N.lib().cn_llama_create_from_gguf(ctx.handle, self.handle, max_batch, kv, C.byref(h), arr, n),
                   "cn_llama_create_from_gguf")
