@@ -121,6 +121,34 @@ def test_the_bound_tells_lost_bits(hd):
     assert worst("row", 1e4, True) > 2 and worst("row", 1e5, True) > 2
 
 
+def _low_half_dropped(x):
+    """64-bit values with 11 bits left, cut off as the high halves are."""
+    m, e = torch.frexp(x)
+    return torch.ldexp(torch.trunc(m * 2048) / 2048, e)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("lost", ["weights", "values"])
+def test_the_bound_tells_lost_bits_of_weights_and_values(hd, lost):
+    """On mild queries, whose scores are off by little, it tells weights or V's values without their low halves."""
+    gen = torch.Generator().manual_seed(hd + 1)
+    (lk, dk), (lv, dv) = _cache_values((2, 40, hd), gen, False)
+    k, v = ref.values(ref.pack(lk), dk), ref.values(ref.pack(lv), dv)
+    q = _rows((8, 4, hd), gen).double() * 0.1
+    want, tol = attend_bound(q, k, v, 20, hd ** -0.5)
+    got = torch.empty_like(want)
+    for h in range(4):
+        for i in range(8):
+            x = k[h // 2, :21 + i] @ q[i, h] * hd ** -0.5
+            w, y = torch.exp(x - x.max()), v[h // 2, :21 + i]
+            if lost == "weights":
+                w, total = _low_half_dropped(w), w.sum()  # (the sum is taken before)
+            else:
+                y, total = y.half().double(), w.sum()
+            got[i, h] = w @ y / total
+    assert float(((got - want).abs() / tol).max()) > 2
+
+
 # ---- GPU -------------------------------------------------------------------------------------------------------------
 
 
@@ -174,6 +202,16 @@ def test_queries_with_one_large_entry(ctx, form, ratio, border):
     gen = _gen(31)
     q = _rows((len(pos), n_new, kv * mul, hd), gen, ratio, border).flatten(2)
     assert check(ctx, hd, kv, mul, ctx_len, n_new, pos, gen, q, hole=True) <= 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qmul", [0.1, 1.0])
+@pytest.mark.parametrize("form", FORMS)
+def test_ordinary_queries(ctx, form, qmul):
+    hd, kv, mul, ctx_len, n_new, pos = form
+    gen = _gen(33)
+    q = _rows((len(pos), n_new, kv * mul, hd), gen).flatten(2) * qmul
+    assert check(ctx, hd, kv, mul, ctx_len, n_new, pos, gen, q) <= 1
 
 
 LARGE = [(30.0, None), (1e4, None), (1e6, None), (1e8, None), (3e8, None), (3e9, None), (1e20, None), (1e31, None),
