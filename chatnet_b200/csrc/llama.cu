@@ -736,18 +736,18 @@ static int prefill_layers(cn_llama* m, int n, int pos) {
     return CN_OK;
 }
 
-// Kernels one prefill_layers call launches: 6 per layer besides the matmuls (7
-// with a 4-bit cache),
-// and one matmul per same-type run of each projection group (4 per layer
-// when every group's types agree).
+// Kernels one prefill_layers call launches: one matmul per same-type run of
+// each projection group (4 per layer when every group's types agree), and 6 per layer
+// besides.  With a 4-bit cache the call also stores its position once; with the other
+// caches rotation and attention make it 5 per layer, of which this count is one above.
 static int prefill_kernels(const cn_llama* m) {
     cn_llama* mm = const_cast<cn_llama*>(m);
     const int64_t r[3] = {0, 0, 0};
     float* y[3] = {nullptr, nullptr, nullptr};
-    int k = 0, ns[4];
+    int k = kv_q4(m) ? 1 : 0, ns[4];
     split_counts(m, ns);
     for (int l = 0; l < m->cfg.n_layers; l++)
-        k += (kv_q4(m) ? 7 : 6) + mm_group(mm, l, 3, kSlotsQKV, r, 0, 0, y, r, false, false, true, ns[0]) +
+        k += 6 + mm_group(mm, l, 3, kSlotsQKV, r, 0, 0, y, r, false, false, true, ns[0]) +
              mm_group(mm, l, 1, kSlotsO, r, 0, 0, y, r, false, false, true, ns[1]) +
              mm_group(mm, l, 2, kSlotsGU, r, 0, 0, y, r, false, false, true, ns[2]) +
              mm_group(mm, l, 1, kSlotsDown, r, 0, 0, y, r, false, false, true, ns[3]);

@@ -1,5 +1,7 @@
-"""Scores of texts that run as one prefill pass, on a 4-bit and an fp32 KV cache."""
+"""Scores of texts that run as one prefill pass, on a 4-bit and an fp32 KV cache, and the launches of such a pass."""
 from __future__ import annotations
+
+import ctypes as C
 
 import numpy as np
 import pytest
@@ -60,3 +62,32 @@ def test_entropies_are_optional(build):  # noqa: F811
         assert N.lib().cn_llama_score(g.handle, toks.ctypes.data, 60, 0, lp.ctypes.data, None) == 0
         np.testing.assert_array_equal(lp[:59], want)
         assert lp[59] == 7.5
+
+
+def kernel_nodes(graph):
+    cu = C.CDLL("libcuda.so.1")
+    h, n = C.c_void_p(graph.raw_cuda_graph()), C.c_size_t(0)
+    assert cu.cuGraphGetNodes(h, None, C.byref(n)) == 0
+    nodes = (C.c_void_p * n.value)()
+    assert cu.cuGraphGetNodes(h, nodes, C.byref(n)) == 0
+    kinds = []
+    for v in nodes:
+        k = C.c_int(-1)
+        assert cu.cuGraphNodeGetType(C.c_void_p(v), C.byref(k)) == 0
+        kinds.append(k.value)
+    return kinds.count(0)  # CU_GRAPH_NODE_TYPE_KERNEL
+
+
+def test_kernels_of_a_prefill_pass(ctx, build):  # noqa: F811
+    dc = q4_dc(ctx_len=100)
+    g, _ = build(dc)
+    x = torch.randn(40, dc.model.dim, device="cuda")
+    out = torch.empty_like(x)
+    torch.cuda.synchronize()
+    g.prefill_hidden_dev(x.data_ptr(), 40, 0, out.data_ptr())  # (the first pass makes its buffers)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph, stream=torch.cuda.ExternalStream(ctx.stream)):
+        g.prefill_hidden_dev(x.data_ptr(), 40, 0, out.data_ptr())
+    assert kernel_nodes(graph) == g.prefill_kernels()
+    graph.reset()
