@@ -271,6 +271,8 @@ int kvq4_check(const cn_ctx* ctx, const cn_kvq4* c, int batch, int n_new) {
     CN_CHECK(c->n_seqs >= 1 && c->n_kv_heads >= 1 && c->ctx_len >= 1, CN_ERR_INVALID_ARG,
              "4-bit cache: bad shape (%d sequences, %d heads, %d positions)", c->n_seqs, c->n_kv_heads, c->ctx_len);
     CN_CHECK(c->ctx_len % 8 == 0, CN_ERR_INVALID_ARG, "4-bit cache: ctx_len %d is not a multiple of 8", c->ctx_len);
+    // (the end of the last tile, and of what a cluster steps past it, stays below 2^31)
+    CN_CHECK(c->ctx_len <= 1 << 30, CN_ERR_INVALID_ARG, "4-bit cache: ctx_len %d is above 2^30", c->ctx_len);
     const int64_t rows = (int64_t)c->n_kv_heads * c->ctx_len;
     CN_CHECK(c->seq_rows == 0 || (c->seq_rows >= rows && c->seq_rows % 8 == 0), CN_ERR_INVALID_ARG,
              "4-bit cache: seq_rows %lld is below %lld or not a multiple of 8", (long long)c->seq_rows,

@@ -268,7 +268,7 @@ typedef struct {
     void* v_scales;
     int n_seqs, n_kv_heads;
     int head_dim;     /* 32, 64, 96, 128 or 256 */
-    int ctx_len;      /* positions per sequence, a multiple of 8 */
+    int ctx_len;      /* positions per sequence, a multiple of 8 up to 2^30 */
     int64_t seq_rows; /* rows between two sequences (a multiple of 8); 0: n_kv_heads * ctx_len */
 } cn_kvq4;
 
