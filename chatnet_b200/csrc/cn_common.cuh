@@ -214,6 +214,12 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// the larger of two, NaN if one is
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 // two fp32 operations in one instruction
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     uint64_t r;
