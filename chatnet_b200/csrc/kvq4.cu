@@ -27,11 +27,6 @@ __device__ __forceinline__ float min_nan(float a, float b) {
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
 
 constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: whole numbers from here on
 
@@ -86,10 +81,11 @@ struct RowAt {
 // loads and stores): the nibbles i = l >> 1 of chunks g = 4 (l & 1) .. + 3.  A
 // word holds two 16-bit pieces; the four lanes of one parity OR their nibbles
 // together, and lane l then writes chunk 4 (l & 1) + (l >> 1).  The fp32 rows'
-// bytes would bound it (reading them alone: 49 us for the case below); with about
-// 500 instructions per 16 values, rotation included, issue does.  8191 tokens of 32
-// heads of 128: 132 us, 4.35 TB/s (149 with rows side by side for many tokens too and
-// the exact level for every value).
+// bytes would bound it (48 us for the case below); with about 500 instructions per 16
+// values for rotation, scale, levels and packing, issue does (80 % of the slots; without
+// the rotation 76 us).  8191 tokens of 32 heads of 128: 80 us, 3.9 TB/s; followed by
+// reading them back 132, and 149 with rows side by side for many tokens too and the
+// exact level for every value.
 template <int NB>
 __global__ void __launch_bounds__(kRowThreads)
     kvq4_append_kernel(const float* __restrict__ k, const float* __restrict__ v, int64_t kv_stride,
@@ -211,6 +207,8 @@ __global__ void __launch_bounds__(kRowThreads)
     if (l < NB) ((is_v ? vd : kd) + dst * NB)[l] = __float2half_rn(scale);
 }
 
+// Eight lanes a row, lane l the values 4l .. 4l + 3 of every block.  Bound by the bytes,
+// most of them written: 8191 tokens of 32 heads of 128 take 61 us, 5.0 TB/s.
 template <int NB>
 __global__ void __launch_bounds__(kRowThreads)
     kvq4_read_kernel(float* __restrict__ k, float* __restrict__ v, int64_t kv_stride, const int* __restrict__ pos,

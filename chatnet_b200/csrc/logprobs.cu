@@ -19,10 +19,12 @@
 // lists meet in the first CTA's shared memory.  No workspace, no atomics on
 // global memory, one launch.
 //
-// 4096 rows of 32000 fp32: 87 us, 6.0 TB/s (0.93 of a copy's rate).  300 rows of
-// 131071 fp16 with 8 alternatives: 39 us, 2.0 TB/s, bound by the instructions of twice
-// the values a byte.  Few rows are bound by the choice among the candidates, about
-// 5 us: one row of 32000 with 5 takes 7 us, 32 with 20 10.6.
+// 4096 rows of 32000 fp32: 88 us, 5.9 TB/s (0.92 of a copy's rate).  300 rows of
+// 131071 fp16 with 8 alternatives: 40 us, 2.0 TB/s, bound by latency: one CTA a row is two
+// CTAs on most SMs and three on four, sixteen warps whose loads, conversions and
+// exponentials follow one another (43 % of the issue slots, 24 % of DRAM's rate).  Few rows
+// are bound by the choice among the candidates, about 5 us: one row of 32000 with 5 takes
+// 9 us, 32 with 20 11.
 #include <float.h>
 
 #include "cn_common.cuh"
@@ -64,12 +66,6 @@ __device__ __forceinline__ float order_value(uint32_t o) {
     return o == 0u ? NAN : __uint_as_float((o & 0x80000000u) ? o & 0x7FFFFFFFu : ~o);
 }
 constexpr uint32_t kMinusInf = 0x007FFFFFu, kZero = 0x80000000u;  // order32 of -inf and 0
-
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
 
 // 16 bytes of logits as floats
 template <typename T>
