@@ -116,10 +116,14 @@ __device__ __forceinline__ uint32_t pair16(const uint32_t* a, int i, const uint3
 // of that, whatever the cache's range.  Each tile's products are summed from
 // zero and joined in fp32 (the tensor cores truncate where fp32 rounds).
 //
-// Bound: instruction issue and the latency of the MMAs between (about 690 warp
-// instructions for 32 positions; the loads alone run at the copy rate).  8 sequences
-// of 131 thousand positions, 64 heads over 8 of 128: 312 us, 3.03 TB/s; 32 sequences
-// to 1001 positions, 32 kv heads: 57 us, 2 TB/s; one of 512, 4 kv heads of 64: 6.2 us.
+// Bound: latency.  168 registers a thread let three CTAs on an SM, and its twelve warps
+// (ten active) wait for one MMA's or conversion's result after the other: at 32 thousand
+// positions 46 % of the issue slots are used and 31 % of DRAM's rate (the loads alone run
+// at the copy rate).  Short sequences pay each CTA's set-up, first loads and two merges
+// besides (16 at 2047: 31 % of the slots), and with one query head to a kv head 14 of the
+// 16 rows of every MMA are empty.  8 sequences of 131 thousand positions, 64 heads over 8
+// of 128: 314 us, 3.0 TB/s; 16 to 2047: 19.3 us; 32 to 1001, 32 kv heads: 57 us, 2 TB/s;
+// one of 512, 4 kv heads of 64: 6.2 us.
 template <int NB>
 __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NB)) kvq4_attend_rows_kernel(const AttendArgs a) {
     constexpr int HD = 32 * NB, RB = 16 * NB, SB = 2 * NB;  // bytes of a row's quants and scales
@@ -573,8 +577,9 @@ int kvq4_attend(cn_ctx* ctx, const cn_kvq4& c, const float* q, int64_t q_stride,
     const int nb = c.head_dim / 32;
     const int64_t room = (int64_t)ctx->sms * ctas_per_sm(nb);
     if (kvq4_prompt_ok(c.head_dim)) {
-        // Which kernel: both as measured over the cache's length (the positions are
-        // on the device).  Here: 6 us for each round of CTAs and 23 positions of 128
+        // Which kernel: by both kernels' times over the cache's length, as the positions
+        // are on the device; all figures are of full caches, and near the start of a long
+        // one the other kernel may be the faster.  Here: 6 us for each round of CTAs and 23 positions of 128
         // values a ns.  One sequence, 64 heads over 8 of 128, 8 x tokens rows, here /
         // there: at 2000 positions 64 rows 16 / 20 us, 192 rows 27 / 24; at 16000 64
         // rows 53 / 49, 96 rows 73 / 50, 192 rows 136 / 84.  Four sequences of 32

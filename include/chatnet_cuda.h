@@ -286,7 +286,9 @@ int cn_kvq4_append_dev(cn_ctx* ctx, const cn_kvq4* cache, const float* d_k, cons
  * Softmax, LlamaModel.cs:241-346).  q (rotated first when d_rope is given) and
  * out: n_heads * head_dim fp32 values per token, strides multiples of 4, not
  * overlapping, 16-byte aligned.  fp32 results (products of q and of the softmax
- * weights carry 22 bits, sums 24), for scores of any size that fp32 holds. */
+ * weights carry 22 bits, sums 24), for scores of any size that fp32 holds; blocks
+ * of V whose scale is below 2^-15 of the largest that the sequence's head holds, and
+ * blocks of K below 2^-22 of it, may keep fewer bits. */
 int cn_kvq4_attend_dev(cn_ctx* ctx, const cn_kvq4* cache, const float* d_q, int64_t q_stride, float* d_out,
                        int64_t out_stride, const int* d_pos, const int* d_count, int batch, int n_new, int n_heads,
                        float scale, const float* d_rope, int rope_neox, void* stream);
@@ -305,8 +307,9 @@ int cn_kvq4_read_dev(cn_ctx* ctx, const cn_kvq4* cache, float* d_k, float* d_v, 
  * outside [0, vocab) gets NaN.  -inf logits (banned tokens) have probability
  * 0; a row that holds a NaN or +inf, or nothing but -inf, has no distribution:
  * its results are NaN (its alternatives still in order, NaN last).  vocab is
- * below 2^30, row_stride below 2^40.  Enqueues on `stream` only, allocates nothing, keeps nothing between calls.  (no
- * reference counterpart: TemperatureSampler discards its probabilities,
+ * below 2^30, row_stride below 2^40.  Enqueues on `stream` only, allocates
+ * nothing, keeps nothing between calls.  (no reference counterpart:
+ * TemperatureSampler discards its probabilities,
  * Samplers/TemperatureSampler.cs:33-113) */
 int cn_logprobs_dev(cn_ctx* ctx, int type, const void* d_logits, int64_t row_stride, int rows, int vocab,
                     const int* d_tokens, int top_n, float* d_logprob, float* d_entropy, int* d_top_ids,
