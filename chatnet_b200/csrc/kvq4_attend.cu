@@ -579,10 +579,10 @@ int kvq4_attend(cn_ctx* ctx, const cn_kvq4& c, const float* q, int64_t q_stride,
     if (kvq4_prompt_ok(c.head_dim)) {
         // Which kernel: by both kernels' times over the cache's length, as the positions
         // are on the device; all figures are of full caches, and near the start of a long
-        // one the other kernel may be the faster.  Here: 6 us for each round of CTAs and 23 positions of 128
-        // values a ns.  One sequence, 64 heads over 8 of 128, 8 x tokens rows, here /
-        // there: at 2000 positions 64 rows 16 / 20 us, 192 rows 27 / 24; at 16000 64
-        // rows 53 / 49, 96 rows 73 / 50, 192 rows 136 / 84.  Four sequences of 32
+        // one the other kernel may be the faster.  Here: 6 us for each round of CTAs and 23
+        // positions of 128 values a ns.  One sequence, 64 heads over 8 of 128, 8 x tokens
+        // rows, here / there: at 2000 positions 64 rows 16 / 20 us, 192 rows 27 / 24; at
+        // 16000 64 rows 53 / 49, 96 rows 73 / 50, 192 rows 136 / 84.  Four sequences of 32
         // heads, 64 rows: at 100 29 / 16, at 2000 100 / 50, at 16000 540 / 287.
         int k, rc;
         double there = 0;
