@@ -21,9 +21,9 @@
 // other is computed.  What it took, 64 query heads over 8 of hd 128, 1111 tokens at
 // position 6000: 508 us at 1965 MHz, 470 TFLOP/s of the formula's 4 hd a pair, three
 // times that as multiplied; call after call the power cap takes the clock to 1620 MHz,
-// and it is 586 us, 407 TFLOP/s.  Other forms, at 1965 MHz: MMAs issued by a thread by itself, 84 cycles each: 831.  So with Q
-// in shared memory and wide MMAs, fewer to issue: 641.  P in shared memory: 982.
-// Weights by eight warps on alternate tiles: 547.
+// and it is 586 us, 407 TFLOP/s.  Other forms, at 1965 MHz: MMAs issued by a thread by
+// itself, 84 cycles each: 831.  So with Q in shared memory and wide MMAs, fewer to issue:
+// 641.  P in shared memory: 982.  Weights by eight warps on alternate tiles: 547.
 // A CTA's first output comes 16600 cycles after its start, most of them the first
 // pass through code that is in no instruction cache yet, and writing it takes 4000:
 // 512 tokens at 0 (32 heads) take 24 us, of which their eight tiles are 9.
